@@ -5,6 +5,7 @@ nothing here falls back to PyTorch or to the CPU oracle.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import os
 from typing import Optional
@@ -34,7 +35,7 @@ _i32 = C.c_int32
 _f = C.c_float
 _int = C.c_int
 
-# name -> argument types (all functions return int)
+# name -> argument types (all functions return int, those of _SIZES a 64-bit size)
 SIGNATURES = {
     "bg_zero_bytes": [_p, _i64, _p],
     "bg_copy2d_bytes": [_p, _i64, _p, _i64, _i64, _i64, _p],
@@ -44,6 +45,15 @@ SIGNATURES = {
     "bg_plan_floor_level": [_p, _p, _i64, _i64, _p, _p, _p],
     "bg_plan_counts": [_p, _i64, _p, _p],
     "bg_plan_chunks": [_p, _i64, _i32, _p, _p],
+    "bg_embedding_fwd": [_int, _p, _i64, _i64, _p, _int, _i64, _i64, _f, _p, _i64, _p],
+    "bg_embedding_bwd": [_int, _p, _i64, _p, _int, _i64, _i64, _i64, _f, _p, _p, _i64, _p],
+    "bg_embedding_bwd_workspace": [_i64] * 3,
+    "bg_gated_scan_heads": [_i64] * 2,
+    "bg_gated_scan_workspace": [_i64] * 2,
+    "bg_gated_scan_fwd": [_int, _p, _i64, _p, _i64, _p, _i64, _i64, _i64, _p, _int, _p, _i64, _p, _p, _p, _i64, _p],
+    "bg_gated_scan_bwd": [_int, _p, _i64, _p, _i64, _p, _i64, _p, _p, _i64, _i64, _i64, _p, _int, _p, _p, _i64, _p, _i64, _p, _p,
+                          _i64, _p],
+    "bg_gated_scan_step": [_int, _p, _i64, _p, _i64, _p, _i64, _i64, _i64, _p, _i64, _p, _i64, _p],
     "bg_spmm_f32": [_p, _i64, _p, _p, _p, _p, _p, _int, _p, _int, _p, _i64, _i64, _i64, _p],
     "bg_connectivity": [_p, _i64, _p, _p, _i64, _p, _i64, _i64, _p, _p, _i64, _p, _i64, _p, _i64, _p, _p],
     "bg_program_ratio_f32": [_p, _p, _p, _i64, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _p],
@@ -137,6 +147,7 @@ SIGNATURES = {
     "bg_plan_build": [_p, _p, _p, _p],
 }
 
+_SIZES = ("bg_embedding_bwd_workspace", "bg_gated_scan_heads", "bg_gated_scan_workspace")
 _fp = C.c_void_p      # device pointers travel as integers
 BG_OK, BG_ERR_ARG, BG_ERR_SHAPE, BG_ERR_ALIGN, BG_ERR_LAUNCH, BG_ERR_SCRATCH = 0, -1, -2, -3, -4, -5      # include/bgan.h
 
@@ -209,6 +220,8 @@ def load() -> C.CDLL:
         fn = getattr(lib, name)
         fn.argtypes = argtypes
         fn.restype = C.c_int
+    for name in _SIZES:
+        getattr(lib, name).restype = C.c_int64
     lib.bg_version.restype = C.c_int
     lib.bg_generator_forward_workspace.restype = C.c_int64
     lib.bg_generator_forward_workspace.argtypes = [_i64] * 5
@@ -268,6 +281,17 @@ def stream() -> int:
     if _raw_stream is not None and _get_device is not None:
         return _raw_stream(_get_device())
     return torch.cuda.current_stream().cuda_stream
+
+
+def on_device(t: torch.Tensor):
+    """Context in which launches and allocations go to ``t``'s device (and to its current stream), whichever device is the
+    current one: nothing to do -- and nothing paid -- where they are the same."""
+    if t.device.index == (_get_device() if _get_device is not None else torch.cuda.current_device()):
+        return _HERE_ALREADY
+    return torch.cuda.device(t.device)
+
+
+_HERE_ALREADY = contextlib.nullcontext()
 
 
 def require_device(t: torch.Tensor, what: str) -> None:

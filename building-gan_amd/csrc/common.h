@@ -128,3 +128,31 @@ __device__ __forceinline__ float bg_tanh(float x) {
 __device__ __forceinline__ float4 bg_scale4(float s, float4 a) {
     return make_float4(s * a.x, s * a.y, s * a.z, s * a.w);
 }
+
+// ---- element types of the operators that take more than fp32 (BG_F32 / BG_F16 / BG_BF16, include/bgan.h).  Arithmetic is
+// fp32 throughout; a result is rounded to the element type once, to nearest even, where it is stored.
+typedef _Float16 bg_half;
+typedef __bf16 bg_bf16;
+template <class T, int N>
+struct alignas(sizeof(T) * N) BgVec { T v[N]; };
+
+// Round an fp32 value that also lives on as fp32.  The empty statement keeps the compiler from folding the conversion into
+// the fma that made the value (v_fma_mixlo_f16 rounds the exact result): two kernels that agree in fp32 agree in T.
+template <class T>
+__device__ __forceinline__ T bg_round(float x) {
+    asm("" : "+v"(x));
+    return (T)x;
+}
+
+static inline int bg_elem_size(int dtype) { return dtype == BG_F32 ? 4 : (dtype == BG_F16 || dtype == BG_BF16) ? 2 : 0; }
+
+// one instantiation of `body` (a generic lambda taking a value of the element type) for the run-time type code
+template <class F>
+static inline int bg_dispatch_dtype(int dtype, F&& body) {
+    switch (dtype) {
+        case BG_F32: return body(float(0));
+        case BG_F16: return body(bg_half(0));
+        case BG_BF16: return body(bg_bf16(0));
+    }
+    return BG_ERR_ARG;
+}

@@ -913,6 +913,269 @@ class GatherArg(torch.autograd.Function):
         return ScatterArg.apply(g, arg, ctx.n_rows, ctx.seg_of), None, None
 
 
+# ------------------------------------------------------------------------------- table lookup
+_ELEM = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}      # include/bgan.h: BG_F32, BG_F16, BG_BF16
+
+
+def _elem(t: torch.Tensor, what: str) -> int:
+    code = _ELEM.get(t.dtype)
+    if code is None:
+        raise _lib.BganError(f"{what}: element type {t.dtype} is not one of float32, float16, bfloat16")
+    return code
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """A matrix with unit inner stride and a row pitch of at least its width (t itself where it has them)."""
+    if (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
+        return t.contiguous()
+    return t
+
+
+def _token_ids(ids: torch.Tensor, like: torch.Tensor, what: str) -> torch.Tensor:
+    if ids.dtype not in (torch.int64, torch.int32):
+        raise _lib.BganError(f"{what}: ids must be int64 or int32, got {ids.dtype}")
+    if ids.device != like.device:
+        raise _lib.BganError(f"{what}: ids on {ids.device}, rows on {like.device}")
+    return ids.reshape(-1).contiguous()
+
+
+def embedding_raw(weight: torch.Tensor, ids: torch.Tensor, scale: float = 1.0) -> torch.Tensor:
+    """``scale * weight[ids]`` [*ids.shape, D], zero rows where an id is outside [0, V) (bg_embedding_fwd: one launch)."""
+    lib = _lib.load()
+    _lib.require_device(weight, "embedding")
+    if weight.dim() != 2:
+        raise _lib.BganError(f"embedding: weight must be [V, D], got {tuple(weight.shape)}")
+    code, w, i = _elem(weight, "embedding"), _rows(weight), _token_ids(ids, weight, "embedding")
+    V, D = w.shape
+    with _lib.on_device(w):
+        out = torch.empty(i.numel(), D, dtype=w.dtype, device=w.device)
+        check(lib.bg_embedding_fwd(code, ptr(w), _ld(w), V, ptr(i), i.dtype == torch.int64, i.numel(), D, scale, ptr(out), D,
+                                   stream()), "bg_embedding_fwd")
+    return out.view(*ids.shape, D)
+
+
+def embedding_grad_raw(g: torch.Tensor, ids: torch.Tensor, n_rows: int, scale: float = 1.0) -> torch.Tensor:
+    """``dw[v] = scale * sum of g's rows whose id is v`` [n_rows, D], in g's type: the lookup's gradient, bit-reproducible
+    (bg_embedding_bwd: ids sorted, fp32 sums in a fixed order)."""
+    lib = _lib.load()
+    _lib.require_device(g, "embedding_grad")
+    code, i = _elem(g, "embedding_grad"), _token_ids(ids, g, "embedding_grad")
+    if g.dim() != ids.dim() + 1 or g.shape[:-1] != ids.shape:
+        raise _lib.BganError(f"embedding_grad: rows {tuple(g.shape)} do not belong to ids {tuple(ids.shape)}")
+    if n_rows < 0:
+        raise _lib.BganError("embedding_grad: n_rows must not be negative")
+    D = g.shape[-1]
+    g2 = _rows(g.reshape(i.numel(), D))
+    with _lib.on_device(g):
+        dw = torch.empty(n_rows, D, dtype=g.dtype, device=g.device)
+        size = lib.bg_embedding_bwd_workspace(i.numel(), n_rows, D)
+        ws = torch.empty(size, dtype=torch.uint8, device=g.device) if size else None
+        check(lib.bg_embedding_bwd(code, ptr(g2), _ld(g2), ptr(i), i.dtype == torch.int64, i.numel(), D, n_rows, scale, ptr(dw),
+                                   ptr(ws), size, stream()), "bg_embedding_bwd")
+    return dw
+
+
+class Embedding(torch.autograd.Function):
+    """y = scale * weight[ids]; the backward is EmbeddingGrad (both are linear, so the pair is closed)."""
+
+    @staticmethod
+    def forward(ctx, weight, ids, scale: float):
+        ctx.save_for_backward(ids)
+        ctx.n_rows, ctx.scale = weight.shape[0], scale
+        return embedding_raw(weight, ids, scale)
+
+    @staticmethod
+    def backward(ctx, g):
+        (ids,) = ctx.saved_tensors
+        return EmbeddingGrad.apply(g, ids, ctx.n_rows, ctx.scale), None, None
+
+
+class EmbeddingGrad(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, g, ids, n_rows: int, scale: float):
+        ctx.save_for_backward(ids)
+        ctx.scale = scale
+        return embedding_grad_raw(g, ids, n_rows, scale)
+
+    @staticmethod
+    def backward(ctx, gg):
+        (ids,) = ctx.saved_tensors
+        return Embedding.apply(gg, ids, ctx.scale), None, None, None
+
+
+def embedding(weight: torch.Tensor, ids: torch.Tensor, scale: float = 1.0, validate: bool = False) -> torch.Tensor:
+    """Rows of a learned table: ``scale * weight[ids]``, shape [*ids.shape, D], in the table's type (float32, float16,
+    bfloat16; int64 or int32 ids).  A categorical node feature (program class, floor level) as a vector without the
+    one-hot matrix of Model/models.py:84; its gradient sums each row's terms in fp32 in a fixed order.
+
+    An id outside [0, V) is a missing token: a zero row that takes no part in the gradient.  ``validate=True`` reads the
+    ids back (one synchronisation) and raises IndexError on any id outside [0, V) instead."""
+    if validate and ids.numel():
+        lo, hi = (int(v) for v in torch.stack(torch.aminmax(ids)).tolist())
+        if lo < 0 or hi >= weight.shape[0]:
+            raise IndexError(f"embedding: ids span [{lo}, {hi}], the table has {weight.shape[0]} rows")
+    if torch.is_grad_enabled() and weight.requires_grad:
+        return Embedding.apply(weight, ids, float(scale))
+    return embedding_raw(weight, ids, float(scale))
+
+
+# ------------------------------------------------------------------------------- scan along segments
+def _scan_operands(x, gate, rowptr, h0, what):
+    """(type code, x, gate, row pointer, segments) as bg_gated_scan_* take them; BganError for what they do not take."""
+    _lib.require_device(x, what)
+    code = _elem(x, what)
+    if x.dim() != 2 or gate.shape != x.shape:
+        raise _lib.BganError(f"{what}: x and gate must be [rows, D] alike, got {tuple(x.shape)} and {tuple(gate.shape)}")
+    if gate.dtype != x.dtype or gate.device != x.device:
+        raise _lib.BganError(f"{what}: gate is {gate.dtype} on {gate.device}, x is {x.dtype} on {x.device}")
+    if isinstance(rowptr, torch.Tensor):
+        if rowptr.dtype != torch.int32 or rowptr.dim() != 1 or rowptr.numel() < 1 or rowptr.device != x.device:
+            raise _lib.BganError(f"{what}: rowptr must be int32 [segments + 1] on {x.device}")
+        rowptr = rowptr.contiguous()
+        n_seg = rowptr.numel() - 1
+    else:                                        # a number of segments of equal length
+        rowptr, n_seg = None, rowptr
+        if n_seg < 0 or (x.shape[0] % n_seg if n_seg else x.shape[0]):
+            raise _lib.BganError(f"{what}: {x.shape[0]} rows are not {n_seg} segments of equal length")
+    if h0 is not None and (h0.dtype != torch.float32 or h0.device != x.device or tuple(h0.shape) != (n_seg, x.shape[1])):
+        raise _lib.BganError(f"{what}: h0 must be float32 [{n_seg}, {x.shape[1]}] on {x.device}, got {h0.dtype} {tuple(h0.shape)}")
+    return code, _rows(x), _rows(gate), rowptr, n_seg
+
+
+def gated_scan_raw(x, gate, rowptr, h0=None, reverse: bool = False, keep_heads: bool = False):
+    """(h, h_last, heads) of ``gated_scan`` on [rows, D] operands (bg_gated_scan_fwd); ``rowptr`` is the segments' int32 row
+    pointer or, for segments of equal length, their number; ``heads`` (None unless kept) is what the backward pass takes."""
+    lib = _lib.load()
+    code, x2, g2, rp, n_seg = _scan_operands(x, gate, rowptr, h0, "gated_scan")
+    N, D = x2.shape
+    h0c = None if h0 is None else h0.contiguous()
+    dev = x.device
+    with _lib.on_device(x):
+        h = torch.empty(N, D, dtype=x.dtype, device=dev)
+        h_last = torch.empty(n_seg, D, dtype=torch.float32, device=dev)
+        heads = torch.empty(lib.bg_gated_scan_heads(N, D), dtype=torch.float32, device=dev) if keep_heads else None
+        size = lib.bg_gated_scan_workspace(N, D)
+        ws = torch.empty(size, dtype=torch.uint8, device=dev)
+        check(lib.bg_gated_scan_fwd(code, ptr(x2), _ld(x2), ptr(g2), _ld(g2), ptr(rp), n_seg, N, D, ptr(h0c), reverse, ptr(h),
+                                    max(D, 1), ptr(h_last), ptr(heads), ptr(ws), size, stream()), "bg_gated_scan_fwd")
+    return h, h_last, heads
+
+
+def gated_scan_grad_raw(x, gate, rowptr, h0, reverse: bool, heads, dh, dlast, need_dh0: bool = True):
+    """(dx, dgate, dh0) from the gradients of h (``dh``, may be None) and h_last (``dlast``, may be None)
+    (bg_gated_scan_bwd); ``heads`` is the forward call's."""
+    lib = _lib.load()
+    code, x2, g2, rp, n_seg = _scan_operands(x, gate, rowptr, h0, "gated_scan_grad")
+    N, D = x2.shape
+    if dh is not None and (dh.dtype != x.dtype or dh.shape != x.shape or dh.device != x.device):
+        raise _lib.BganError("gated_scan_grad: dh must be like x")
+    if dlast is not None and (dlast.dtype != torch.float32 or tuple(dlast.shape) != (n_seg, D) or dlast.device != x.device):
+        raise _lib.BganError(f"gated_scan_grad: dlast must be float32 [{n_seg}, {D}]")
+    if heads.numel() != lib.bg_gated_scan_heads(N, D) or heads.dtype != torch.float32:
+        raise _lib.BganError("gated_scan_grad: heads are not a forward call's over these rows")
+    d2 = None if dh is None else _rows(dh)
+    dl = None if dlast is None else dlast.contiguous()
+    h0c = None if h0 is None else h0.contiguous()
+    dev = x.device
+    with _lib.on_device(x):
+        dx = torch.empty(N, D, dtype=x.dtype, device=dev)
+        dgate = torch.empty(N, D, dtype=x.dtype, device=dev)
+        dh0 = torch.empty(n_seg, D, dtype=torch.float32, device=dev) if need_dh0 else None
+        size = lib.bg_gated_scan_workspace(N, D)
+        ws = torch.empty(size, dtype=torch.uint8, device=dev)
+        check(lib.bg_gated_scan_bwd(code, ptr(x2), _ld(x2), ptr(g2), _ld(g2), ptr(d2), _ld(d2) if d2 is not None else 0, ptr(dl),
+                                    ptr(rp), n_seg, N, D, ptr(h0c), reverse, ptr(heads), ptr(dx), max(D, 1), ptr(dgate), max(D, 1),
+                                    ptr(dh0), ptr(ws), size, stream()), "bg_gated_scan_bwd")
+    return dx, dgate, dh0
+
+
+class GatedScan(torch.autograd.Function):
+    """(h, h_last) of gated_scan on [rows, D] operands (first-order autograd only)."""
+
+    @staticmethod
+    def forward(ctx, x, gate, h0, rowptr, reverse: bool):
+        h, h_last, heads = gated_scan_raw(x, gate, rowptr, h0, reverse, keep_heads=True)
+        ctx.reverse = reverse
+        ctx.n_seg = None if isinstance(rowptr, torch.Tensor) else rowptr
+        ctx.save_for_backward(x, gate, h0, rowptr if ctx.n_seg is None else None, heads)
+        ctx.set_materialize_grads(False)
+        return h, h_last
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dh, dlast):
+        x, gate, h0, rowptr, heads = ctx.saved_tensors
+        if dh is None and dlast is None:
+            return None, None, None, None, None
+        dx, dgate, dh0 = gated_scan_grad_raw(x, gate, rowptr if ctx.n_seg is None else ctx.n_seg, h0, ctx.reverse, heads, dh, dlast,
+                                             need_dh0=ctx.needs_input_grad[2])
+        return dx, dgate, dh0, None, None
+
+
+def gated_scan(x: torch.Tensor, gate: torch.Tensor, rowptr: Optional[torch.Tensor] = None, h0: Optional[torch.Tensor] = None,
+               reverse: bool = False):
+    """State carried along the rows of each segment: with ``a = sigmoid(gate)``, per column,
+    ``h_t = a_t h_{t-1} + (1 - a_t) x_t``; returns (h, h_last).
+
+    ``x``, ``gate``: [rows, D] (float32, float16, bfloat16; a row pitch is taken, so the halves of one projection need no
+    copy) with the segments' int32 row pointer ``rowptr`` [S + 1] (``Csr.rowptr`` of a plan's story or graph segments), one
+    segment of all rows without it; or [B, T, D], B segments of T rows.  ``h0`` [S, D] float32 is the state before a
+    segment's first row (default zero), ``h_last`` [S, D] float32 the one after its last; a segment without rows passes
+    its state through.  Rows in no segment are zero in ``h`` and in the gradients.  ``reverse`` walks every segment from
+    its last row to its first.  The state is carried in fp32 and ``h`` rounded once; results are bit-reproducible."""
+    shape = x.shape
+    if x.dim() == 3:
+        if rowptr is not None:
+            raise _lib.BganError("gated_scan: rowptr goes with [rows, D] operands, not with [B, T, D]")
+        if gate.shape != shape:
+            raise _lib.BganError(f"gated_scan: x and gate must be alike, got {tuple(shape)} and {tuple(gate.shape)}")
+        x, gate, rowptr = x.flatten(0, 1), gate.flatten(0, 1), shape[0]
+        if shape[1] == 0:                        # (segments without rows: a row pointer of zeros says how many)
+            rowptr = torch.zeros(shape[0] + 1, dtype=torch.int32, device=x.device)
+    elif rowptr is None:
+        rowptr = 1 if x.dim() == 2 and x.shape[0] else torch.zeros(2, dtype=torch.int32, device=x.device)
+    if torch.is_grad_enabled() and (x.requires_grad or gate.requires_grad or (h0 is not None and h0.requires_grad)):
+        h, h_last = GatedScan.apply(x, gate, h0, rowptr, bool(reverse))
+    else:
+        h, h_last, _ = gated_scan_raw(x, gate, rowptr, h0, bool(reverse))
+    return h.view(shape), h_last
+
+
+def _shifted_overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two float32 matrices overlap in memory without holding every element at the same address."""
+    if a.numel() == 0 or (a.data_ptr() == b.data_ptr() and a.stride() == b.stride()):
+        return False
+    lo, hi = zip(*((t.data_ptr(), t.data_ptr() + 4 * sum((n - 1) * s for n, s in zip(t.shape, t.stride()))) for t in (a, b)))
+    return lo[0] <= hi[1] and lo[1] <= hi[0]
+
+
+def gated_scan_step(x: torch.Tensor, gate: torch.Tensor, state: torch.Tensor, state_out: Optional[torch.Tensor] = None):
+    """One row for each of n segments whose states are kept between calls: (h [n, D] in x's type, state' [n, D] float32)
+    with ``state' = a state + (1 - a) x``; ``state_out=state`` updates the states in place (bg_gated_scan_step, no
+    autograd)."""
+    lib = _lib.load()
+    _lib.require_device(x, "gated_scan_step")
+    code = _elem(x, "gated_scan_step")
+    if x.dim() != 2 or gate.shape != x.shape or gate.dtype != x.dtype or gate.device != x.device:
+        raise _lib.BganError("gated_scan_step: x and gate must be [n, D] of one type")
+    if state.shape != x.shape or state.dtype != torch.float32 or state.device != x.device:
+        raise _lib.BganError(f"gated_scan_step: state must be float32 {tuple(x.shape)} on {x.device}")
+    n, D = x.shape
+    x2, g2, s2 = _rows(x), _rows(gate), _rows(state)
+    with _lib.on_device(x):
+        h = torch.empty(n, D, dtype=x.dtype, device=x.device)
+        if state_out is None:
+            state_out = torch.empty(n, D, dtype=torch.float32, device=x.device)
+        elif (state_out.shape != x.shape or state_out.dtype != torch.float32 or state_out.device != x.device
+              or _rows(state_out) is not state_out):
+            raise _lib.BganError(f"gated_scan_step: state_out must be float32 {tuple(x.shape)} with contiguous rows on {x.device}")
+        elif _shifted_overlap(state_out, state):
+            raise _lib.BganError("gated_scan_step: state_out shares memory with state without being the same rows")
+        check(lib.bg_gated_scan_step(code, ptr(x2), _ld(x2), ptr(g2), _ld(g2), ptr(s2), _ld(s2), n, D, ptr(h), max(D, 1),
+                                     ptr(state_out), _ld(state_out), stream()), "bg_gated_scan_step")
+    return h, state_out
+
+
 # ------------------------------------------------------------------------------- attention ops
 class CrossLogits(torch.autograd.Function):
     """att[e] = theta . tanh(a[cev[e]] + b[cep[e]])  (first-order autograd only)."""

@@ -32,6 +32,11 @@ extern "C" {
 #define BG_ERR_LAUNCH (-4)   /* HIP reported a launch / enqueue error                   */
 #define BG_ERR_SCRATCH (-5)  /* request exceeds the library's static scratch buffer     */
 
+/* element types of the entry points that take a `dtype` */
+#define BG_F32 0
+#define BG_F16 1
+#define BG_BF16 2
+
 typedef void* bgStream;
 
 int bg_version(void);
@@ -117,6 +122,60 @@ int bg_plan_layout(const bgPlanIn* in, int64_t* offs_i32, int64_t* offs_f32, int
  * once.  arena_i32 must be 16-byte aligned.
  * replaces: the COO bookkeeping of every torch_scatter / torch_geometric call of a pass (see bg_plan_csr).          */
 int bg_plan_build(const bgPlanIn* in, int32_t* arena_i32, float* arena_f32, bgStream stream);
+
+/* ------------------------------------------------------------------ table lookup -------- */
+
+/* out[i,:] = scale * weight[ids[i],:] for a table weight[V, D] of `dtype` (row pitches in elements); ids are int64
+ * (ids_is_64 != 0) or int32.  An id outside [0, V) is a missing token: its row of `out` is zero.  One fp32 product and
+ * one rounding per element.  Rows are moved in the widest pieces (16 bytes down to one element) that D, the pitches and
+ * the addresses allow.  D <= 2^15, n * D <= 2^33 (BG_ERR_SHAPE).
+ * replaces: one-hot x Linear over a categorical node feature and the position table's gather, Model/models.py:25,84. */
+int bg_embedding_fwd(int dtype, const void* weight, int64_t ldw, int64_t V, const void* ids, int ids_is_64, int64_t n, int64_t D,
+                     float scale, void* out, int64_t ldo, bgStream stream);
+
+/* The lookup's gradient: dw[v,:] = scale * sum over ids[i] == v of g[i,:], every row of dw[V, D] (contiguous, 16-byte
+ * aligned) written, zero where a token does not occur.  Tokens are sorted (stable) and every row's terms are summed in
+ * fp32 in an order that depends on the sizes and ids only, with no floating-point atomics: equal inputs give equal bits.
+ * n <= 2^30, V < 2^31 - 1, D <= 2^15 (BG_ERR_SHAPE).  ws: bg_embedding_bwd_workspace(...) bytes, 16-byte aligned
+ * (BG_ERR_SCRATCH when ws_bytes is less); its contents need no preparation.
+ * replaces: the weight gradient of the Linear over a one-hot feature, Model/models.py:84 under autograd.            */
+int64_t bg_embedding_bwd_workspace(int64_t n, int64_t V, int64_t D);
+int bg_embedding_bwd(int dtype, const void* g, int64_t ldg, const void* ids, int ids_is_64, int64_t n, int64_t D, int64_t V,
+                     float scale, void* dw, void* ws, int64_t ws_bytes, bgStream stream);
+
+/* ------------------------------------------------------------------ scan along segments - */
+
+/* Gated linear recurrence along the rows of each segment [rowptr[s], rowptr[s+1]), per column, with a = sigmoid(gate):
+ *     h_t = a_t h_{t-1} + (1 - a_t) x_t,    h before the first row = h0[s,:] (h0 NULL: zero),
+ * walked from a segment's first row to its last (reverse != 0: from its last to its first).  x, gate, h: [n_rows, D] of
+ * `dtype`, row pitches in elements; h0, h_last: fp32 [n_seg, D], contiguous.  h_last (may be NULL) receives the state
+ * after a segment's rows; a segment without rows passes h0 through.  Rows in no segment (before rowptr[0], from
+ * rowptr[n_seg] on) are zero in h.  rowptr: int32 [n_seg + 1], non-decreasing; entries outside [0, n_rows] are taken as
+ * the nearer end.  rowptr NULL: n_seg segments of n_rows / n_seg rows each.  The state is fp32; h is rounded once.
+ * heads (may be NULL): fp32 [bg_gated_scan_heads(n_rows, D)], the state at the head of every tile of rows, which the
+ * backward pass takes.  ws: bg_gated_scan_workspace(n_rows, D) bytes, 16-byte aligned (BG_ERR_SCRATCH when ws_bytes is
+ * less); it needs no preparation.  x, gate and h in pieces of four elements where D, the pitches and the addresses allow.
+ * n_rows < 2^31, D <= 2^20 (BG_ERR_SHAPE).  Equal inputs give equal bits.
+ * replaces: nothing in the reference, whose only state along a building is the floor level of Model/models.py:22-25.    */
+int64_t bg_gated_scan_heads(int64_t n_rows, int64_t D);
+int64_t bg_gated_scan_workspace(int64_t n_rows, int64_t D);
+int bg_gated_scan_fwd(int dtype, const void* x, int64_t ldx, const void* gate, int64_t ldg, const int32_t* rowptr, int64_t n_seg,
+                      int64_t n_rows, int64_t D, const float* h0, int reverse, void* h, int64_t ldh, float* h_last, float* heads,
+                      void* ws, int64_t ws_bytes, bgStream stream);
+
+/* Its backward pass.  dh (of `dtype`, NULL: zero) and dlast (fp32 [n_seg, D], NULL: zero) are the gradients of h and h_last;
+ * dx, dgate (of `dtype`) and dh0 (fp32 [n_seg, D], may be NULL) receive the inputs' gradients, rows in no segment zero.
+ * h is not an input: it is rebuilt from `heads`, which must be the forward call's for the same x, gate, rowptr, h0 and
+ * reverse.                                                                                                            */
+int bg_gated_scan_bwd(int dtype, const void* x, int64_t ldx, const void* gate, int64_t ldg, const void* dh, int64_t lddh,
+                      const float* dlast, const int32_t* rowptr, int64_t n_seg, int64_t n_rows, int64_t D, const float* h0,
+                      int reverse, const float* heads, void* dx, int64_t lddx, void* dgate, int64_t lddg, float* dh0, void* ws,
+                      int64_t ws_bytes, bgStream stream);
+
+/* One row for each of n segments whose states are kept: state_out = a state + (1 - a) x, h = state_out in `dtype`.
+ * state, state_out: fp32 [n, D] with row pitches; state_out may be state.                                            */
+int bg_gated_scan_step(int dtype, const void* x, int64_t ldx, const void* gate, int64_t ldg, const float* state, int64_t lds, int64_t n,
+                       int64_t D, void* h, int64_t ldh, float* state_out, int64_t ldso, bgStream stream);
 
 /* ------------------------------------------------------------------ segment kernels ----- */
 

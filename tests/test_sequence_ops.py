@@ -1,0 +1,614 @@
+"""Table lookup (ops.embedding) and gated scan (ops.gated_scan, ops.gated_scan_step) against plain float64 loops.
+
+Tolerances.  u = 2^-24 is half a step of fp32, ``half(t)`` half a step of the element type; results are fp32 values rounded
+to the type once.
+ * lookup: one product and one rounding of the scale to fp32 (2 u) and the rounding to the type.
+ * lookup gradient: m terms added in fp32 in some order: m u sum|g|, then the scale (2 u) and the rounding.
+ * a = sigmoid(g) and c = sigmoid(-g) come from exp2 and a reciprocal (1 ulp = 2 u each) with a compensated argument:
+   e within 4 u, 1 / (1 + e) within 5 u, e / (1 + e) within 10 u.  One step of the recurrence adds at most 12 u of
+   a |h| + c |x|, and what a step has wrong decays with the a's behind it: ``err_t = a_t err_{t-1} + 12 u (a |h| + c |x|)``.
+   Joining row groups, tiles and slices of tiles (at most 32 + 32 + tiles / 32 joins, factors at most 1) adds 2 u max|h| each.
+ * the backward recurrence alike, with the sums of |terms| in the place of |h|; dx and dgate multiply a few factors each
+   known to the errors above.
+"""
+import ctypes
+import os
+
+import pytest
+import torch
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+U = 2.0 ** -24
+TYPES = [torch.float32, torch.float16, torch.bfloat16]
+
+
+def half(t):
+    return torch.finfo(t).eps / 2
+
+
+def floor_of(t):
+    return torch.finfo(t).smallest_normal * torch.finfo(t).eps      # a rounding among the subnormal numbers
+
+
+def within(got, want, bound, what):
+    got = got.detach().cpu().double()
+    assert got.shape == want.shape, (what, got.shape, want.shape)
+    bad = ~((got - want).abs() <= bound)
+    assert not bad.any(), "%s: %d of %d beyond the bound, worst %.3g times it" % (
+        what, int(bad.sum()), bad.numel(), float(((got - want).abs() / bound.clamp_min(1e-300)).max()))
+
+
+# ------------------------------------------------------------------------------------------------ refusals (no GPU)
+def test_operands_on_the_cpu_are_refused():
+    from building_gan_amd import _lib, ops
+    w, ids = torch.zeros(4, 8), torch.zeros(3, dtype=torch.int64)
+    for call in (lambda: ops.embedding(w, ids), lambda: ops.embedding_grad_raw(torch.zeros(3, 8), ids, 4),
+                 lambda: ops.gated_scan(w, w), lambda: ops.gated_scan_step(w, w, w),
+                 lambda: ops.embedding(w.clone().requires_grad_(True), ids),
+                 lambda: ops.gated_scan(w.clone().requires_grad_(True), w)):
+        with pytest.raises(_lib.BganError):
+            call()
+    with pytest.raises(IndexError):
+        ops.embedding(w, ids + 4, validate=True)
+    with pytest.raises(IndexError):
+        ops.embedding(w, ids - 1, validate=True)
+
+
+def test_entry_points_refuse_bad_arguments_before_any_launch():
+    """Status codes of the C entry points for what they do not take (no kernel is launched, so no GPU is needed)."""
+    from building_gan_amd import _lib
+    lib = _lib.load()
+    p = 1 << 20                                              # an address that is never read
+    fwd = lambda **k: lib.bg_embedding_fwd(*{**dict(dt=0, w=p, ldw=8, V=4, ids=p, i64=1, n=3, D=8, scale=1.0, out=p, ldo=8, s=None), **k}.values())
+    assert fwd(dt=3) == -1 and fwd(ldw=7) == -1 and fwd(ldo=7) == -1 and fwd(n=-1) == -1 and fwd(w=None) == -1
+    assert fwd(ids=None) == -1 and fwd(out=None) == -1 and fwd(V=-1) == -1
+    assert fwd(D=1 << 16, ldw=1 << 16, ldo=1 << 16) == -2 and fwd(n=1 << 40) == -2
+    assert fwd(n=0) == 0 and fwd(D=0, ldw=0, ldo=0) == 0
+    size = lib.bg_embedding_bwd_workspace(3, 4, 8)
+    assert size > 0 and lib.bg_embedding_bwd_workspace(0, 4, 8) == 0
+    bwd = lambda **k: lib.bg_embedding_bwd(*{**dict(dt=0, g=p, ldg=8, ids=p, i64=1, n=3, D=8, V=4, scale=1.0, dw=p, ws=p, size=size, s=None), **k}.values())
+    assert bwd(dt=-1) == -1 and bwd(ldg=7) == -1 and bwd(dw=None) == -1 and bwd(ws=None) == -1 and bwd(g=None) == -1
+    assert bwd(dw=p + 4) == -3 and bwd(ws=p + 8) == -3 and bwd(size=size - 1) == -5
+    assert bwd(V=(1 << 31) - 1) == -2 and bwd(n=(1 << 30) + 1) == -2 and bwd(D=1 << 16, ldg=1 << 16) == -2
+    assert bwd(V=0) == 0 and bwd(D=0, ldg=0) == 0
+    size = lib.bg_gated_scan_workspace(10, 8)
+    heads = lib.bg_gated_scan_heads(10, 8)
+    assert size > 0 and heads == 8 and lib.bg_gated_scan_workspace(0, 8) == 0
+    scan = lambda **k: lib.bg_gated_scan_fwd(*{**dict(dt=0, x=p, ldx=8, g=p, ldg=8, rp=p, S=2, N=10, D=8, h0=None, rev=0, h=p, ldh=8, hl=p,
+                                                      heads=None, ws=p, size=size, s=None), **k}.values())
+    assert scan(dt=7) == -1 and scan(ldx=7) == -1 and scan(ldg=7) == -1 and scan(ldh=7) == -1 and scan(x=None) == -1
+    assert scan(ws=None) == -1 and scan(ws=p + 8) == -3 and scan(size=size - 1) == -5 and scan(S=-1) == -1
+    assert scan(rp=None, S=3) == -1 and scan(rp=None, S=0) == -1 and scan(N=1 << 31) == -2 and scan(D=1 << 21, ldx=1 << 21, ldg=1 << 21, ldh=1 << 21) == -2
+    assert scan(D=0, ldx=0, ldg=0, ldh=0) == 0 and scan(N=0, hl=None) == 0
+    back = lambda **k: lib.bg_gated_scan_bwd(*{**dict(dt=0, x=p, ldx=8, g=p, ldg=8, dh=p, lddh=8, dl=None, rp=p, S=2, N=10, D=8, h0=None,
+                                                      rev=0, heads=p, dx=p, lddx=8, dg=p, lddg=8, dh0=None, ws=p, size=size, s=None), **k}.values())
+    assert back(lddh=7) == -1 and back(lddx=7) == -1 and back(lddg=7) == -1 and back(heads=None) == -1 and back(dx=None) == -1
+    assert back(size=size - 1) == -5 and back(ws=p + 4) == -3 and back(dt=5) == -1
+    step = lambda **k: lib.bg_gated_scan_step(*{**dict(dt=0, x=p, ldx=8, g=p, ldg=8, st=p, lds=8, n=3, D=8, h=p, ldh=8, so=p, ldso=8, s=None), **k}.values())
+    assert step(st=None) == -1 and step(lds=7) == -1 and step(ldso=7) == -1 and step(n=-1) == -1 and step(n=1 << 30) == -2 and step(n=0) == 0
+
+
+@pytest.mark.gpu
+def test_wrappers_refuse_what_does_not_fit(cuda):
+    from building_gan_amd import _lib, ops
+    w = torch.zeros(4, 8, device=cuda)
+    ids = torch.zeros(3, dtype=torch.int64, device=cuda)
+    rp = torch.tensor([0, 2, 4], dtype=torch.int32, device=cuda)
+    bad = [lambda: ops.embedding(w.double(), ids), lambda: ops.embedding(w[0], ids), lambda: ops.embedding(w, ids.float()),
+           lambda: ops.embedding(w, ids.cpu()), lambda: ops.embedding_grad_raw(torch.zeros(4, 8, device=cuda), ids, 4),
+           lambda: ops.embedding_grad_raw(torch.zeros(3, 8, device=cuda), ids, -1),
+           lambda: ops.gated_scan(w, w.half()), lambda: ops.gated_scan(w, w[:3]), lambda: ops.gated_scan(w, w, rp.long()),
+           lambda: ops.gated_scan(w, w, rp.cpu()), lambda: ops.gated_scan(w, w, rp, h0=torch.zeros(3, 8, device=cuda)),
+           lambda: ops.gated_scan(w, w, rp, h0=torch.zeros(2, 8, device=cuda, dtype=torch.float16)),
+           lambda: ops.gated_scan(w.view(2, 2, 8), w.view(2, 2, 8), rp), lambda: ops.gated_scan(w[0], w[0]),
+           lambda: ops.gated_scan_step(w, w, w.half()), lambda: ops.gated_scan_step(w, w, w[:3]),
+           lambda: ops.gated_scan_step(w, w, w, state_out=w[:3]),
+           lambda: ops.gated_scan_raw(w, w, 3)]
+    for k, call in enumerate(bad):
+        with pytest.raises(_lib.BganError):
+            call()
+            pytest.fail("call %d was accepted" % k)
+    buf = torch.zeros(5, 8, device=cuda)
+    with pytest.raises(_lib.BganError):
+        ops.gated_scan_step(w, w, buf[:4], state_out=buf[1:])
+    with pytest.raises(IndexError):
+        ops.embedding(w, ids + 4, validate=True)
+    assert torch.equal(ops.embedding(w, ids + 3, validate=True), w[ids + 3])
+
+
+# ------------------------------------------------------------------------------------------------ lookup
+def lookup_case(V, D, n, dtype, seed, kind="uniform", ids_dtype=torch.int64):
+    gen = torch.Generator().manual_seed(seed)
+    w = torch.randn(V, D, generator=gen).to(dtype)
+    g = torch.randn(n, D, generator=gen).to(dtype)
+    ids = torch.randint(0, V, (n,), generator=gen)
+    if kind == "one":
+        ids[:] = V - 1
+    elif kind == "hot":                                     # three tokens in four are the same one
+        ids[torch.rand(n, generator=gen) < 0.75] = V // 2
+    elif kind == "missing":
+        ids[::3] = torch.tensor([-1, V, -(2 ** 31), 2 ** 31 - 1])[torch.arange(len(ids[::3])) % 4]
+    elif kind == "none":
+        ids[:] = -1
+    return w, ids.to(ids_dtype), g
+
+
+def check_lookup(cuda, w, ids, g, scale):
+    from building_gan_amd import ops
+    V, D = w.shape
+    dt = w.dtype
+    wd = w.to(cuda).requires_grad_(True)
+    out = ops.embedding(wd, ids.to(cuda), scale)
+    (dw,) = torch.autograd.grad(out, wd, g.to(cuda))
+    assert out.dtype == dt and dw.dtype == dt and out.shape == (*ids.shape, D)
+    i = ids.long().reshape(-1)
+    there = (i >= 0) & (i < V)
+    want = torch.zeros(i.numel(), D, dtype=torch.float64)
+    want[there] = w.double()[i[there]] * scale
+    within(out.reshape(-1, D), want, want.abs() * (half(dt) + 2.1 * U) + floor_of(dt), "lookup")
+    gd = g.reshape(-1, D).double()[there]
+    s = torch.zeros(V, D, dtype=torch.float64).index_add_(0, i[there], gd)
+    sa = torch.zeros(V, D, dtype=torch.float64).index_add_(0, i[there], gd.abs())
+    m = torch.zeros(V, 1, dtype=torch.float64).index_add_(0, i[there], torch.ones(len(gd), 1, dtype=torch.float64))
+    within(dw, s * scale, (s.abs() * half(dt) + sa * (m + 2.1) * U * 1.01) * scale + floor_of(dt), "lookup gradient")
+    assert not dw.detach().cpu()[(m == 0)[:, 0]].any(), "a row without tokens has a gradient"
+    with torch.no_grad():
+        assert torch.equal(ops.embedding(wd, ids.to(cuda), scale), out)
+    assert torch.equal(ops.embedding_grad_raw(g.to(cuda), ids.to(cuda), V, scale), dw), "not reproducible"
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("V,D,n,kind", [
+    (7, 128, 1440, "uniform"), (20, 128, 333, "uniform"), (7, 4, 5000, "hot"), (1, 64, 257, "uniform"), (1000, 32, 1, "uniform"),
+    (1000, 520, 700, "missing"), (513, 33, 1500, "missing"), (300, 1, 2000, "hot"), (2, 7, 9, "none"), (40000, 16, 5000, "hot"),
+    (300000, 8, 3000, "uniform"), (511, 72, 1024, "one"), (512, 8, 1025, "one"), (5000, 256, 2049, "uniform")])
+def test_lookup_and_gradient_match_float64(cuda, V, D, n, kind, dtype):
+    w, ids, g = lookup_case(V, D, n, dtype, V + D + n, kind, torch.int32 if n % 2 else torch.int64)
+    check_lookup(cuda, w, ids, g, 0.75 if D % 2 else 11.313708498984761)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("V,D,n,kind", [(70000, 8, 70001, "hot"), (70000, 12, 300000, "uniform"), (6, 24, 200000, "uniform"),
+                                        (31, 16, 70000, "hot"), (100, 40, 131072, "one")])
+def test_lookup_gradient_with_many_tokens(cuda, V, D, n, kind):
+    """More tokens than one scan of the tile counts covers, runs over many tiles."""
+    w, ids, g = lookup_case(V, D, n, torch.float32, n, kind)
+    check_lookup(cuda, w, ids, g, 1.0)
+
+
+@pytest.mark.gpu
+def test_lookup_strides_shapes_and_empty_operands(cuda):
+    from building_gan_amd import ops
+    gen = torch.Generator().manual_seed(3)
+    big = torch.randn(50, 40, generator=gen).to(cuda)
+    ids = torch.randint(0, 50, (4, 5, 6), generator=gen).to(cuda)
+    for w in (big[:, :24], big[:, 3:27], big[::2, :24], big.t()[:40]):      # pitched, unaligned, strided rows, transposed
+        i = ids % w.shape[0]
+        assert torch.equal(ops.embedding(w, i), w[i])
+        assert torch.equal(ops.embedding(w, i.transpose(0, 2)), w[i.transpose(0, 2)])
+    w = big.clone().requires_grad_(True)
+    ops.embedding(w, ids, 2.0).sum().backward()                              # a gradient without strides of its own
+    assert torch.equal(w.grad[:, 0].cpu(), 2.0 * torch.bincount(ids.flatten().cpu(), minlength=50).float())
+    gbig = torch.randn(120, 60, generator=gen).to(cuda)
+    flat = ids.flatten()
+    for gg in (gbig[:, 1:41], gbig[:, :40]):                                 # a pitch, with and without alignment
+        assert torch.equal(ops.embedding_grad_raw(gg, flat, 50), ops.embedding_grad_raw(gg.contiguous(), flat, 50))
+    assert ops.embedding(big, ids[:0]).shape == (0, 5, 6, 40)
+    assert ops.embedding(big[:, :0], ids).shape == (4, 5, 6, 0)
+    assert not ops.embedding_grad_raw(gbig[:0, :40], flat[:0], 50).any()
+    assert ops.embedding_grad_raw(gbig[:, :40], flat, 0).shape == (0, 40)
+    assert not ops.embedding(big[:0], ids).any()
+
+
+@pytest.mark.gpu
+def test_lookup_not_finite_values_stay_where_they_are(cuda):
+    from building_gan_amd import ops
+    w = torch.ones(6, 16, device=cuda)
+    w[2], w[3] = float("nan"), float("inf")
+    ids = torch.tensor([0, 2, -1, 3, 99, 5], device=cuda)
+    out = ops.embedding(w, ids)
+    assert torch.equal(out[[0, 5]], w[[0, 5]]) and out[1].isnan().all() and out[3].isinf().all() and not out[[2, 4]].any()
+    g = torch.ones(6, 16, device=cuda)
+    g[2] = g[4] = float("nan")                                               # behind the missing tokens
+    g[1] = float("inf")
+    dw = ops.embedding_grad_raw(g, ids, 6)
+    assert torch.equal(dw.sum(1).cpu(), torch.tensor([16.0, 0, float("inf"), 16, 0, 16]))
+
+
+@pytest.mark.gpu
+def test_lookup_twice_differentiable(cuda):
+    """The gradient's own backward is the lookup (both are linear)."""
+    from building_gan_amd import ops
+    w = torch.randn(9, 12, device=cuda, requires_grad=True)
+    ids = torch.randint(0, 9, (40,), device=cuda)
+    v = torch.randn(40, 12, device=cuda, requires_grad=True)
+    (dw,) = torch.autograd.grad(ops.embedding(w, ids, 3.0), w, v, create_graph=True)
+    t = torch.randn(9, 12, device=cuda)
+    (dv,) = torch.autograd.grad(dw, v, t)
+    assert torch.equal(dv, 3.0 * t[ids])
+
+
+# ------------------------------------------------------------------------------------------------ scan
+def scan_reference(x, gate, ptr, h0, reverse, dh, dlast):
+    """float64 loops: values and error bounds (before the rounding to the type) of h, h_last, dx, dgate, dh0."""
+    N, D = x.shape
+    S = len(ptr) - 1
+    x, gate = x.double(), gate.double()
+    a, c = torch.sigmoid(gate), torch.sigmoid(-gate)
+    z = lambda *s: torch.zeros(*s, dtype=torch.float64)
+    h0 = z(S, D) if h0 is None else h0.double()
+    dlast = z(S, D) if dlast is None else dlast.double()
+    dh = z(N, D) if dh is None else dh.double()
+    h, e, hp, ep, lam, el, big = z(N, D), z(N, D), z(N, D), z(N, D), z(N, D), z(N, D), z(N, D)
+    hl, ehl, d0, ed0 = h0.clone(), z(S, D), dlast.clone(), z(S, D)
+    top = max([float(t.abs().max()) for t in (x, h0) if t.numel()] + [0.0])
+    joins = 64 + N / (32 * 128)
+    for s in range(S):
+        rows = list(range(ptr[s], ptr[s + 1]))
+        if reverse:
+            rows.reverse()
+        st, er = h0[s], z(D)
+        for t in rows:
+            hp[t], ep[t] = st, er
+            er = a[t] * er + 12 * U * (a[t] * st.abs() + c[t] * x[t].abs())
+            st = a[t] * st + c[t] * x[t]
+            h[t], e[t] = st, er
+        hl[s], ehl[s] = st, er
+        mu, em, sz = dlast[s], z(D), dlast[s].abs()
+        for t in reversed(rows):
+            lam[t] = dh[t] + mu
+            big[t] = dh[t].abs() + sz
+            el[t] = em + U * big[t]
+            mu, sz, em = a[t] * lam[t], a[t] * big[t], a[t] * el[t] + 12 * U * a[t] * big[t]
+        d0[s], ed0[s] = mu, em
+    jh = 2 * U * joins * top
+    jl = 2 * U * joins * (float(big.max()) if N else 0.0)
+    e, ep, ehl = e + jh, ep + jh, ehl + jh
+    el, ed0 = el + jl, ed0 + jl
+    ac = a * c
+    dx, dg = c * lam, lam * (hp - x) * ac
+    edx = c * el + 12 * U * c * big
+    edg = ac * (el * (hp - x).abs() + big * (ep + U * (hp.abs() + x.abs())) + 25 * U * big * (hp - x).abs() + el * ep)
+    return (h, hl, dx, dg, d0), (e, ehl, edx, edg, ed0)
+
+
+def scan_case(N, D, ptr, dtype, seed, h0=True, slow=False):
+    gen = torch.Generator().manual_seed(seed)
+    z = torch.randn(N, 2 * D, generator=gen)
+    z[:, D:] += torch.linspace(-2.0, 9.0 if slow else 5.0, D)
+    z = z.to(dtype)
+    S = len(ptr) - 1
+    return dict(z=z, x=z[:, :D], gate=z[:, D:], h0=torch.randn(S, D, generator=gen) if h0 else None,
+                dh=torch.randn(N, D, generator=gen).to(dtype), dlast=torch.randn(S, D, generator=gen))
+
+
+def check_scan(cuda, c, ptr, reverse=False, use_dh=True, use_dlast=True, packed=True, rowptr="ptr"):
+    from building_gan_amd import ops
+    dt = c["x"].dtype
+    z = c["z"].to(cuda)
+    D = c["x"].shape[1]
+    x, gate = (z[:, :D], z[:, D:]) if packed else (z[:, :D].contiguous(), z[:, D:].contiguous())
+    x, gate = x.detach().requires_grad_(True), gate.detach().requires_grad_(True)
+    h0 = None if c["h0"] is None else c["h0"].to(cuda).requires_grad_(True)
+    rp = torch.tensor(ptr, dtype=torch.int32, device=cuda) if rowptr == "ptr" else rowptr
+    dh, dlast = c["dh"] if use_dh else None, c["dlast"] if use_dlast else None
+    h, hl = ops.gated_scan(x, gate, rp, h0, reverse)
+    outs, grads = [], []
+    if use_dh:
+        outs.append(h), grads.append(dh.to(cuda))
+    if use_dlast:
+        outs.append(hl), grads.append(dlast.to(cuda))
+    got = torch.autograd.grad(outs, [x, gate] + ([] if h0 is None else [h0]), grads)
+    want, err = scan_reference(c["x"], c["gate"], ptr, c["h0"], reverse, dh, dlast)
+    for name, g, w, e, t in zip(("h", "h_last", "dx", "dgate", "dh0"), (h, hl) + got, want, err, (dt, torch.float32, dt, dt, torch.float32)):
+        assert g.dtype == t
+        within(g, w, e * 1.01 + w.abs() * half(t) + floor_of(t), name)
+    with torch.no_grad():                                    # without heads, and again: the same bits
+        h2, hl2 = ops.gated_scan(x, gate, rp, h0, reverse)
+    assert torch.equal(h2, h) and torch.equal(hl2, hl)
+    return (h, hl) + got
+
+
+RAGGED = [0, 0, 1, 40, 40, 40, 41, 200, 201, 460, 460]       # no rows, one row, first and last segment empty
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("reverse", [False, True])
+@pytest.mark.parametrize("D", [1, 3, 8, 33, 64, 100, 128, 260])
+def test_scan_and_gradients_match_float64(cuda, D, reverse, dtype):
+    c = scan_case(460, D, RAGGED, dtype, D)
+    check_scan(cuda, c, RAGGED, reverse, packed=D % 8 != 0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("reverse", [False, True])
+@pytest.mark.parametrize("N,D,ptr", [(300, 36, [5, 5, 100, 260]), (300, 8, [300, 300]), (17, 5, [0, 17]), (1, 4, [0, 1]),
+                                     (2, 130, [0, 1, 2]), (128, 128, [0, 128]), (129, 132, [0, 128, 129]), (700, 68, [0, 0, 700, 700]),
+                                     (1030, 12, [0, 512, 1030]), (9000, 8, [0, 100, 8900]), (5000, 132, [0, 5000])])
+def test_scan_rows_behind_the_segments_and_tile_edges(cuda, N, D, ptr, reverse):
+    c = scan_case(N, D, ptr, torch.float32, N + D, slow=True)
+    got = check_scan(cuda, c, ptr, reverse)
+    for t in (got[0], got[2], got[3]):
+        assert not t[:ptr[0]].any() and not t[ptr[-1]:].any(), "a row in no segment is not zero"
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("h0,use_dh,use_dlast", [(False, True, True), (True, False, True), (True, True, False), (False, False, True)])
+def test_scan_without_optional_operands(cuda, h0, use_dh, use_dlast):
+    c = scan_case(460, 20, RAGGED, torch.float32, 5, h0=h0)
+    check_scan(cuda, c, RAGGED, use_dh=use_dh, use_dlast=use_dlast)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("reverse", [False, True])
+def test_scan_of_equal_segments_and_batches(cuda, reverse):
+    from building_gan_amd import ops
+    B, T, D = 6, 77, 24
+    c = scan_case(B * T, D, list(range(0, B * T + 1, T)), torch.float32, 11)
+    ptr = list(range(0, B * T + 1, T))
+    a = check_scan(cuda, c, ptr, reverse)
+    b = check_scan(cuda, c, ptr, reverse, rowptr=None) if B == 1 else None
+    x, gate, h0 = c["x"].to(cuda), c["gate"].to(cuda), c["h0"].to(cuda)
+    h, hl = ops.gated_scan(x.view(B, T, D), gate.view(B, T, D), h0=h0, reverse=reverse)
+    assert torch.equal(h.view(-1, D), a[0]) and torch.equal(hl, a[1]) and b is None
+    z = c["z"].to(cuda).view(B, T, 2 * D)
+    h, hl = ops.gated_scan(z[..., :D], z[..., D:], h0=h0, reverse=reverse)
+    assert torch.equal(h.view(-1, D), a[0])
+    h, hl = ops.gated_scan(x.view(B, T, D).transpose(0, 1), gate.view(B, T, D).transpose(0, 1), reverse=reverse)   # copied first
+    e, el = ops.gated_scan(x.view(B, T, D).transpose(0, 1).contiguous(), gate.view(B, T, D).transpose(0, 1).contiguous(), reverse=reverse)
+    assert torch.equal(h, e) and torch.equal(hl, el)
+    one, onel = ops.gated_scan(x, gate, reverse=reverse)     # no row pointer: one segment
+    two, twol = ops.gated_scan(x, gate, torch.tensor([0, B * T], dtype=torch.int32, device=cuda), reverse=reverse)
+    assert torch.equal(one, two) and torch.equal(onel, twol)
+
+
+@pytest.mark.gpu
+def test_scan_of_nothing(cuda):
+    from building_gan_amd import ops
+    h0 = torch.randn(3, 8, device=cuda, requires_grad=True)
+    x = torch.zeros(0, 8, device=cuda, requires_grad=True)
+    h, hl = ops.gated_scan(x, x.detach(), torch.zeros(4, dtype=torch.int32, device=cuda), h0)
+    assert h.shape == (0, 8) and torch.equal(hl, h0)
+    g = torch.randn(3, 8, device=cuda)
+    assert torch.equal(torch.autograd.grad(hl, h0, g)[0], g)
+    h, hl = ops.gated_scan(x.detach(), x.detach())
+    assert h.shape == (0, 8) and hl.shape == (1, 8) and not hl.any()
+    e = torch.zeros(3, 0, 8, device=cuda)
+    h, hl = ops.gated_scan(e, e, h0=h0.detach())
+    assert h.shape == (3, 0, 8) and torch.equal(hl, h0)
+    w = torch.zeros(5, 0, device=cuda)
+    assert ops.gated_scan(w, w)[0].shape == (5, 0)
+    y = torch.ones(5, 8, device=cuda)                        # rows, but no segment
+    h, hl = ops.gated_scan(y, y, torch.zeros(1, dtype=torch.int32, device=cuda))
+    assert not h.any() and hl.shape == (0, 8)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("reverse", [False, True])
+def test_scan_with_many_segments(cuda, reverse):
+    """More segments than a workgroup has threads: the search for a tile's first segment takes two rounds."""
+    gen = torch.Generator().manual_seed(9)
+    lens = torch.randint(0, 3, (3000,), generator=gen)
+    ptr = [0] + torch.cumsum(lens, 0).tolist()
+    c = scan_case(ptr[-1], 8, ptr, torch.float32, 2)
+    check_scan(cuda, c, ptr, reverse)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("reverse", [False, True])
+def test_scan_not_finite_values_stay_in_their_segment_and_column(cuda, reverse):
+    from building_gan_amd import ops
+    ptr = [0, 150, 151, 400, 600]
+    c = scan_case(620, 12, ptr, torch.float32, 4)
+    x, gate, h0 = c["x"].clone(), c["gate"].clone(), c["h0"].clone()
+    clean = [t.clone() for t in ops.gated_scan(x.to(cuda), gate.to(cuda), torch.tensor(ptr, dtype=torch.int32, device=cuda), h0.to(cuda), reverse)]
+    x[160, 3] = float("nan")
+    x[605, 4] = gate[610, 5] = float("nan")                  # rows in no segment
+    h0[0, 7] = float("inf")
+    rp = torch.tensor(ptr, dtype=torch.int32, device=cuda)
+    xs, gs, hs = x.to(cuda).requires_grad_(True), gate.to(cuda).requires_grad_(True), h0.to(cuda).requires_grad_(True)
+    h, hl = ops.gated_scan(xs, gs, rp, hs, reverse)
+    dx, dg, d0 = torch.autograd.grad((h, hl), (xs, gs, hs), (torch.ones_like(h), torch.ones_like(hl)))
+    touched = torch.zeros(620, 12, dtype=torch.bool)
+    touched[151:400, 3] = True
+    touched[0:150, 7] = True
+    same = (h == clean[0]).cpu()
+    assert same[~touched].all() and not h[600:].any() and not dx[600:].any() and not dg[600:].any()
+    assert h[160 if reverse else 399, 3].isnan() and hl[2, 3].isnan()
+    assert torch.isfinite(dx).all() and torch.isfinite(d0).all() and torch.isfinite(dg.cpu()[~touched]).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_scan_saturated_gates(cuda, dtype):
+    """Gates that hold the state (a = 1 exactly, c = 0) and that replace it (a = 0)."""
+    from building_gan_amd import ops
+    inf = float("inf")
+    x = torch.arange(1.0, 7.0, device=cuda).view(6, 1).expand(6, 8).contiguous().to(dtype)
+    gate = torch.tensor([-inf, inf, 200.0, -200.0, inf, -inf], device=cuda).view(6, 1).expand(6, 8).contiguous().to(dtype)
+    x.requires_grad_(True), gate.requires_grad_(True)
+    h, hl = ops.gated_scan(x, gate)
+    assert h[:, 0].tolist() == [1, 1, 1, 4, 4, 6] and hl[0, 0] == 6
+    dx, dg = torch.autograd.grad(h, (x, gate), torch.ones_like(h))
+    assert dx[:, 0].tolist() == [3, 0, 0, 2, 0, 1] and not dg.any()
+    gate = torch.tensor([30.0, -30.0, 80.0, -80.0, 1e-30, -1e-30], device=cuda).view(6, 1).contiguous()
+    one = torch.ones(6, 1, device=cuda)
+    c1 = ops.gated_scan_step(one, gate, torch.zeros(6, 1, device=cuda))[1].cpu().double()      # sigmoid(-gate) itself
+    a1 = ops.gated_scan_step(torch.zeros_like(one), gate, one)[1].cpu().double()
+    g = gate.cpu().double()
+    within(c1, torch.sigmoid(-g), torch.sigmoid(-g) * 12 * U, "sigmoid(-gate)")
+    within(a1, torch.sigmoid(g), torch.sigmoid(g) * 12 * U, "sigmoid(gate)")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("reverse", [False, True])
+def test_scan_gradients_against_differences(cuda, reverse):
+    """<gradient, direction> against central differences of the float64 loops (step 1e-4: their own error is below 1e-7 of
+    the derivative's scale)."""
+    from building_gan_amd import ops
+    ptr = [0, 30, 30, 95, 131]
+    c = scan_case(140, 6, ptr, torch.float32, 8)
+    x, gate, h0 = (c[k].to(cuda).contiguous().requires_grad_(True) for k in ("x", "gate", "h0"))
+    h, hl = ops.gated_scan(x, gate, torch.tensor(ptr, dtype=torch.int32, device=cuda), h0, reverse)
+    grads = torch.autograd.grad((h, hl), (x, gate, h0), (c["dh"].to(cuda), c["dlast"].to(cuda)))
+    _, err = scan_reference(c["x"], c["gate"], ptr, c["h0"], reverse, c["dh"], c["dlast"])
+
+    def loss(xx, gg, hh):
+        v, _ = scan_reference(xx, gg, ptr, hh, reverse, None, None)
+        return float((v[0] * c["dh"].double()).sum() + (v[1] * c["dlast"].double()).sum())
+
+    at = [c["x"].double(), c["gate"].double(), c["h0"].double()]
+    gen = torch.Generator().manual_seed(1)
+    for k in range(3):
+        d = torch.randn(at[k].shape, generator=gen, dtype=torch.float64)
+        up, dn = list(at), list(at)
+        up[k], dn[k] = at[k] + 1e-4 * d, at[k] - 1e-4 * d
+        diff = (loss(*up) - loss(*dn)) / 2e-4
+        g = grads[k].cpu().double()
+        tol = float(((err[2 + k] + g.abs() * U) * d.abs()).sum()) + 1e-7 * float((g * d).abs().sum())
+        assert abs(float((g * d).sum()) - diff) <= tol, (k, float((g * d).sum()), diff, tol)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,D", [(1, 1), (3, 7), (50, 256), (5, 1028), (9, 2051)])
+def test_step_matches_float64_and_the_scan(cuda, n, D, dtype):
+    from building_gan_amd import ops
+    c = scan_case(n, D, list(range(n + 1)), dtype, n * D)
+    z, state = c["z"].to(cuda), c["h0"].to(cuda)
+    h, new = ops.gated_scan_step(z[:, :D], z[:, D:], state)
+    want, err = scan_reference(c["x"], c["gate"], list(range(n + 1)), c["h0"], False, None, None)
+    within(new, want[1], err[1], "state")
+    within(h, want[0], err[0] + want[0].abs() * half(dtype) + floor_of(dtype), "h")
+    hs, hl = ops.gated_scan(z[:, :D], z[:, D:], torch.arange(n + 1, dtype=torch.int32, device=cuda), state)
+    assert torch.equal(hs, h) and torch.equal(hl, new), "a scan over segments of one row is the step"
+    kept = state.clone()
+    h2, out = ops.gated_scan_step(z[:, :D], z[:, D:], kept, state_out=kept)
+    assert out is kept and torch.equal(kept, new) and torch.equal(h2, h)
+
+
+@pytest.mark.gpu
+def test_step_leaves_other_rows_alone(cuda):
+    from building_gan_amd import ops
+    buf = torch.randn(9, 40, device=cuda)
+    before = buf.clone()
+    x = torch.randn(4, 36, device=cuda)
+    view = buf[2:6, 2:38]                                    # a pitch and no 16-byte alignment
+    h, _ = ops.gated_scan_step(x, x, view, state_out=view)
+    want = ops.gated_scan_step(x, x, before[2:6, 2:38].contiguous())[1]
+    assert torch.equal(view, want)
+    buf[2:6, 2:38] = before[2:6, 2:38]
+    assert torch.equal(buf, before)
+    assert ops.gated_scan_step(x[:0], x[:0], view[:0])[0].shape == (0, 36)
+
+
+# ------------------------------------------------------------------------------------------------ together
+def run_together(dev, seed=0):
+    from building_gan_amd.synthetic import make_batch
+    from building_gan_amd.plan import build_plan
+    g = make_batch("small", seed=seed, ragged=True).to(dev)
+    return build_plan(g)
+
+
+@pytest.mark.gpu
+def test_levels_looked_up_scanned_along_stories_and_pooled(cuda):
+    """A batch's floor levels -> learned vectors -> state along each graph's voxels -> graph pooling, with gradients, against
+    float64 autograd over the same steps."""
+    from building_gan_amd import ops
+    p = run_together(cuda)
+    seg = p.graph_seg if hasattr(p, "graph_seg") else p.story_seg
+    N, D = seg.n_cols, 32
+    level = p.level
+    gen = torch.Generator().manual_seed(2)
+    table = (torch.randn(20, 2 * D, generator=gen) * 0.5)
+    start = torch.randn(seg.n_rows, D, generator=gen)
+    wt, st = table.to(cuda).requires_grad_(True), start.to(cuda).requires_grad_(True)
+    z = ops.embedding(wt, level, 1.5)
+    h, hl = ops.gated_scan(z[:, :D], z[:, D:], seg.rowptr, st)
+    pooled, _ = ops.SegMax.apply(h, seg)
+    cot = torch.randn(seg.n_rows, D, generator=gen)
+    loss = (pooled * cot.to(cuda)).sum() + (hl * cot.to(cuda)).sum()
+    dw, ds = torch.autograd.grad(loss, (wt, st))
+    w64, s64 = table.double().requires_grad_(True), start.double().requires_grad_(True)
+    z64 = 1.5 * w64[level.cpu().long()]
+    ptr = seg.rowptr.tolist()
+    best, last = [], []
+    for s in range(seg.n_rows):
+        state, hs = s64[s], []
+        for t in range(ptr[s], ptr[s + 1]):
+            a = torch.sigmoid(z64[t, D:])
+            state = a * state + (1 - a) * z64[t, :D]
+            hs.append(state)
+        best.append(torch.stack(hs).max(0).values), last.append(state)
+    want = (torch.stack(best) * cot.double()).sum() + (torch.stack(last) * cot.double()).sum()
+    dw64, ds64 = torch.autograd.grad(want, (w64, s64))
+    # the sums of some hundred products of fp32 factors each known to about 100 u (module docstring: a state's error after many rows)
+    torch.testing.assert_close(loss.detach().cpu().double(), want.detach(), rtol=1e-5, atol=1e-4)
+    assert float((dw.cpu().double() - dw64).abs().max()) <= 1e-5 * float(dw64.abs().max()) * 10
+    assert float((ds.cpu().double() - ds64).abs().max()) <= 1e-5 * float(ds64.abs().max()) * 10
+
+
+@pytest.mark.gpu
+def test_captured_and_replayed(cuda):
+    """Forward, backward and step captured into one graph and replayed with other inputs in the same buffers, eager work and
+    synchronisations in between."""
+    from building_gan_amd import ops
+    V, D, n, S = 600, 64, 3000, 5
+    ptr = torch.tensor([0, 10, 10, 900, 2500, 2900], dtype=torch.int32, device=cuda)
+    gen = torch.Generator(device=cuda).manual_seed(0)
+
+    def fill():
+        ids.copy_(torch.randint(-1, V, (n,), generator=gen, device=cuda))
+        w.copy_(torch.randn(V, 2 * D, generator=gen, device=cuda))
+        g.copy_(torch.randn(n, D, generator=gen, device=cuda))
+        dl.copy_(torch.randn(S, D, generator=gen, device=cuda))
+
+    def passes():
+        z = ops.embedding_raw(w, ids, 2.0)
+        h, hl, heads = ops.gated_scan_raw(z[:, :D], z[:, D:], ptr, None, False, keep_heads=True)
+        dx, dg, _ = ops.gated_scan_grad_raw(z[:, :D], z[:, D:], ptr, None, False, heads, g, dl)
+        dw = ops.embedding_grad_raw(torch.cat([dx, dg], 1), ids, V, 2.0)
+        hs, new = ops.gated_scan_step(z[:S, :D], z[:S, D:], hl)
+        return z, h, hl, dx, dg, dw, hs, new
+
+    ids = torch.zeros(n, dtype=torch.int64, device=cuda)
+    w, g, dl = (torch.zeros(*s, device=cuda) for s in ((V, 2 * D), (n, D), (S, D)))
+    fill()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        passes()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = passes()
+    for k in range(4):
+        fill()
+        graph.replay()
+        if k % 2:
+            torch.cuda.synchronize()
+        got = [t.clone() for t in outs]
+        want = passes()
+        for i, (a, b) in enumerate(zip(got, want)):
+            assert torch.equal(a, b), (k, i)
+
+
+@pytest.mark.gpu
+def test_on_another_stream_and_two_calls_at_once(cuda):
+    from building_gan_amd import ops
+    c = scan_case(4000, 128, [0, 1000, 4000], torch.float32, 3)
+    x, gate = c["x"].to(cuda).contiguous(), c["gate"].to(cuda).contiguous()
+    ptr = torch.tensor([0, 1000, 4000], dtype=torch.int32, device=cuda)
+    ids = torch.randint(0, 50, (4000,), device=cuda)
+    want = ops.gated_scan(x, gate, ptr)[0]
+    want_w = ops.embedding_grad_raw(x, ids, 50)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    outs = []
+    for k in range(6):
+        with torch.cuda.stream(streams[k % 2]):
+            outs.append((ops.gated_scan(x, gate, ptr)[0], ops.embedding_grad_raw(x, ids, 50)))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, want) and torch.equal(b, want_w) for a, b in outs)
