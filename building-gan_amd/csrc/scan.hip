@@ -5,17 +5,24 @@
 //   backward:  mu_t = a_t (dh_t + mu_{t+1})                mu after a segment's last row = dlast (or 0)
 //              dx_t = c_t (dh_t + mu_{t+1}),  dgate_t = (dh_t + mu_{t+1}) (h_{t-1} - x_t) a_t c_t,  dh0 = mu_first
 // Both are chains of maps  s -> A s + B, which compose:  (A2, B2) o (A1, B1) = (A2 A1, A2 B1 + B2).  A segment's first row
-// is a CUT: the map that forgets what comes in (kept as a flag, not as A = 0: 0 * inf of another segment would leak).
-// Rows are cut into tiles whatever the segments are; a workgroup composes a tile's rows in registers, the tiles are
-// composed along each column, and the tile's rows are walked again from the state that comes in.
-// h is never read back: the backward pass rebuilds it in registers from the fp32 state kept at the head of every tile.
-#include <type_traits>
+// (its last, for mu) is a CUT: the map that forgets what comes in.  It is marked by A = -1 (a true A is never negative) and
+// taken by selection: a product with 0 would let an inf or NaN of another segment through.
+//
+// Rows are cut into tiles whatever the segments are.  A workgroup reads its tile ONCE, keeps it in registers, composes its
+// rows' maps, publishes the tile's map, finds the state that enters the tile from what the tiles before it published, and
+// walks its rows from there.  h is never read back: the backward pass rebuilds it from the fp32 state kept at the head of
+// every 2048 / CG rows.
 #include "common.h"
 
 namespace {
 
-constexpr int kTileElems = 4096;                 // rows of a tile * column groups (of 4 columns) of a tile
-constexpr int kCarryCols = 32, kCarrySlices = 32;
+// A tile: THREADS / CG row groups of kRows rows times CG column groups of 4 columns.  16-byte (8-byte) pieces of a row per
+// lane; CG = 32 makes 512 B (256 B) of a row of fp32 (16-bit) elements, narrower matrices take fewer columns and more rows.
+constexpr int kRows = 8;
+constexpr int kFwdThreads = 512, kBwdThreads = 256;
+constexpr int kGroup = 8;                        // tiles of a group, groups of a block (see enter_tile)
+constexpr uint32_t kEmpty = 0xFFFFFFFFu;         // what unpublished words hold
+constexpr int kSpinLimit = 1 << 22;              // a wait of several seconds: only a workspace in use by another call gets there
 
 struct Segs { const int32_t* ptr; int64_t S, N, T; };      // ptr NULL: S segments of T rows
 
@@ -28,15 +35,20 @@ __device__ __forceinline__ int64_t seg_lo(const Segs& g, int64_t j) {           
     return REV ? g.N - p : p;
 }
 
-// first[r] / last[r]: the segment whose first / last row is row r of the tile, -1: none; first[r] = -2: r is in no segment.
-// The segment of the tile's first row is found by a search THREADS wide: one round for up to THREADS segments.
+// mask[group]: bit i = row i of the group is a segment's first row, bit 8 + i = its last, bit 16 + i = in no segment;
+// first[row] / last[row] = that segment where the bit is set.  The segment of the tile's first row is found by a search
+// as wide as the workgroup: one round of loads for up to blockDim.x segments.
 template <bool REV>
-__device__ __forceinline__ void mark_tile(const Segs& g, int64_t row0, int rows, int32_t* first, int32_t* last) {
-    const int t = threadIdx.x, threads = blockDim.x;
+__device__ __forceinline__ void mark_tile(const Segs& g, int64_t row0, int groups, uint32_t* mask, int32_t* first, int32_t* last) {
+    const int t = threadIdx.x, threads = blockDim.x, rows = groups * kRows;
     const int64_t lo_all = seg_lo<REV>(g, 0), hi_all = seg_lo<REV>(g, g.S), end = row0 + rows;
-    for (int r = t; r < rows; r += threads) {
-        first[r] = row0 + r >= lo_all && row0 + r < hi_all ? -1 : -2;
-        last[r] = -1;
+    if (t < groups) {
+        uint32_t m = 0;
+        for (int i = 0; i < kRows; ++i) {
+            const int64_t r = row0 + t * kRows + i;
+            if (r < g.N && (r < lo_all || r >= hi_all)) m |= 0x10000u << i;
+        }
+        mask[t] = m;
     }
     int64_t lo = 0, hi = g.S;                    // lo -> how many segments begin at or before row0
     if (!g.ptr) lo = hi = g.T > 0 ? row0 / g.T + 1 : 0;
@@ -53,338 +65,478 @@ __device__ __forceinline__ void mark_tile(const Segs& g, int64_t row0, int rows,
         if (a >= end) break;
         if (a >= b) continue;
         const int32_t s = (int32_t)(REV ? g.S - 1 - j : j);
-        if (a >= row0) first[a - row0] = s;
-        if (b - 1 >= row0 && b - 1 < end) last[b - 1 - row0] = s;
+        if (a >= row0) {
+            first[a - row0] = s;
+            atomicOr(&mask[(a - row0) / kRows], 1u << ((a - row0) % kRows));
+        }
+        if (b - 1 >= row0 && b - 1 < end) {
+            last[b - 1 - row0] = s;
+            atomicOr(&mask[(b - 1 - row0) / kRows], 0x100u << ((b - 1 - row0) % kRows));
+        }
     }
     __syncthreads();
 }
 
 // a = sigmoid(g), c = sigmoid(-g) without cancellation: e = exp(-|g|) <= 1, r = 1 / (1 + e); one of them is r, the other e r.
-// The product |g| log2(e) is carried in two parts, so e is good to ~2 ulp at any g.
+// The product |g| log2(e) is carried in two parts and the reciprocal takes one Newton step: v_exp_f32 and v_rcp_f32 alone are
+// off by up to an ulp to one side, which a product over a long memory's a's would add up.
 __device__ __forceinline__ void gate_pair(float g, float& a, float& c) {
     const float m = fabsf(g), p = m * -1.4426950408889634f;
-    const float lo = fmaf(m, -1.4426950408889634f, -p) - m * 1.9259629911266175e-8f;
+    const float lo = fmaf(m, -1.9259629911266175e-8f, fmaf(m, -1.4426950408889634f, -p));
     float e = __builtin_amdgcn_exp2f(p);
-    e = fmaf(e, lo * 0.6931471805599453f, e);
-    if (!(m < 120.f)) e = g != g ? g : 0.f;                              // (the correction term is inf * 0 for an infinite gate)
-    const float r = __builtin_amdgcn_rcpf(1.f + e), er = e * r;
+    e = m < 100.f ? fmaf(e, lo * 0.6931471805599453f, e) : e;            // (inf: the correction is inf - inf; NaN stays)
+    const float s = 1.f + e, r0 = __builtin_amdgcn_rcpf(s), r = fmaf(r0, fmaf(-s, r0, 1.f), r0), er = e * r;
     a = g < 0.f ? er : r;
     c = g < 0.f ? r : er;
 }
 
-// four columns of a row: one piece (WIDE) or CG apart
-template <class T, bool WIDE>
-__device__ __forceinline__ void ld4(const T* __restrict__ row, int64_t c, int CG, int64_t D, float (&v)[4]) {
-    if (WIDE) {
-        if (c < D) {
-            const BgVec<T, 4> x = *reinterpret_cast<const BgVec<T, 4>*>(row + c);
+// Four columns of a row as one access at whatever alignment the row has (the hardware takes any; the alignment promised to
+// the compiler is the element's)
+template <class T>
+struct __attribute__((packed, aligned(sizeof(T)))) Piece { T v[4]; };
+
+// What a thread touches of its tile: uniform base + 32-bit offset of its first row's piece + `step` elements a row.
+struct Lane {
+    int nv, nrows;                               // columns (0 .. 4) and rows (0 .. kRows) that exist
+    __device__ __forceinline__ bool whole() const { return nv == 4 && nrows == kRows; }
+};
+template <class T>
+__device__ __forceinline__ void load_rows(const T* __restrict__ base, uint32_t off, int32_t step, Lane l, float (&v)[kRows][4]) {
+    if (l.whole()) {
+        Piece<T> x[kRows];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = (float)x.v[e];
-        }
+        for (int i = 0; i < kRows; ++i) x[i] = *reinterpret_cast<const Piece<T>*>(base + (uint32_t)(off + i * step));
+#pragma unroll
+        for (int i = 0; i < kRows; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[i][e] = (float)x[i].v[e];
     } else {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) if (c + e * CG < D) v[e] = (float)row[c + e * CG];
+        for (int i = 0; i < kRows; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[i][e] = i < l.nrows && e < l.nv ? (float)base[(uint32_t)(off + i * step) + e] : 0.f;
     }
 }
-template <class T, bool WIDE>
-__device__ __forceinline__ void st4(T* __restrict__ row, int64_t c, int CG, int64_t D, const float (&v)[4]) {
-    if (WIDE) {
-        BgVec<T, 4> x;
+template <class T>
+__device__ __forceinline__ void store_row(T* __restrict__ base, uint32_t off, Lane l, int i, const float (&v)[4]) {
+    if (l.whole()) {
+        Piece<T> x;
 #pragma unroll
         for (int e = 0; e < 4; ++e) x.v[e] = bg_round<T>(v[e]);
-        if (c < D) *reinterpret_cast<BgVec<T, 4>*>(row + c) = x;
-    } else {
+        *reinterpret_cast<Piece<T>*>(base + off) = x;
+    } else if (i < l.nrows) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) if (c + e * CG < D) row[c + e * CG] = bg_round<T>(v[e]);
+        for (int e = 0; e < 4; ++e) if (e < l.nv) base[off + e] = bg_round<T>(v[e]);
     }
 }
-
-struct Map4 { float A[4], B[4]; };
-struct TileAgg { float* ab; int32_t* cut; };     // ab[(2 * tile + which) * D + c], cut[tile]
-
-// The maps of the tile's row groups -> LDS; then `in` (the state that enters the tile) becomes the state that enters this
-// thread's row group (from below: groups 0 .. rg - 1; from above with UP: groups RG - 1 .. rg + 1).
-template <bool UP>
-__device__ __forceinline__ void enter_group(const float (*sA)[4], const float (*sB)[4], const int32_t* sCut, int cg, int rg, int CG,
-                                            int RG, float (&s)[4]) {
-    for (int k = UP ? RG - 1 : 0; UP ? k > rg : k < rg; k += UP ? -1 : 1) {
-        const bool cut = sCut[k] != 0;
+// fp32 rows of [n, D] (states): rare, element by element
+__device__ __forceinline__ void ld_state(const float* __restrict__ p, int64_t row, int64_t D, int64_t c, int nv, float (&v)[4]) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const float b = sB[k * CG + cg][e];
-            s[e] = cut ? b : fmaf(sA[k * CG + cg][e], s[e], b);
-        }
-    }
+    for (int e = 0; e < 4; ++e) v[e] = p && e < nv ? p[row * D + c + e] : 0.f;
 }
-template <bool UP>
-__device__ __forceinline__ void write_agg(const float (*sA)[4], const float (*sB)[4], const int32_t* sCut, int cg, int CG, int RG,
-                                          TileAgg agg, int64_t tile, int64_t c0, int64_t D, bool wide) {
-    float A[4] = {1.f, 1.f, 1.f, 1.f}, B[4] = {0.f, 0.f, 0.f, 0.f};
-    int cut_any = 0;
-    for (int i = 0; i < RG; ++i) {
-        const int k = UP ? RG - 1 - i : i;
-        const bool cut = sCut[k] != 0;
-        cut_any |= cut;
+__device__ __forceinline__ void st_state(float* __restrict__ p, int64_t row, int64_t D, int64_t c, int nv, const float (&v)[4]) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const float a = sA[k * CG + cg][e], b = sB[k * CG + cg][e];
-            B[e] = cut ? b : fmaf(a, B[e], b);
-            A[e] = cut ? 0.f : a * A[e];
-        }
-    }
+    for (int e = 0; e < 4; ++e) if (e < nv) p[row * D + c + e] = v[e];
+}
+
+// ------------------------------------------------------------------------------------------------ maps
+struct Map { float A[4], B[4]; };
+__device__ __forceinline__ void after(Map& m, const float (&A1)[4], const float (&B1)[4]) {          // m <- m o (A1, B1)
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-        const int64_t c = wide ? c0 + cg * 4 + e : c0 + cg + e * CG;
-        if (c < D) { agg.ab[2 * tile * D + c] = A[e]; agg.ab[(2 * tile + 1) * D + c] = B[e]; }
+        m.B[e] = m.A[e] < 0.f ? m.B[e] : fmaf(m.A[e], B1[e], m.B[e]);
+        m.A[e] = m.A[e] < 0.f || A1[e] < 0.f ? -1.f : m.A[e] * A1[e];
     }
-    if (cg == 0 && blockIdx.y == 0) agg.cut[tile] = cut_any;
+}
+__device__ __forceinline__ float apply(float A, float B, float s) { return A < 0.f ? B : fmaf(A, s, B); }
+
+// Maps of the workgroup's row groups: `m` becomes the map of everything before this thread's group (UP: the rows are walked
+// from the last group to the first).  In a wave by shuffles (64 / CG groups), then over the waves through LDS.  Returns the
+// map of the whole tile in the threads of the LAST group of the walk.
+struct WaveMaps { float A[kFwdThreads / 64][128], B[kFwdThreads / 64][128]; };
+template <bool UP>
+__device__ __forceinline__ Map before_group(Map& m, int CG, int cg, WaveMaps& w) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+    const int at = UP ? 63 - lane : lane, edge = at / CG;                // this group's place in the wave's walk
+    for (int o = 1; o * CG < 64; o <<= 1) {
+        float A1[4], B1[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            A1[e] = UP ? __shfl_down(m.A[e], o * CG, 64) : __shfl_up(m.A[e], o * CG, 64);
+            B1[e] = UP ? __shfl_down(m.B[e], o * CG, 64) : __shfl_up(m.B[e], o * CG, 64);
+        }
+        if (edge >= o) after(m, A1, B1);
+    }
+    if (at >= 64 - CG)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) { w.A[wave][cg * 4 + e] = m.A[e]; w.B[wave][cg * 4 + e] = m.B[e]; }
+    const Map own = m;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        m.A[e] = UP ? __shfl_down(own.A[e], CG, 64) : __shfl_up(own.A[e], CG, 64);
+        m.B[e] = UP ? __shfl_down(own.B[e], CG, 64) : __shfl_up(own.B[e], CG, 64);
+        if (edge == 0) { m.A[e] = 1.f; m.B[e] = 0.f; }
+    }
+    __syncthreads();
+    Map pre;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) { pre.A[e] = 1.f; pre.B[e] = 0.f; }
+    for (int k = 0; k < waves - 1; ++k) {
+        const int x = UP ? waves - 1 - k : k;
+        if (UP ? x <= wave : x >= wave) break;
+        Map y;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) { y.A[e] = w.A[x][cg * 4 + e]; y.B[e] = w.B[x][cg * 4 + e]; }
+        after(y, pre.A, pre.B);
+        pre = y;
+    }
+    after(m, pre.A, pre.B);
+    Map all = own;
+    after(all, pre.A, pre.B);
+    return all;
 }
 
-// ------------------------------------------------------------------------------------------------ forward
-// APPLY false: the tile's map -> agg.  APPLY true: heads[tile] enters, h and h_last leave.
-template <class T, int K, bool WIDE, bool REV, bool APPLY>
-__global__ __launch_bounds__(256) void k_scan_fwd(const T* __restrict__ x, int64_t ldx, const T* __restrict__ gate, int64_t ldg, Segs g,
-                                                  int64_t D, const float* __restrict__ h0, int CG, TileAgg agg,
-                                                  const float* __restrict__ heads, T* __restrict__ h, int64_t ldh,
-                                                  float* __restrict__ h_last) {
-    __shared__ int32_t first[kTileElems / 8], last[kTileElems / 8];
-    __shared__ float sA[256][4], sB[256][4];
-    __shared__ int32_t sCut[32];
-    const int RG = 256 / CG, cg = threadIdx.x & (CG - 1), rg = threadIdx.x / CG, rows = RG * K;
-    const int64_t tile = blockIdx.x, row0 = tile * rows, c0 = (int64_t)blockIdx.y * (CG * 4), c = WIDE ? c0 + cg * 4 : c0 + cg;
-    const int64_t r0 = row0 + rg * K;
-    float a[K][4], b[K][4];
+// ------------------------------------------------------------------------------------------------ from tile to tile
+// Tiles are taken in the order of the walk by a ticket, so whatever a tile waits for belongs to a workgroup that already
+// runs.  Every tile publishes its map, the last of 8 tiles their group's map, the last of 8 groups the STATE behind its 64
+// tiles: a tile reads at most 7 maps of tiles, 7 of groups and one state, and the only chain along the sequence has a link
+// per 64 tiles.  The products are always formed in this order, so the bits do not depend on who was first (a look-back
+// that takes the nearest state it finds would).  A word is its own flag: (A, B) travel as one 64-bit relaxed atomic,
+// B's bits never being kEmpty; no fences, no other memory is ordered by them.
+struct Chain { uint64_t *tile, *group; uint32_t *state, *ticket; };
+struct Neighbours { float A[2 * kGroup - 1][128], B[2 * kGroup - 1][128]; };       // 7 tiles, 7 groups, the state (in B)
+
+__device__ __forceinline__ void publish(uint64_t* p, float A, float B) {
+    uint32_t b = __float_as_uint(B);
+    if (b == kEmpty) b = 0x7FC00000u;                                    // a NaN stays a NaN
+    __hip_atomic_store(p, ((uint64_t)b << 32) | __float_as_uint(A), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ void await_map(const uint64_t* p, float& A, float& B) {
+    uint64_t v = 0;
+    for (int i = 0; i < kSpinLimit; ++i) {
+        v = __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if ((uint32_t)(v >> 32) != kEmpty) break;
+        __builtin_amdgcn_s_sleep(1);
+    }
+    A = __uint_as_float((uint32_t)v);
+    B = __uint_as_float((uint32_t)(v >> 32));
+}
+__device__ __forceinline__ float await_state(const uint32_t* p) {
+    uint32_t v = 0;
+    for (int i = 0; i < kSpinLimit; ++i) {
+        v = __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (v != kEmpty) break;
+        __builtin_amdgcn_s_sleep(1);
+    }
+    return __uint_as_float(v);
+}
+
+// sIn[column] = the state that enters tile number `k` of the walk.  `all` (in the threads with last_group set): its map.
+__device__ __forceinline__ void enter_tile(const Chain& ch, int64_t k, int64_t D, int64_t c, int nv, int CG, int cg, int rg, bool last_group,
+                                           const Map& all, Neighbours& nb, float (&own)[2][128], float (&sIn)[128]) {
+    const int p = (int)(k % kGroup), gp = (int)(k / kGroup % kGroup), RG = blockDim.x / CG;
+    const int64_t block = k / (kGroup * kGroup);
+    if (last_group)
 #pragma unroll
-    for (int i = 0; i < K; ++i) {
-        const int64_t r = r0 + i, p = REV ? g.N - 1 - r : r;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) a[i][e] = b[i][e] = 0.f;
-        if (r < g.N) {
-            ld4<T, WIDE>(gate + p * ldg, c, CG, D, a[i]);
-            ld4<T, WIDE>(x + p * ldx, c, CG, D, b[i]);
+        for (int e = 0; e < 4; ++e) {
+            own[0][cg * 4 + e] = all.A[e];
+            own[1][cg * 4 + e] = all.B[e];
+            if (p < kGroup - 1 && e < nv) publish(ch.tile + k * D + c + e, all.A[e], all.B[e]);
+        }
+    if (p == kGroup - 1) {                                               // the group's map, before anything else is waited for
+        for (int i = rg; i < kGroup - 1; i += RG)
+            for (int e = 0; e < nv; ++e) await_map(ch.tile + (k - p + i) * D + c + e, nb.A[i][cg * 4 + e], nb.B[i][cg * 4 + e]);
+        __syncthreads();
+        if (rg == 0 && gp < kGroup - 1)
+            for (int e = 0; e < nv; ++e) {
+                float A = nb.A[0][cg * 4 + e], B = nb.B[0][cg * 4 + e];
+                for (int i = 1; i < kGroup; ++i) {
+                    const float A2 = i < p ? nb.A[i][cg * 4 + e] : own[0][cg * 4 + e], B2 = i < p ? nb.B[i][cg * 4 + e] : own[1][cg * 4 + e];
+                    B = apply(A2, B2, B);
+                    A = A2 < 0.f || A < 0.f ? -1.f : A2 * A;
+                }
+                publish(ch.group + k / kGroup * D + c + e, A, B);
+            }
+    }
+    for (int i = rg; i < 2 * kGroup - 1; i += RG) {
+        const bool want = i < kGroup - 1 ? p < kGroup - 1 && i < p : i < 2 * kGroup - 2 ? i - (kGroup - 1) < gp : block > 0;
+        if (!want) continue;
+        for (int e = 0; e < nv; ++e) {
+            const int q = cg * 4 + e;
+            if (i < kGroup - 1) await_map(ch.tile + (k - p + i) * D + c + e, nb.A[i][q], nb.B[i][q]);
+            else if (i < 2 * kGroup - 2) await_map(ch.group + (k / kGroup - gp + i - (kGroup - 1)) * D + c + e, nb.A[i][q], nb.B[i][q]);
+            else nb.B[i][q] = await_state(ch.state + (block - 1) * D + c + e);
         }
     }
-    mark_tile<REV>(g, row0, rows, first, last);
-    float A[4] = {1.f, 1.f, 1.f, 1.f}, B[4] = {0.f, 0.f, 0.f, 0.f};
-    uint32_t cuts = 0;
+    __syncthreads();
+    if (rg == 0)
+        for (int e = 0; e < nv; ++e) {
+            const int q = cg * 4 + e;
+            float s = block > 0 ? nb.B[2 * kGroup - 2][q] : 0.f;
+            for (int i = 0; i < gp; ++i) s = apply(nb.A[kGroup - 1 + i][q], nb.B[kGroup - 1 + i][q], s);
+            for (int i = 0; i < p; ++i) s = apply(nb.A[i][q], nb.B[i][q], s);
+            sIn[q] = s;
+            if (p == kGroup - 1 && gp == kGroup - 1) {
+                uint32_t b = __float_as_uint(apply(own[0][q], own[1][q], s));
+                if (b == kEmpty) b = 0x7FC00000u;
+                __hip_atomic_store(ch.state + block * D + c + e, b, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            }
+        }
+    __syncthreads();
+}
+
+// The next (tile, column block) in the order of the walk; with a single tile there is nothing to order.  false: none left
+// (a ticket that another call's workgroups also draw from).
+__device__ __forceinline__ bool take_tile(const Chain& ch, int64_t n_tiles, int64_t& tile, int& cb) {
+    __shared__ uint32_t ticket;
+    uint32_t k = blockIdx.x;
+    const uint32_t ncb = gridDim.x / (uint32_t)n_tiles;
+    if (n_tiles > 1) {
+        if (threadIdx.x == 0) ticket = atomicAdd(ch.ticket, 1u);
+        __syncthreads();
+        k = ticket;
+    }
+    tile = k / ncb;
+    cb = (int)(k % ncb);
+    return k < gridDim.x;
+}
+
+__global__ __launch_bounds__(256) void k_scan_clear(uint4* p, int64_t n16, uint32_t* ticket) {
+    if (blockIdx.x == 0 && threadIdx.x == 0) *ticket = 0;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n16; i += (int64_t)gridDim.x * 256)
+        p[i] = make_uint4(kEmpty, kEmpty, kEmpty, kEmpty);
+}
+
+// Offset and step of a thread's rows in a matrix of pitch ld, from the tile's lowest row in memory
+template <bool REV>
+__device__ __forceinline__ uint32_t row_off(int r, int rows, int64_t ld, int c) { return (uint32_t)((REV ? rows - 1 - r : r) * (uint32_t)ld) + c; }
+
+// ------------------------------------------------------------------------------------------------ forward
+template <class T, bool REV>
+__global__ __launch_bounds__(kFwdThreads) void k_scan_fwd(const T* __restrict__ x, int64_t ldx, const T* __restrict__ gate, int64_t ldg,
+                                                          Segs g, int64_t D, const float* __restrict__ h0, int CG, Chain ch,
+                                                          int64_t n_tiles, T* __restrict__ h, int64_t ldh, float* __restrict__ h_last,
+                                                          float* __restrict__ heads) {
+    __shared__ int32_t first[4096 / 8], last[4096 / 8];
+    __shared__ uint32_t mask[kFwdThreads / 8];
+    __shared__ WaveMaps wm;
+    __shared__ Neighbours nb;
+    __shared__ float own[2][128], sIn[128];
+    int64_t tile;
+    int cb;
+    if (!take_tile(ch, n_tiles, tile, cb)) return;
+    const int RG = kFwdThreads / CG, cg = threadIdx.x & (CG - 1), rg = threadIdx.x / CG, rows = RG * kRows, r0 = rg * kRows;
+    const int64_t row0 = tile * rows, c0 = (int64_t)cb * (CG * 4), c = c0 + cg * 4, low = REV ? g.N - row0 - rows : row0;
+    const int64_t left = g.N - row0 - r0;
+    const Lane l{c + 4 <= D ? 4 : c < D ? (int)(D - c) : 0, left >= kRows ? kRows : left > 0 ? (int)left : 0};
+    float a[kRows][4], b[kRows][4];
+    load_rows(gate + low * ldg + c0, row_off<REV>(r0, rows, ldg, cg * 4), REV ? -(int32_t)ldg : (int32_t)ldg, l, a);
+    load_rows(x + low * ldx + c0, row_off<REV>(r0, rows, ldx, cg * 4), REV ? -(int32_t)ldx : (int32_t)ldx, l, b);
+    mark_tile<REV>(g, row0, RG, mask, first, last);
+    const uint32_t m = mask[rg], cuts = (m | m >> 16) & 0xFF;
+    Map f;
 #pragma unroll
-    for (int i = 0; i < K; ++i) {
-        const int f = first[rg * K + i];
-        float hs[4] = {0.f, 0.f, 0.f, 0.f};
-        if (f >= 0 && h0) ld4<float, false>(h0 + f * D, c, WIDE ? 1 : CG, D, hs);
-        if (f != -1) cuts |= 1u << i;
+    for (int e = 0; e < 4; ++e) { f.A[e] = 1.f; f.B[e] = 0.f; }
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             float ae, ce;
             gate_pair(a[i][e], ae, ce);
-            float be = ce * b[i][e];
-            if (f >= 0) be = fmaf(ae, hs[e], be);
-            if (f == -2) be = 0.f;
             a[i][e] = ae;
-            b[i][e] = be;
-            B[e] = f != -1 ? be : fmaf(ae, B[e], be);
-            A[e] *= ae;
+            b[i][e] = ce * b[i][e];
         }
-    }
+        if (i >= l.nrows) {                                              // no row: the map that changes nothing
 #pragma unroll
-    for (int e = 0; e < 4; ++e) { sA[threadIdx.x][e] = A[e]; sB[threadIdx.x][e] = B[e]; }
-    if (cg == 0) sCut[rg] = cuts != 0;
-    __syncthreads();
-    if (!APPLY) {
-        if (rg == 0) write_agg<false>(sA, sB, sCut, cg, CG, RG, agg, tile, c0, D, WIDE);
-        return;
-    }
-    float s[4] = {0.f, 0.f, 0.f, 0.f};
-    ld4<float, false>(heads + tile * D, c, WIDE ? 1 : CG, D, s);
-    enter_group<false>(sA, sB, sCut, cg, rg, CG, RG, s);
-#pragma unroll
-    for (int i = 0; i < K; ++i) {
-        const int64_t r = r0 + i, p = REV ? g.N - 1 - r : r;
-        const bool cut = (cuts >> i) & 1;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s[e] = cut ? b[i][e] : fmaf(a[i][e], s[e], b[i][e]);
-        if (r < g.N) {
-            st4<T, WIDE>(h + p * ldh, c, CG, D, s);
-            const int l = last[rg * K + i];
-            if (l >= 0 && h_last) st4<float, false>(h_last + l * D, c, WIDE ? 1 : CG, D, s);
+            for (int e = 0; e < 4; ++e) { a[i][e] = 1.f; b[i][e] = 0.f; }
         }
-    }
-    if (h_last)                                                          // segments without rows: the state passes through
-        for (int64_t k = tile; k < g.S; k += gridDim.x)
-            if (seg_lo<REV>(g, k) >= seg_lo<REV>(g, k + 1) && rg == 0) {
-                const int64_t sg = REV ? g.S - 1 - k : k;
-                float v[4] = {0.f, 0.f, 0.f, 0.f};
-                if (h0) ld4<float, false>(h0 + sg * D, c, WIDE ? 1 : CG, D, v);
-                st4<float, false>(h_last + sg * D, c, WIDE ? 1 : CG, D, v);
+        if ((cuts >> i) & 1) {
+            float s0[4] = {0.f, 0.f, 0.f, 0.f};
+            if ((m >> i) & 1) ld_state(h0, first[r0 + i], D, c, l.nv, s0);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                b[i][e] = (m >> i) & 1 ? fmaf(a[i][e], s0[e], b[i][e]) : 0.f;
+                a[i][e] = -1.f;
             }
-}
-
-// ------------------------------------------------------------------------------------------------ states between the tiles
-// heads[tile] = the state that enters the tile (from below, or from above with UP).  A workgroup: 32 columns, the tiles in
-// 32 slices of consecutive ones.
-template <bool UP>
-__global__ __launch_bounds__(kCarryCols* kCarrySlices) void k_scan_carry(TileAgg agg, int64_t n_tiles, int64_t D, float* __restrict__ heads) {
-    __shared__ float sA[kCarrySlices][kCarryCols], sB[kCarrySlices][kCarryCols];
-    __shared__ int32_t sCut[kCarrySlices];
-    const int tx = threadIdx.x % kCarryCols, ty = threadIdx.x / kCarryCols;
-    const int64_t c = (int64_t)blockIdx.x * kCarryCols + tx, per = (n_tiles + kCarrySlices - 1) / kCarrySlices;
-    const int64_t i0 = ty * per < n_tiles ? ty * per : n_tiles, i1 = i0 + per < n_tiles ? i0 + per : n_tiles;
-    float A = 1.f, B = 0.f;
-    int any = 0;
-    if (c < D)
-#pragma unroll 8
-        for (int64_t i = i0; i < i1; ++i) {
-            const int64_t t = UP ? n_tiles - 1 - i : i;
-            const float a = agg.ab[2 * t * D + c], b = agg.ab[(2 * t + 1) * D + c];
-            const bool cut = agg.cut[t] != 0;
-            any |= cut;
-            B = cut ? b : fmaf(a, B, b);
-            A = cut ? 0.f : a * A;
         }
-    sA[ty][tx] = A;
-    sB[ty][tx] = B;
-    if (tx == 0) sCut[ty] = any;
-    __syncthreads();
-    float s = 0.f;
-    for (int k = 0; k < ty; ++k) s = sCut[k] ? sB[k][tx] : fmaf(sA[k][tx], s, sB[k][tx]);
-    if (c < D)
-#pragma unroll 8
-        for (int64_t i = i0; i < i1; ++i) {
-            const int64_t t = UP ? n_tiles - 1 - i : i;
-            const float a = agg.ab[2 * t * D + c], b = agg.ab[(2 * t + 1) * D + c];
-            heads[t * D + c] = s;
-            s = agg.cut[t] ? b : fmaf(a, s, b);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            f.B[e] = apply(a[i][e], b[i][e], f.B[e]);
+            f.A[e] *= a[i][e];
         }
+    }
+    if (cuts)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) f.A[e] = -1.f;
+    const Map all = before_group<false>(f, CG, cg, wm);
+    if (n_tiles > 1) enter_tile(ch, tile, D, c, l.nv, CG, cg, rg, rg == RG - 1, all, nb, own, sIn);
+    float s[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s[e] = apply(f.A[e], f.B[e], n_tiles > 1 ? sIn[cg * 4 + e] : 0.f);
+    if (heads && (rg == 0 || rg == RG / 2) && row0 + r0 < g.N) st_state(heads, 2 * tile + (rg != 0), D, c, l.nv, s);
+    const uint32_t oh = row_off<REV>(r0, rows, ldh, cg * 4);
+    const int32_t sh = REV ? -(int32_t)ldh : (int32_t)ldh;
+    T* hb = h + low * ldh + c0;
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[e] = apply(a[i][e], b[i][e], s[e]);
+        store_row(hb, oh + i * sh, l, i, s);
+        if (((m >> 8) >> i) & 1 && h_last) st_state(h_last, last[r0 + i], D, c, l.nv, s);
+    }
+    if (h_last && rg == 0)                                               // segments without rows: the state passes through
+        for (int64_t k = tile; k < g.S; k += n_tiles)
+            if (seg_lo<REV>(g, k) >= seg_lo<REV>(g, k + 1)) {
+                const int64_t sg = REV ? g.S - 1 - k : k;
+                float v[4];
+                ld_state(h0, sg, D, c, l.nv, v);
+                st_state(h_last, sg, D, c, l.nv, v);
+            }
 }
 
 // ------------------------------------------------------------------------------------------------ backward
-// APPLY false: the tile's map of mu -> agg.  APPLY true: heads (h below the tile) and tails (mu above it) enter.
-template <class T, int K, bool WIDE, bool REV, bool APPLY>
-__global__ __launch_bounds__(512) void k_scan_bwd(const T* __restrict__ x, int64_t ldx, const T* __restrict__ gate, int64_t ldg,
-                                                  const T* __restrict__ dh, int64_t lddh, const float* __restrict__ dlast, Segs g,
-                                                  int64_t D, const float* __restrict__ h0, int CG, TileAgg agg,
-                                                  const float* __restrict__ heads, const float* __restrict__ tails, T* __restrict__ dx,
-                                                  int64_t lddx, T* __restrict__ dgate, int64_t lddg, float* __restrict__ dh0) {
-    __shared__ int32_t first[kTileElems / 8], last[kTileElems / 8];
-    __shared__ float sA[512][4], sB[512][4];
-    __shared__ int32_t sCut[64];
-    const int RG = 512 / CG, cg = threadIdx.x & (CG - 1), rg = threadIdx.x / CG, rows = RG * K;
-    const int64_t tile = blockIdx.x, row0 = tile * rows, c0 = (int64_t)blockIdx.y * (CG * 4), c = WIDE ? c0 + cg * 4 : c0 + cg;
-    const int64_t r0 = row0 + rg * K;
-    float a[K][4], cc[K][4], xx[K][4], d[K][4];
+// The walk for mu goes from the last tile to the first; h inside the tile comes from heads.  Kept per element: a, c, dh and
+// q = (h_before - x) a c, so dx = c lam and dgate = q lam.
+template <class T, bool REV>
+__global__ __launch_bounds__(kBwdThreads) void k_scan_bwd(const T* __restrict__ x, int64_t ldx, const T* __restrict__ gate, int64_t ldg,
+                                                          const T* __restrict__ dh, int64_t lddh, const float* __restrict__ dlast, Segs g,
+                                                          int64_t D, const float* __restrict__ h0, int CG, Chain ch, int64_t n_tiles,
+                                                          const float* __restrict__ heads, T* __restrict__ dx, int64_t lddx,
+                                                          T* __restrict__ dgate, int64_t lddg, float* __restrict__ dh0) {
+    __shared__ int32_t first[2048 / 8], last[2048 / 8];
+    __shared__ uint32_t mask[kBwdThreads / 8];
+    __shared__ WaveMaps wm;
+    __shared__ Neighbours nb;
+    __shared__ float own[2][128], sIn[128];
+    int64_t k;
+    int cb;
+    if (!take_tile(ch, n_tiles, k, cb)) return;
+    const int64_t tile = n_tiles - 1 - k;
+    const int RG = kBwdThreads / CG, cg = threadIdx.x & (CG - 1), rg = threadIdx.x / CG, rows = RG * kRows, r0 = rg * kRows;
+    const int64_t row0 = tile * rows, c0 = (int64_t)cb * (CG * 4), c = c0 + cg * 4, low = REV ? g.N - row0 - rows : row0;
+    const int64_t left = g.N - row0 - r0;
+    const Lane l{c + 4 <= D ? 4 : c < D ? (int)(D - c) : 0, left >= kRows ? kRows : left > 0 ? (int)left : 0};
+    float a[kRows][4], cc[kRows][4], q[kRows][4], d[kRows][4];
+    load_rows(gate + low * ldg + c0, row_off<REV>(r0, rows, ldg, cg * 4), REV ? -(int32_t)ldg : (int32_t)ldg, l, a);
+    load_rows(x + low * ldx + c0, row_off<REV>(r0, rows, ldx, cg * 4), REV ? -(int32_t)ldx : (int32_t)ldx, l, q);
+    if (dh) load_rows(dh + low * lddh + c0, row_off<REV>(r0, rows, lddh, cg * 4), REV ? -(int32_t)lddh : (int32_t)lddh, l, d);
+    else
 #pragma unroll
-    for (int i = 0; i < K; ++i) {
-        const int64_t r = r0 + i, p = REV ? g.N - 1 - r : r;
+        for (int i = 0; i < kRows; ++i)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) a[i][e] = xx[i][e] = d[i][e] = 0.f;
-        if (r < g.N) {
-            ld4<T, WIDE>(gate + p * ldg, c, CG, D, a[i]);
-            if (dh) ld4<T, WIDE>(dh + p * lddh, c, CG, D, d[i]);
-            if (APPLY) ld4<T, WIDE>(x + p * ldx, c, CG, D, xx[i]);
+            for (int e = 0; e < 4; ++e) d[i][e] = 0.f;
+    float s[4];
+    ld_state(heads, tile, D, c, l.nv, s);
+    mark_tile<REV>(g, row0, RG, mask, first, last);
+    const uint32_t m = mask[rg], none = m >> 16, fcut = (m | none) & 0xFF, lcut = (m >> 8 | none) & 0xFF;
+    Map f, u;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) { f.A[e] = u.A[e] = 1.f; f.B[e] = u.B[e] = 0.f; }
+    // h, to the row group's end
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) gate_pair(a[i][e], a[i][e], cc[i][e]);
+        if (i >= l.nrows) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) { a[i][e] = 1.f; cc[i][e] = 0.f; }
         }
-    }
-    mark_tile<REV>(g, row0, rows, first, last);
-    uint32_t fcuts = 0, lcuts = 0, none = 0;
-    float A[4] = {1.f, 1.f, 1.f, 1.f}, B[4] = {0.f, 0.f, 0.f, 0.f}, M[4] = {0.f, 0.f, 0.f, 0.f};
+        if ((fcut >> i) & 1) {
+            ld_state((m >> i) & 1 ? h0 : nullptr, (m >> i) & 1 ? first[r0 + i] : 0, D, c, l.nv, f.B);
 #pragma unroll
-    for (int i = K - 1; i >= 0; --i) {
-        const int f = first[rg * K + i], l = last[rg * K + i];
-        float ds[4] = {0.f, 0.f, 0.f, 0.f};
-        if (l >= 0 && dlast) ld4<float, false>(dlast + l * D, c, WIDE ? 1 : CG, D, ds);
-        if (f != -1) fcuts |= 1u << i;
-        if (f == -2) none |= 1u << i;
-        if (l >= 0 || f == -2) lcuts |= 1u << i;
+            for (int e = 0; e < 4; ++e) f.A[e] = -1.f;
+        }
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            gate_pair(a[i][e], a[i][e], cc[i][e]);
-            if (l >= 0) d[i][e] += ds[e];
-            if (f == -2) d[i][e] = 0.f;
-            A[e] *= a[i][e];
-            M[e] = a[i][e] * (l >= 0 || f == -2 ? d[i][e] : d[i][e] + M[e]);
+            f.B[e] = fmaf(a[i][e], f.B[e], cc[i][e] * q[i][e]);
+            f.A[e] *= a[i][e];
         }
     }
-    float s[4] = {0.f, 0.f, 0.f, 0.f};
-    float hp[K][4];
-    if (APPLY) {
-        // h before every row, from the state at the tile's head
+    if (fcut)
 #pragma unroll
-        for (int i = 0; i < K; ++i) {
-            const int f = first[rg * K + i];
-            float hs[4] = {0.f, 0.f, 0.f, 0.f};
-            if (f >= 0 && h0) ld4<float, false>(h0 + f * D, c, WIDE ? 1 : CG, D, hs);
+        for (int e = 0; e < 4; ++e) f.A[e] = -1.f;
+    // mu, to the row group's head
+#pragma unroll
+    for (int i = kRows - 1; i >= 0; --i) {
+        if ((lcut >> i) & 1) {
+            float ds[4] = {0.f, 0.f, 0.f, 0.f};
+            if (((m >> 8) >> i) & 1) ld_state(dlast, last[r0 + i], D, c, l.nv, ds);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                hp[i][e] = hs[e];
-                B[e] = fmaf(a[i][e], f == -1 ? B[e] : hs[e], cc[i][e] * xx[i][e]);
+                d[i][e] = (none >> i) & 1 ? 0.f : d[i][e] + ds[e];
+                u.B[e] = 0.f;
             }
         }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) { sA[threadIdx.x][e] = A[e]; sB[threadIdx.x][e] = B[e]; }
-        if (cg == 0) sCut[rg] = fcuts != 0;
-        __syncthreads();
-        ld4<float, false>(heads + tile * D, c, WIDE ? 1 : CG, D, s);
-        enter_group<false>(sA, sB, sCut, cg, rg, CG, RG, s);
-#pragma unroll
-        for (int i = 0; i < K; ++i) {
-            const bool cut = (fcuts >> i) & 1;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                if (!cut) hp[i][e] = s[e];
-                s[e] = fmaf(a[i][e], hp[i][e], cc[i][e] * xx[i][e]);
-            }
+        for (int e = 0; e < 4; ++e) {
+            u.B[e] = a[i][e] * (d[i][e] + u.B[e]);
+            u.A[e] *= a[i][e];
         }
-        __syncthreads();
     }
+    if (lcut)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) { sA[threadIdx.x][e] = A[e]; sB[threadIdx.x][e] = M[e]; }
-    if (cg == 0) sCut[rg] = lcuts != 0;
-    __syncthreads();
-    if (!APPLY) {
-        if (rg == 0) write_agg<true>(sA, sB, sCut, cg, CG, RG, agg, tile, c0, D, WIDE);
-        return;
-    }
+        for (int e = 0; e < 4; ++e) u.A[e] = -1.f;
+    before_group<false>(f, CG, cg, wm);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) s[e] = 0.f;
-    ld4<float, false>(tails + tile * D, c, WIDE ? 1 : CG, D, s);
-    enter_group<true>(sA, sB, sCut, cg, rg, CG, RG, s);
+    for (int e = 0; e < 4; ++e) s[e] = apply(f.A[e], f.B[e], s[e]);
+    __syncthreads();                                                     // wm is written again
+    const Map all = before_group<true>(u, CG, cg, wm);
 #pragma unroll
-    for (int i = K - 1; i >= 0; --i) {
-        const int64_t r = r0 + i, p = REV ? g.N - 1 - r : r;
-        const bool cut = (lcuts >> i) & 1, out = (none >> i) & 1;
-        float ox[4], og[4];
+    for (int i = 0; i < kRows; ++i) {
+        if ((fcut >> i) & 1) ld_state((m >> i) & 1 ? h0 : nullptr, (m >> i) & 1 ? first[r0 + i] : 0, D, c, l.nv, s);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const float lam = cut ? d[i][e] : d[i][e] + s[e];
-            ox[e] = out ? 0.f : cc[i][e] * lam;
-            og[e] = out ? 0.f : lam * (hp[i][e] - xx[i][e]) * (a[i][e] * cc[i][e]);
+            const float xi = q[i][e], hb = s[e];
+            s[e] = fmaf(a[i][e], hb, cc[i][e] * xi);
+            q[i][e] = (hb - xi) * (a[i][e] * cc[i][e]);
+        }
+        if ((none >> i) & 1) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) q[i][e] = cc[i][e] = 0.f;
+        }
+    }
+    if (n_tiles > 1) enter_tile(ch, k, D, c, l.nv, CG, cg, rg, rg == 0, all, nb, own, sIn);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s[e] = apply(u.A[e], u.B[e], n_tiles > 1 ? sIn[cg * 4 + e] : 0.f);
+    const uint32_t ox = row_off<REV>(r0, rows, lddx, cg * 4), og = row_off<REV>(r0, rows, lddg, cg * 4);
+    const int32_t sx = REV ? -(int32_t)lddx : (int32_t)lddx, sg = REV ? -(int32_t)lddg : (int32_t)lddg;
+    T *xb = dx + low * lddx + c0, *gb = dgate + low * lddg + c0;
+#pragma unroll
+    for (int i = kRows - 1; i >= 0; --i) {
+        float vx[4], vg[4];
+        if ((lcut >> i) & 1) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[e] = 0.f;
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float lam = d[i][e] + s[e];
+            vx[e] = cc[i][e] * lam;
+            vg[e] = q[i][e] * lam;
             s[e] = a[i][e] * lam;
         }
-        if (r < g.N) {
-            st4<T, WIDE>(dx + p * lddx, c, CG, D, ox);
-            st4<T, WIDE>(dgate + p * lddg, c, CG, D, og);
-            const int f = first[rg * K + i];
-            if (f >= 0 && dh0) st4<float, false>(dh0 + f * D, c, WIDE ? 1 : CG, D, s);
-        }
+        store_row(xb, ox + i * sx, l, i, vx);
+        store_row(gb, og + i * sg, l, i, vg);
+        if ((m >> i) & 1 && dh0) st_state(dh0, first[r0 + i], D, c, l.nv, s);
     }
-    if (dh0)
-        for (int64_t k = tile; k < g.S; k += gridDim.x)
-            if (seg_lo<REV>(g, k) >= seg_lo<REV>(g, k + 1) && rg == 0) {
-                const int64_t sg = REV ? g.S - 1 - k : k;
-                float v[4] = {0.f, 0.f, 0.f, 0.f};
-                if (dlast) ld4<float, false>(dlast + sg * D, c, WIDE ? 1 : CG, D, v);
-                st4<float, false>(dh0 + sg * D, c, WIDE ? 1 : CG, D, v);
+    if (dh0 && rg == 0)
+        for (int64_t j = tile; j < g.S; j += n_tiles)
+            if (seg_lo<REV>(g, j) >= seg_lo<REV>(g, j + 1)) {
+                const int64_t sgm = REV ? g.S - 1 - j : j;
+                float v[4];
+                ld_state(dlast, sgm, D, c, l.nv, v);
+                st_state(dh0, sgm, D, c, l.nv, v);
             }
 }
 
 // ------------------------------------------------------------------------------------------------ one row per segment
-template <class T, bool WIDE>
+template <class T, int W>
 __global__ __launch_bounds__(256) void k_scan_step(const T* __restrict__ x, int64_t ldx, const T* __restrict__ gate, int64_t ldg,
                                                    const float* state, int64_t lds_, int64_t D, T* __restrict__ h, int64_t ldh,
                                                    float* state_out, int64_t ldso) {
     const int64_t row = blockIdx.x;
-    const int64_t c0 = (int64_t)blockIdx.y * (WIDE ? 1024 : 256) + threadIdx.x * (WIDE ? 4 : 1);
+    const int64_t c0 = ((int64_t)blockIdx.y * 256 + threadIdx.x) * W;
     if (c0 >= D) return;
-    constexpr int W = WIDE ? 4 : 1;
     const BgVec<T, W> xv = *reinterpret_cast<const BgVec<T, W>*>(x + row * ldx + c0);
     const BgVec<T, W> gv = *reinterpret_cast<const BgVec<T, W>*>(gate + row * ldg + c0);
     BgVec<float, W> sv = *reinterpret_cast<const BgVec<float, W>*>(state + row * lds_ + c0);
@@ -402,8 +554,11 @@ __global__ __launch_bounds__(256) void k_scan_step(const T* __restrict__ x, int6
 
 // ------------------------------------------------------------------------------------------------ host side
 int column_groups(int64_t D) { return D > 64 ? 32 : D > 32 ? 16 : 8; }
-int64_t tile_rows(int64_t D) { return kTileElems / column_groups(D); }
-int64_t tiles_of(int64_t n, int64_t D) { return (n + tile_rows(D) - 1) / tile_rows(D); }
+int64_t tiles_of(int64_t n, int64_t D, int threads) {
+    const int64_t rows = threads * kRows / column_groups(D);
+    return (n + rows - 1) / rows;
+}
+unsigned column_blocks(int64_t D) { return (unsigned)((D + 4 * column_groups(D) - 1) / (4 * column_groups(D))); }
 
 template <class T>
 bool piece_ok(const void* p, int64_t ld, int64_t D) {
@@ -413,45 +568,50 @@ bool piece_ok(const void* p, int64_t ld, int64_t D) {
 int check_scan(int dtype, int64_t n, int64_t D, int64_t S, const int32_t* rowptr) {
     if (!bg_elem_size(dtype) || n < 0 || D < 0 || S < 0) return BG_ERR_ARG;
     if (!rowptr && (S == 0 ? n != 0 : n % S != 0)) return BG_ERR_ARG;
-    if (n > INT32_MAX || S >= INT32_MAX || D > (1 << 20) || tiles_of(n, D) * 512 > UINT32_MAX) return BG_ERR_SHAPE;
+    if (n > INT32_MAX || S >= INT32_MAX || D > (1 << 20)) return BG_ERR_SHAPE;
+    if (D > 0 && tiles_of(n, D, kBwdThreads) > (int64_t)(UINT32_MAX / kFwdThreads) / column_blocks(D)) return BG_ERR_SHAPE;   // work-items < 2^32
     return BG_OK;
 }
+bool pitch_ok(int64_t ld) { return ld <= (1 << 21); }      // a tile's offsets (at most 512 rows) fit 32 bits, in bytes too
 
-struct ScanWs { int64_t ab, cut, heads, bytes; };
-ScanWs scan_ws(int64_t n, int64_t D) {
-    const int64_t t = tiles_of(n, D);
+struct ScanWs { int64_t tile, group, state, ticket, bytes; };
+ScanWs scan_ws(int64_t n, int64_t D) {                      // of the backward pass, whose tiles are the smaller ones
+    const int64_t t = tiles_of(n, D, kBwdThreads);
     ScanWs w;
     int64_t at = 0;
     auto take = [&](int64_t bytes) { const int64_t o = at; at += (bytes + 255) / 256 * 256; return o; };
-    w.ab = take(8 * t * D);
-    w.cut = take(4 * t);
-    w.heads = take(4 * t * D);
+    w.tile = take(8 * t * D);
+    w.group = take(8 * (t / kGroup + 1) * D);
+    w.state = take(4 * (t / (kGroup * kGroup) + 1) * D);
+    w.ticket = take(4);
     w.bytes = at;
     return w;
 }
-
-template <class T, bool WIDE, bool REV>
-void launch_scan_fwd(const T* x, int64_t ldx, const T* gate, int64_t ldg, Segs g, int64_t D, const float* h0, TileAgg agg, float* heads,
-                     T* h, int64_t ldh, float* h_last, hipStream_t s) {
-    const int CG = column_groups(D);
-    const int64_t tiles = tiles_of(g.N, D);
-    const dim3 grid((unsigned)tiles, (unsigned)((D + 4 * CG - 1) / (4 * CG)));
-    k_scan_fwd<T, 16, WIDE, REV, false><<<grid, 256, 0, s>>>(x, ldx, gate, ldg, g, D, h0, CG, agg, nullptr, h, ldh, h_last);
-    k_scan_carry<false><<<(unsigned)((D + kCarryCols - 1) / kCarryCols), kCarryCols * kCarrySlices, 0, s>>>(agg, tiles, D, heads);
-    k_scan_fwd<T, 16, WIDE, REV, true><<<grid, 256, 0, s>>>(x, ldx, gate, ldg, g, D, h0, CG, agg, heads, h, ldh, h_last);
+// the words of `tiles` tiles emptied, the ticket at zero
+Chain make_chain(void* ws, int64_t n, int64_t D, int64_t tiles, hipStream_t s) {
+    const ScanWs w = scan_ws(n, D);
+    char* base = static_cast<char*>(ws);
+    const Chain ch{reinterpret_cast<uint64_t*>(base + w.tile), reinterpret_cast<uint64_t*>(base + w.group),
+                   reinterpret_cast<uint32_t*>(base + w.state), reinterpret_cast<uint32_t*>(base + w.ticket)};
+    if (tiles > 1) k_scan_clear<<<bg_grid_for(w.ticket / 16, 256 * 4, 2048), 256, 0, s>>>(static_cast<uint4*>(ws), w.ticket / 16, ch.ticket);
+    return ch;
 }
-template <class T, bool WIDE, bool REV>
+
+template <class T, bool REV>
+void launch_scan_fwd(const T* x, int64_t ldx, const T* gate, int64_t ldg, Segs g, int64_t D, const float* h0, void* ws, T* h, int64_t ldh,
+                     float* h_last, float* heads, hipStream_t s) {
+    const int64_t tiles = tiles_of(g.N, D, kFwdThreads);
+    const Chain ch = make_chain(ws, g.N, D, tiles, s);
+    k_scan_fwd<T, REV><<<(unsigned)tiles * column_blocks(D), kFwdThreads, 0, s>>>(x, ldx, gate, ldg, g, D, h0, column_groups(D), ch, tiles, h,
+                                                                                   ldh, h_last, heads);
+}
+template <class T, bool REV>
 void launch_scan_bwd(const T* x, int64_t ldx, const T* gate, int64_t ldg, const T* dh, int64_t lddh, const float* dlast, Segs g, int64_t D,
-                     const float* h0, TileAgg agg, const float* heads, float* tails, T* dx, int64_t lddx, T* dgate, int64_t lddg,
-                     float* dh0, hipStream_t s) {
-    const int CG = column_groups(D);
-    const int64_t tiles = tiles_of(g.N, D);
-    const dim3 grid((unsigned)tiles, (unsigned)((D + 4 * CG - 1) / (4 * CG)));
-    k_scan_bwd<T, 8, WIDE, REV, false><<<grid, 512, 0, s>>>(x, ldx, gate, ldg, dh, lddh, dlast, g, D, h0, CG, agg, heads, tails, dx, lddx,
-                                                            dgate, lddg, dh0);
-    k_scan_carry<true><<<(unsigned)((D + kCarryCols - 1) / kCarryCols), kCarryCols * kCarrySlices, 0, s>>>(agg, tiles, D, tails);
-    k_scan_bwd<T, 8, WIDE, REV, true><<<grid, 512, 0, s>>>(x, ldx, gate, ldg, dh, lddh, dlast, g, D, h0, CG, agg, heads, tails, dx, lddx,
-                                                           dgate, lddg, dh0);
+                     const float* h0, void* ws, const float* heads, T* dx, int64_t lddx, T* dgate, int64_t lddg, float* dh0, hipStream_t s) {
+    const int64_t tiles = tiles_of(g.N, D, kBwdThreads);
+    const Chain ch = make_chain(ws, g.N, D, tiles, s);
+    k_scan_bwd<T, REV><<<(unsigned)tiles * column_blocks(D), kBwdThreads, 0, s>>>(x, ldx, gate, ldg, dh, lddh, dlast, g, D, h0,
+                                                                                   column_groups(D), ch, tiles, heads, dx, lddx, dgate, lddg, dh0);
 }
 
 __global__ __launch_bounds__(256) void k_copy_or_zero(const float* __restrict__ src, float* __restrict__ dst, int64_t n) {
@@ -460,7 +620,7 @@ __global__ __launch_bounds__(256) void k_copy_or_zero(const float* __restrict__ 
 
 }  // namespace
 
-extern "C" int64_t bg_gated_scan_heads(int64_t n_rows, int64_t D) { return n_rows > 0 && D > 0 ? tiles_of(n_rows, D) * D : 0; }
+extern "C" int64_t bg_gated_scan_heads(int64_t n_rows, int64_t D) { return n_rows > 0 && D > 0 ? tiles_of(n_rows, D, kBwdThreads) * D : 0; }
 
 extern "C" int64_t bg_gated_scan_workspace(int64_t n_rows, int64_t D) { return n_rows > 0 && D > 0 ? scan_ws(n_rows, D).bytes : 0; }
 
@@ -470,6 +630,7 @@ extern "C" int bg_gated_scan_fwd(int dtype, const void* x, int64_t ldx, const vo
     const int rc = check_scan(dtype, n_rows, D, n_seg, rowptr);
     if (rc != BG_OK) return rc;
     if (ldx < D || ldg < D || ldh < D) return BG_ERR_ARG;
+    if (!pitch_ok(ldx) || !pitch_ok(ldg) || !pitch_ok(ldh)) return BG_ERR_SHAPE;
     if (D == 0) return BG_OK;
     hipStream_t s = (hipStream_t)stream;
     if (n_rows == 0) {                                     // no rows: the states pass through
@@ -480,20 +641,14 @@ extern "C" int bg_gated_scan_fwd(int dtype, const void* x, int64_t ldx, const vo
     }
     if (!x || !gate || !h || !ws) return BG_ERR_ARG;
     if (!bg_aligned16(ws)) return BG_ERR_ALIGN;
-    const ScanWs w = scan_ws(n_rows, D);
-    if (ws_bytes < w.bytes) return BG_ERR_SCRATCH;
-    char* base = static_cast<char*>(ws);
-    const TileAgg agg{reinterpret_cast<float*>(base + w.ab), reinterpret_cast<int32_t*>(base + w.cut)};
-    float* hd = heads ? heads : reinterpret_cast<float*>(base + w.heads);
+    if (ws_bytes < scan_ws(n_rows, D).bytes) return BG_ERR_SCRATCH;
     const Segs g{rowptr, n_seg, n_rows, rowptr ? 0 : n_rows / n_seg};
     return bg_dispatch_dtype(dtype, [&](auto z) -> int {
         typedef decltype(z) T;
         const T *xx = static_cast<const T*>(x), *gg = static_cast<const T*>(gate);
         T* hh = static_cast<T*>(h);
-        const bool wide = piece_ok<T>(x, ldx, D) && piece_ok<T>(gate, ldg, D) && piece_ok<T>(h, ldh, D);
-        auto go = [&](auto W, auto R) { launch_scan_fwd<T, decltype(W)::value, decltype(R)::value>(xx, ldx, gg, ldg, g, D, h0, agg, hd, hh, ldh, h_last, s); };
-        if (wide) reverse ? go(std::true_type(), std::true_type()) : go(std::true_type(), std::false_type());
-        else reverse ? go(std::false_type(), std::true_type()) : go(std::false_type(), std::false_type());
+        if (reverse) launch_scan_fwd<T, true>(xx, ldx, gg, ldg, g, D, h0, ws, hh, ldh, h_last, heads, s);
+        else launch_scan_fwd<T, false>(xx, ldx, gg, ldg, g, D, h0, ws, hh, ldh, h_last, heads, s);
         BG_LAUNCH_CHECK();
         return BG_OK;
     });
@@ -506,6 +661,7 @@ extern "C" int bg_gated_scan_bwd(int dtype, const void* x, int64_t ldx, const vo
     const int rc = check_scan(dtype, n_rows, D, n_seg, rowptr);
     if (rc != BG_OK) return rc;
     if (ldx < D || ldg < D || (dh && lddh < D) || lddx < D || lddg < D) return BG_ERR_ARG;
+    if (!pitch_ok(ldx) || !pitch_ok(ldg) || (dh && !pitch_ok(lddh)) || !pitch_ok(lddx) || !pitch_ok(lddg)) return BG_ERR_SHAPE;
     if (D == 0) return BG_OK;
     hipStream_t s = (hipStream_t)stream;
     if (n_rows == 0) {
@@ -516,24 +672,14 @@ extern "C" int bg_gated_scan_bwd(int dtype, const void* x, int64_t ldx, const vo
     }
     if (!x || !gate || !heads || !dx || !dgate || !ws) return BG_ERR_ARG;
     if (!bg_aligned16(ws)) return BG_ERR_ALIGN;
-    const ScanWs w = scan_ws(n_rows, D);
-    if (ws_bytes < w.bytes) return BG_ERR_SCRATCH;
-    char* base = static_cast<char*>(ws);
-    const TileAgg agg{reinterpret_cast<float*>(base + w.ab), reinterpret_cast<int32_t*>(base + w.cut)};
-    float* tails = reinterpret_cast<float*>(base + w.heads);
+    if (ws_bytes < scan_ws(n_rows, D).bytes) return BG_ERR_SCRATCH;
     const Segs g{rowptr, n_seg, n_rows, rowptr ? 0 : n_rows / n_seg};
     return bg_dispatch_dtype(dtype, [&](auto z) -> int {
         typedef decltype(z) T;
         const T *xx = static_cast<const T*>(x), *gg = static_cast<const T*>(gate), *dd = static_cast<const T*>(dh);
         T *ox = static_cast<T*>(dx), *og = static_cast<T*>(dgate);
-        const bool wide = piece_ok<T>(x, ldx, D) && piece_ok<T>(gate, ldg, D) && (!dh || piece_ok<T>(dh, lddh, D)) &&
-                          piece_ok<T>(dx, lddx, D) && piece_ok<T>(dgate, lddg, D);
-        auto go = [&](auto W, auto R) {
-            launch_scan_bwd<T, decltype(W)::value, decltype(R)::value>(xx, ldx, gg, ldg, dd, lddh, dlast, g, D, h0, agg, heads, tails, ox,
-                                                                       lddx, og, lddg, dh0, s);
-        };
-        if (wide) reverse ? go(std::true_type(), std::true_type()) : go(std::true_type(), std::false_type());
-        else reverse ? go(std::false_type(), std::true_type()) : go(std::false_type(), std::false_type());
+        if (reverse) launch_scan_bwd<T, true>(xx, ldx, gg, ldg, dd, lddh, dlast, g, D, h0, ws, heads, ox, lddx, og, lddg, dh0, s);
+        else launch_scan_bwd<T, false>(xx, ldx, gg, ldg, dd, lddh, dlast, g, D, h0, ws, heads, ox, lddx, og, lddg, dh0, s);
         BG_LAUNCH_CHECK();
         return BG_OK;
     });
@@ -552,8 +698,8 @@ extern "C" int bg_gated_scan_step(int dtype, const void* x, int64_t ldx, const v
         const bool wide = piece_ok<T>(x, ldx, D) && piece_ok<T>(gate, ldg, D) && piece_ok<T>(h, ldh, D) && piece_ok<float>(state, lds, D) &&
                           piece_ok<float>(state_out, ldso, D);
         const dim3 grid((unsigned)n, (unsigned)((D + (wide ? 1023 : 255)) / (wide ? 1024 : 256)));
-        if (wide) k_scan_step<T, true><<<grid, 256, 0, (hipStream_t)stream>>>(xx, ldx, gg, ldg, state, lds, D, hh, ldh, state_out, ldso);
-        else k_scan_step<T, false><<<grid, 256, 0, (hipStream_t)stream>>>(xx, ldx, gg, ldg, state, lds, D, hh, ldh, state_out, ldso);
+        if (wide) k_scan_step<T, 4><<<grid, 256, 0, (hipStream_t)stream>>>(xx, ldx, gg, ldg, state, lds, D, hh, ldh, state_out, ldso);
+        else k_scan_step<T, 1><<<grid, 256, 0, (hipStream_t)stream>>>(xx, ldx, gg, ldg, state, lds, D, hh, ldh, state_out, ldso);
         BG_LAUNCH_CHECK();
         return BG_OK;
     });
