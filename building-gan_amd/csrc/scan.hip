@@ -11,15 +11,16 @@
 // Rows are cut into tiles whatever the segments are.  A workgroup reads its tile ONCE, keeps it in registers, composes its
 // rows' maps, publishes the tile's map, finds the state that enters the tile from what the tiles before it published, and
 // walks its rows from there.  h is never read back: the backward pass rebuilds it from the fp32 state kept at the head of
-// every 2048 / CG rows.
+// every tile.
 #include "common.h"
 
 namespace {
 
-// A tile: THREADS / CG row groups of kRows rows times CG column groups of 4 columns.  16-byte (8-byte) pieces of a row per
-// lane; CG = 32 makes 512 B (256 B) of a row of fp32 (16-bit) elements, narrower matrices take fewer columns and more rows.
+// A tile: kThreads / CG row groups of kRows rows times CG column groups of 4 columns; a lane moves 16 bytes (8 bytes) of a
+// row of fp32 (16-bit) elements.  CG = 16 (64 columns: one wave can look after a tile's columns), fewer for narrow matrices.
 constexpr int kRows = 8;
-constexpr int kFwdThreads = 512, kBwdThreads = 256;
+constexpr int kThreads = 256, kWaves = kThreads / 64;
+constexpr int kMaxCols = 64;
 constexpr int kGroup = 8;                        // tiles of a group, groups of a block (see enter_tile)
 constexpr uint32_t kEmpty = 0xFFFFFFFFu;         // what unpublished words hold
 constexpr int kSpinLimit = 1 << 22;              // a wait of several seconds: only a workspace in use by another call gets there
@@ -36,31 +37,33 @@ __device__ __forceinline__ int64_t seg_lo(const Segs& g, int64_t j) {           
 }
 
 // mask[group]: bit i = row i of the group is a segment's first row, bit 8 + i = its last, bit 16 + i = in no segment;
-// first[row] / last[row] = that segment where the bit is set.  The segment of the tile's first row is found by a search
-// as wide as the workgroup: one round of loads for up to blockDim.x segments.
+// first[row] / last[row] = that segment where the bit is set.  One wave does it: the segment of the tile's first row is
+// found by a search 64 lanes wide.
 template <bool REV>
 __device__ __forceinline__ void mark_tile(const Segs& g, int64_t row0, int groups, uint32_t* mask, int32_t* first, int32_t* last) {
-    const int t = threadIdx.x, threads = blockDim.x, rows = groups * kRows;
+    const int t = threadIdx.x, rows = groups * kRows;
     const int64_t lo_all = seg_lo<REV>(g, 0), hi_all = seg_lo<REV>(g, g.S), end = row0 + rows;
-    if (t < groups) {
+    const bool inside = lo_all <= row0 && (hi_all >= end || hi_all == g.N);
+    for (int k = t; k < groups; k += 64) {
         uint32_t m = 0;
-        for (int i = 0; i < kRows; ++i) {
-            const int64_t r = row0 + t * kRows + i;
-            if (r < g.N && (r < lo_all || r >= hi_all)) m |= 0x10000u << i;
-        }
-        mask[t] = m;
+        if (!inside)
+            for (int i = 0; i < kRows; ++i) {
+                const int64_t r = row0 + k * kRows + i;
+                if (r < g.N && (r < lo_all || r >= hi_all)) m |= 0x10000u << i;
+            }
+        mask[k] = m;
     }
     int64_t lo = 0, hi = g.S;                    // lo -> how many segments begin at or before row0
     if (!g.ptr) lo = hi = g.T > 0 ? row0 / g.T + 1 : 0;
     while (lo < hi) {
-        const int64_t step = (hi - lo + threads - 1) / threads, j = lo + t * step;
-        const int c = __syncthreads_count(j < hi && seg_lo<REV>(g, j) <= row0);
+        const int64_t step = (hi - lo + 63) / 64, j = lo + t * step;
+        const int c = __popcll(__ballot(j < hi && seg_lo<REV>(g, j) <= row0));
         const int64_t nlo = c ? lo + (c - 1) * step + 1 : lo, nhi = c ? lo + c * step : lo;
         lo = nlo;
         hi = nhi < hi ? nhi : hi;
     }
-    __syncthreads();
-    for (int64_t j = (lo > 0 ? lo - 1 : 0) + t; j < g.S; j += threads) {
+    __builtin_amdgcn_wave_barrier();
+    for (int64_t j = (lo > 0 ? lo - 1 : 0) + t; j < g.S; j += 64) {
         const int64_t a = seg_lo<REV>(g, j), b = seg_lo<REV>(g, j + 1);
         if (a >= end) break;
         if (a >= b) continue;
@@ -74,17 +77,17 @@ __device__ __forceinline__ void mark_tile(const Segs& g, int64_t row0, int group
             atomicOr(&mask[(b - 1 - row0) / kRows], 0x100u << ((b - 1 - row0) % kRows));
         }
     }
-    __syncthreads();
 }
 
 // a = sigmoid(g), c = sigmoid(-g) without cancellation: e = exp(-|g|) <= 1, r = 1 / (1 + e); one of them is r, the other e r.
 // The product |g| log2(e) is carried in two parts and the reciprocal takes one Newton step: v_exp_f32 and v_rcp_f32 alone are
 // off by up to an ulp to one side, which a product over a long memory's a's would add up.
 __device__ __forceinline__ void gate_pair(float g, float& a, float& c) {
-    const float m = fabsf(g), p = m * -1.4426950408889634f;
+    const float m = __builtin_elementwise_minimum(fabsf(g), 110.f);      // e^-110 is 0 in fp32; a NaN stays one
+    const float p = m * -1.4426950408889634f;
     const float lo = fmaf(m, -1.9259629911266175e-8f, fmaf(m, -1.4426950408889634f, -p));
     float e = __builtin_amdgcn_exp2f(p);
-    e = m < 100.f ? fmaf(e, lo * 0.6931471805599453f, e) : e;            // (inf: the correction is inf - inf; NaN stays)
+    e = fmaf(e, lo * 0.6931471805599453f, e);
     const float s = 1.f + e, r0 = __builtin_amdgcn_rcpf(s), r = fmaf(r0, fmaf(-s, r0, 1.f), r0), er = e * r;
     a = g < 0.f ? er : r;
     c = g < 0.f ? r : er;
@@ -95,17 +98,19 @@ __device__ __forceinline__ void gate_pair(float g, float& a, float& c) {
 template <class T>
 struct __attribute__((packed, aligned(sizeof(T)))) Piece { T v[4]; };
 
-// What a thread touches of its tile: uniform base + 32-bit offset of its first row's piece + `step` elements a row.
+// What a thread touches of its tile: a base that is the same in every lane, the byte offset of its first row's piece, and a
+// step from row to row (32 bits: the address of an access is one addition).
 struct Lane {
     int nv, nrows;                               // columns (0 .. 4) and rows (0 .. kRows) that exist
     __device__ __forceinline__ bool whole() const { return nv == 4 && nrows == kRows; }
 };
 template <class T>
-__device__ __forceinline__ void load_rows(const T* __restrict__ base, uint32_t off, int32_t step, Lane l, float (&v)[kRows][4]) {
-    if (l.whole()) {
+__device__ __forceinline__ void load_rows(const T* __restrict__ base, uint32_t off, uint32_t step, Lane l, float fill, float (&v)[kRows][4]) {
+    const char* p = reinterpret_cast<const char*>(base);
+    if (__builtin_expect(l.whole(), 1)) {
         Piece<T> x[kRows];
 #pragma unroll
-        for (int i = 0; i < kRows; ++i) x[i] = *reinterpret_cast<const Piece<T>*>(base + (uint32_t)(off + i * step));
+        for (int i = 0; i < kRows; ++i) x[i] = *reinterpret_cast<const Piece<T>*>(p + (uint32_t)(off + i * step));
 #pragma unroll
         for (int i = 0; i < kRows; ++i)
 #pragma unroll
@@ -114,19 +119,27 @@ __device__ __forceinline__ void load_rows(const T* __restrict__ base, uint32_t o
 #pragma unroll
         for (int i = 0; i < kRows; ++i)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[i][e] = i < l.nrows && e < l.nv ? (float)base[(uint32_t)(off + i * step) + e] : 0.f;
+            for (int e = 0; e < 4; ++e)
+                v[i][e] = i < l.nrows && e < l.nv ? (float)reinterpret_cast<const T*>(p + (uint32_t)(off + i * step))[e] : fill;
     }
 }
 template <class T>
-__device__ __forceinline__ void store_row(T* __restrict__ base, uint32_t off, Lane l, int i, const float (&v)[4]) {
-    if (l.whole()) {
-        Piece<T> x;
+__device__ __forceinline__ void store_rows(T* __restrict__ base, uint32_t off, uint32_t step, Lane l, const float (&v)[kRows][4]) {
+    char* p = reinterpret_cast<char*>(base);
+    if (__builtin_expect(l.whole(), 1)) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x.v[e] = bg_round<T>(v[e]);
-        *reinterpret_cast<Piece<T>*>(base + off) = x;
-    } else if (i < l.nrows) {
+        for (int i = 0; i < kRows; ++i) {
+            Piece<T> x;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) if (e < l.nv) base[off + e] = bg_round<T>(v[e]);
+            for (int e = 0; e < 4; ++e) x.v[e] = bg_round<T>(v[i][e]);
+            *reinterpret_cast<Piece<T>*>(p + (uint32_t)(off + i * step)) = x;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < kRows; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (i < l.nrows && e < l.nv) reinterpret_cast<T*>(p + (uint32_t)(off + i * step))[e] = bg_round<T>(v[i][e]);
     }
 }
 // fp32 rows of [n, D] (states): rare, element by element
@@ -141,6 +154,14 @@ __device__ __forceinline__ void st_state(float* __restrict__ p, int64_t row, int
 
 // ------------------------------------------------------------------------------------------------ maps
 struct Map { float A[4], B[4]; };
+// The values stay, what was computed from them does not: keeps the compiler from holding products of a walk over the rows in
+// registers until a later walk can use them again (a multiplication is cheaper than 32 registers).
+__device__ __forceinline__ void forget(float (&v)[kRows][4]) {
+#pragma unroll
+    for (int i = 0; i < kRows; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) asm("" : "+v"(v[i][e]));
+}
 __device__ __forceinline__ void after(Map& m, const float (&A1)[4], const float (&B1)[4]) {          // m <- m o (A1, B1)
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -148,15 +169,20 @@ __device__ __forceinline__ void after(Map& m, const float (&A1)[4], const float 
         m.A[e] = m.A[e] < 0.f || A1[e] < 0.f ? -1.f : m.A[e] * A1[e];
     }
 }
+__device__ __forceinline__ void then(Map& m, float4 A, float4 B) {                   // m <- (A, B) o m
+    Map y{{A.x, A.y, A.z, A.w}, {B.x, B.y, B.z, B.w}};
+    after(y, m.A, m.B);
+    m = y;
+}
 __device__ __forceinline__ float apply(float A, float B, float s) { return A < 0.f ? B : fmaf(A, s, B); }
 
 // Maps of the workgroup's row groups: `m` becomes the map of everything before this thread's group (UP: the rows are walked
 // from the last group to the first).  In a wave by shuffles (64 / CG groups), then over the waves through LDS.  Returns the
 // map of the whole tile in the threads of the LAST group of the walk.
-struct WaveMaps { float A[kFwdThreads / 64][128], B[kFwdThreads / 64][128]; };
+struct WaveMaps { float4 A[kWaves][kMaxCols / 4], B[kWaves][kMaxCols / 4]; };
 template <bool UP>
 __device__ __forceinline__ Map before_group(Map& m, int CG, int cg, WaveMaps& w) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int at = UP ? 63 - lane : lane, edge = at / CG;                // this group's place in the wave's walk
     for (int o = 1; o * CG < 64; o <<= 1) {
         float A1[4], B1[4];
@@ -167,9 +193,10 @@ __device__ __forceinline__ Map before_group(Map& m, int CG, int cg, WaveMaps& w)
         }
         if (edge >= o) after(m, A1, B1);
     }
-    if (at >= 64 - CG)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) { w.A[wave][cg * 4 + e] = m.A[e]; w.B[wave][cg * 4 + e] = m.B[e]; }
+    if (at >= 64 - CG) {
+        w.A[wave][cg] = make_float4(m.A[0], m.A[1], m.A[2], m.A[3]);
+        w.B[wave][cg] = make_float4(m.B[0], m.B[1], m.B[2], m.B[3]);
+    }
     const Map own = m;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -178,17 +205,11 @@ __device__ __forceinline__ Map before_group(Map& m, int CG, int cg, WaveMaps& w)
         if (edge == 0) { m.A[e] = 1.f; m.B[e] = 0.f; }
     }
     __syncthreads();
-    Map pre;
+    Map pre{{1.f, 1.f, 1.f, 1.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
-    for (int e = 0; e < 4; ++e) { pre.A[e] = 1.f; pre.B[e] = 0.f; }
-    for (int k = 0; k < waves - 1; ++k) {
-        const int x = UP ? waves - 1 - k : k;
-        if (UP ? x <= wave : x >= wave) break;
-        Map y;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) { y.A[e] = w.A[x][cg * 4 + e]; y.B[e] = w.B[x][cg * 4 + e]; }
-        after(y, pre.A, pre.B);
-        pre = y;
+    for (int k = 0; k < kWaves - 1; ++k) {
+        const int x = UP ? kWaves - 1 - k : k;
+        if (UP ? x > wave : x < wave) then(pre, w.A[x][cg], w.B[x][cg]);
     }
     after(m, pre.A, pre.B);
     Map all = own;
@@ -204,85 +225,71 @@ __device__ __forceinline__ Map before_group(Map& m, int CG, int cg, WaveMaps& w)
 // that takes the nearest state it finds would).  A word is its own flag: (A, B) travel as one 64-bit relaxed atomic,
 // B's bits never being kEmpty; no fences, no other memory is ordered by them.
 struct Chain { uint64_t *tile, *group; uint32_t *state, *ticket; };
-struct Neighbours { float A[2 * kGroup - 1][128], B[2 * kGroup - 1][128]; };       // 7 tiles, 7 groups, the state (in B)
-
 __device__ __forceinline__ void publish(uint64_t* p, float A, float B) {
     uint32_t b = __float_as_uint(B);
     if (b == kEmpty) b = 0x7FC00000u;                                    // a NaN stays a NaN
     __hip_atomic_store(p, ((uint64_t)b << 32) | __float_as_uint(A), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
-__device__ __forceinline__ void await_map(const uint64_t* p, float& A, float& B) {
-    uint64_t v = 0;
-    for (int i = 0; i < kSpinLimit; ++i) {
-        v = __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        if ((uint32_t)(v >> 32) != kEmpty) break;
-        __builtin_amdgcn_s_sleep(1);
-    }
-    A = __uint_as_float((uint32_t)v);
-    B = __uint_as_float((uint32_t)(v >> 32));
+__device__ __forceinline__ uint64_t peek(const uint64_t* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+__device__ __forceinline__ bool is_empty(uint64_t v) { return (uint32_t)(v >> 32) == kEmpty; }
+// (A, B) <- (A2, B2) o (A, B) for the n words v[0], v[1], ..
+__device__ __forceinline__ void then_words(float& A, float& B, const uint64_t (&v)[kGroup - 1], int n) {
+#pragma unroll
+    for (int i = 0; i < kGroup - 1; ++i)
+        if (i < n) {
+            const float A2 = __uint_as_float((uint32_t)v[i]), B2 = __uint_as_float((uint32_t)(v[i] >> 32));
+            B = apply(A2, B2, B);
+            A = A2 < 0.f || A < 0.f ? -1.f : A2 * A;
+        }
 }
-__device__ __forceinline__ float await_state(const uint32_t* p) {
-    uint32_t v = 0;
-    for (int i = 0; i < kSpinLimit; ++i) {
-        v = __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        if (v != kEmpty) break;
+__device__ __forceinline__ void await_words(const uint64_t* p, int64_t D, int n, uint64_t (&v)[kGroup - 1]) {
+    for (int k = 0; k < kSpinLimit; ++k) {
+        bool wait = false;
+#pragma unroll
+        for (int i = 0; i < kGroup - 1; ++i) v[i] = i < n ? peek(p + i * D) : 0;
+#pragma unroll
+        for (int i = 0; i < kGroup - 1; ++i) wait |= is_empty(v[i]);
+        if (!wait) break;
         __builtin_amdgcn_s_sleep(1);
     }
-    return __uint_as_float(v);
 }
 
-// sIn[column] = the state that enters tile number `k` of the walk.  `all` (in the threads with last_group set): its map.
-__device__ __forceinline__ void enter_tile(const Chain& ch, int64_t k, int64_t D, int64_t c, int nv, int CG, int cg, int rg, bool last_group,
-                                           const Map& all, Neighbours& nb, float (&own)[2][128], float (&sIn)[128]) {
-    const int p = (int)(k % kGroup), gp = (int)(k / kGroup % kGroup), RG = blockDim.x / CG;
+// sIn[column] = the state that enters tile number `k` of the walk; own[0 / 1][column]: A / B of the tile's map.  The first
+// CG * 4 threads, one column each.  All that can be composed is composed before the state is waited for: a link of the chain
+// is one load, one fma and one store.
+__device__ __forceinline__ void enter_tile(const Chain& ch, int64_t k, int64_t D, int64_t c, const float* ownA, const float* ownB, float* sIn,
+                                           int col) {
+    const int p = (int)(k % kGroup), gp = (int)(k / kGroup % kGroup);
     const int64_t block = k / (kGroup * kGroup);
-    if (last_group)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            own[0][cg * 4 + e] = all.A[e];
-            own[1][cg * 4 + e] = all.B[e];
-            if (p < kGroup - 1 && e < nv) publish(ch.tile + k * D + c + e, all.A[e], all.B[e]);
+    const float oA = ownA[col], oB = ownB[col];
+    if (p < kGroup - 1) publish(ch.tile + k * D + c, oA, oB);
+    float A = 1.f, B = 0.f;                                              // of the group's tiles before this one
+    uint64_t v[kGroup - 1];
+    await_words(ch.tile + (k - p) * D + c, D, p, v);
+    then_words(A, B, v, p);
+    if (p == kGroup - 1 && gp < kGroup - 1)
+        publish(ch.group + k / kGroup * D + c, A < 0.f || oA < 0.f ? -1.f : oA * A, apply(oA, oB, B));
+    float gA = 1.f, gB = 0.f;                                            // of the block's groups before this one
+    await_words(ch.group + (k / kGroup - gp) * D + c, D, gp, v);
+    then_words(gA, gB, v, gp);
+    B = apply(A, B, gB);
+    A = A < 0.f || gA < 0.f ? -1.f : A * gA;
+    float s = 0.f;
+    if (block > 0 && !(A < 0.f)) {                                       // behind a cut the state from further back is not needed
+        uint32_t w = 0;
+        for (int i = 0; i < kSpinLimit; ++i) {
+            w = __hip_atomic_load(ch.state + (block - 1) * D + c, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            if (w != kEmpty) break;
         }
-    if (p == kGroup - 1) {                                               // the group's map, before anything else is waited for
-        for (int i = rg; i < kGroup - 1; i += RG)
-            for (int e = 0; e < nv; ++e) await_map(ch.tile + (k - p + i) * D + c + e, nb.A[i][cg * 4 + e], nb.B[i][cg * 4 + e]);
-        __syncthreads();
-        if (rg == 0 && gp < kGroup - 1)
-            for (int e = 0; e < nv; ++e) {
-                float A = nb.A[0][cg * 4 + e], B = nb.B[0][cg * 4 + e];
-                for (int i = 1; i < kGroup; ++i) {
-                    const float A2 = i < p ? nb.A[i][cg * 4 + e] : own[0][cg * 4 + e], B2 = i < p ? nb.B[i][cg * 4 + e] : own[1][cg * 4 + e];
-                    B = apply(A2, B2, B);
-                    A = A2 < 0.f || A < 0.f ? -1.f : A2 * A;
-                }
-                publish(ch.group + k / kGroup * D + c + e, A, B);
-            }
+        s = __uint_as_float(w);
     }
-    for (int i = rg; i < 2 * kGroup - 1; i += RG) {
-        const bool want = i < kGroup - 1 ? p < kGroup - 1 && i < p : i < 2 * kGroup - 2 ? i - (kGroup - 1) < gp : block > 0;
-        if (!want) continue;
-        for (int e = 0; e < nv; ++e) {
-            const int q = cg * 4 + e;
-            if (i < kGroup - 1) await_map(ch.tile + (k - p + i) * D + c + e, nb.A[i][q], nb.B[i][q]);
-            else if (i < 2 * kGroup - 2) await_map(ch.group + (k / kGroup - gp + i - (kGroup - 1)) * D + c + e, nb.A[i][q], nb.B[i][q]);
-            else nb.B[i][q] = await_state(ch.state + (block - 1) * D + c + e);
-        }
+    s = apply(A, B, s);
+    if (p == kGroup - 1 && gp == kGroup - 1) {
+        uint32_t b = __float_as_uint(apply(oA, oB, s));
+        if (b == kEmpty) b = 0x7FC00000u;
+        __hip_atomic_store(ch.state + block * D + c, b, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
-    __syncthreads();
-    if (rg == 0)
-        for (int e = 0; e < nv; ++e) {
-            const int q = cg * 4 + e;
-            float s = block > 0 ? nb.B[2 * kGroup - 2][q] : 0.f;
-            for (int i = 0; i < gp; ++i) s = apply(nb.A[kGroup - 1 + i][q], nb.B[kGroup - 1 + i][q], s);
-            for (int i = 0; i < p; ++i) s = apply(nb.A[i][q], nb.B[i][q], s);
-            sIn[q] = s;
-            if (p == kGroup - 1 && gp == kGroup - 1) {
-                uint32_t b = __float_as_uint(apply(own[0][q], own[1][q], s));
-                if (b == kEmpty) b = 0x7FC00000u;
-                __hip_atomic_store(ch.state + block * D + c + e, b, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            }
-        }
-    __syncthreads();
+    sIn[col] = s;
 }
 
 // The next (tile, column block) in the order of the walk; with a single tile there is nothing to order.  false: none left
@@ -294,7 +301,7 @@ __device__ __forceinline__ bool take_tile(const Chain& ch, int64_t n_tiles, int6
     if (n_tiles > 1) {
         if (threadIdx.x == 0) ticket = atomicAdd(ch.ticket, 1u);
         __syncthreads();
-        k = ticket;
+        k = __builtin_amdgcn_readfirstlane(ticket);                      // addresses of a tile are scalar arithmetic
     }
     tile = k / ncb;
     cb = (int)(k % ncb);
@@ -308,82 +315,108 @@ __global__ __launch_bounds__(256) void k_scan_clear(uint4* p, int64_t n16, uint3
 }
 
 // Offset and step of a thread's rows in a matrix of pitch ld, from the tile's lowest row in memory
-template <bool REV>
-__device__ __forceinline__ uint32_t row_off(int r, int rows, int64_t ld, int c) { return (uint32_t)((REV ? rows - 1 - r : r) * (uint32_t)ld) + c; }
+template <class T, bool REV>
+__device__ __forceinline__ uint32_t row_off(int r, int rows, int64_t ld, int c) {
+    return ((uint32_t)(REV ? rows - 1 - r : r) * (uint32_t)ld + (uint32_t)c) * (uint32_t)sizeof(T);
+}
+template <class T, bool REV>
+__device__ __forceinline__ uint32_t row_step(int64_t ld) { return (REV ? 0u - (uint32_t)ld : (uint32_t)ld) * (uint32_t)sizeof(T); }
 
 // ------------------------------------------------------------------------------------------------ forward
 template <class T, bool REV>
-__global__ __launch_bounds__(kFwdThreads) void k_scan_fwd(const T* __restrict__ x, int64_t ldx, const T* __restrict__ gate, int64_t ldg,
+__global__ __launch_bounds__(kThreads) void k_scan_fwd(const T* __restrict__ x, int64_t ldx, const T* __restrict__ gate, int64_t ldg,
                                                           Segs g, int64_t D, const float* __restrict__ h0, int CG, Chain ch,
                                                           int64_t n_tiles, T* __restrict__ h, int64_t ldh, float* __restrict__ h_last,
                                                           float* __restrict__ heads) {
-    __shared__ int32_t first[4096 / 8], last[4096 / 8];
-    __shared__ uint32_t mask[kFwdThreads / 8];
+    __shared__ int32_t first[2 * kThreads], last[2 * kThreads];            // kThreads / CG * kRows rows, CG >= 4
+    __shared__ uint32_t mask[kThreads / 4];
     __shared__ WaveMaps wm;
-    __shared__ Neighbours nb;
-    __shared__ float own[2][128], sIn[128];
+    __shared__ float4 own[2][kMaxCols / 4], sIn[kMaxCols / 4];
     int64_t tile;
     int cb;
     if (!take_tile(ch, n_tiles, tile, cb)) return;
-    const int RG = kFwdThreads / CG, cg = threadIdx.x & (CG - 1), rg = threadIdx.x / CG, rows = RG * kRows, r0 = rg * kRows;
+    const int RG = kThreads / CG, cg = threadIdx.x & (CG - 1), rg = threadIdx.x / CG, rows = RG * kRows, r0 = rg * kRows;
     const int64_t row0 = tile * rows, c0 = (int64_t)cb * (CG * 4), c = c0 + cg * 4, low = REV ? g.N - row0 - rows : row0;
     const int64_t left = g.N - row0 - r0;
     const Lane l{c + 4 <= D ? 4 : c < D ? (int)(D - c) : 0, left >= kRows ? kRows : left > 0 ? (int)left : 0};
+    if (threadIdx.x < 64) mark_tile<REV>(g, row0, RG, mask, first, last);
     float a[kRows][4], b[kRows][4];
-    load_rows(gate + low * ldg + c0, row_off<REV>(r0, rows, ldg, cg * 4), REV ? -(int32_t)ldg : (int32_t)ldg, l, a);
-    load_rows(x + low * ldx + c0, row_off<REV>(r0, rows, ldx, cg * 4), REV ? -(int32_t)ldx : (int32_t)ldx, l, b);
-    mark_tile<REV>(g, row0, RG, mask, first, last);
-    const uint32_t m = mask[rg], cuts = (m | m >> 16) & 0xFF;
-    Map f;
+    // where there is no row: a = 1, b = 0, the map that changes nothing
+    load_rows(gate + low * ldg + c0, row_off<T, REV>(r0, rows, ldg, cg * 4), row_step<T, REV>(ldg), l, __builtin_inff(), a);
+    load_rows(x + low * ldx + c0, row_off<T, REV>(r0, rows, ldx, cg * 4), row_step<T, REV>(ldx), l, 0.f, b);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) { f.A[e] = 1.f; f.B[e] = 0.f; }
-#pragma unroll
-    for (int i = 0; i < kRows; ++i) {
+    for (int i = 0; i < kRows; ++i)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            float ae, ce;
-            gate_pair(a[i][e], ae, ce);
-            a[i][e] = ae;
-            b[i][e] = ce * b[i][e];
+            float ce;
+            gate_pair(a[i][e], a[i][e], ce);
+            b[i][e] *= ce;
         }
-        if (i >= l.nrows) {                                              // no row: the map that changes nothing
+    __syncthreads();
+    const uint32_t m = mask[rg], cuts = (m | m >> 16) & 0xFF;
+    const bool any = __builtin_expect(__any(m != 0), 0);                 // most waves see no segment begin or end
+    Map f{{1.f, 1.f, 1.f, 1.f}, {0.f, 0.f, 0.f, 0.f}};
+    if (!any) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) { a[i][e] = 1.f; b[i][e] = 0.f; }
-        }
-        if ((cuts >> i) & 1) {
-            float s0[4] = {0.f, 0.f, 0.f, 0.f};
-            if ((m >> i) & 1) ld_state(h0, first[r0 + i], D, c, l.nv, s0);
+        for (int i = 0; i < kRows; ++i)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                b[i][e] = (m >> i) & 1 ? fmaf(a[i][e], s0[e], b[i][e]) : 0.f;
-                a[i][e] = -1.f;
+                f.B[e] = fmaf(a[i][e], f.B[e], b[i][e]);
+                f.A[e] *= a[i][e];
+            }
+    } else {
+#pragma unroll
+        for (int i = 0; i < kRows; ++i) {
+            if ((cuts >> i) & 1) {
+                float s0[4] = {0.f, 0.f, 0.f, 0.f};
+                if ((m >> i) & 1) ld_state(h0, first[r0 + i], D, c, l.nv, s0);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    b[i][e] = (m >> i) & 1 ? fmaf(a[i][e], s0[e], b[i][e]) : 0.f;
+                    a[i][e] = -1.f;
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                f.B[e] = apply(a[i][e], b[i][e], f.B[e]);
+                f.A[e] *= a[i][e];
             }
         }
+        if (cuts)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            f.B[e] = apply(a[i][e], b[i][e], f.B[e]);
-            f.A[e] *= a[i][e];
+            for (int e = 0; e < 4; ++e) f.A[e] = -1.f;
+    }
+    const Map all = before_group<false>(f, CG, cg, wm);
+    float s[4] = {0.f, 0.f, 0.f, 0.f};
+    if (n_tiles > 1) {
+        if (rg == RG - 1) {
+            own[0][cg] = make_float4(all.A[0], all.A[1], all.A[2], all.A[3]);
+            own[1][cg] = make_float4(all.B[0], all.B[1], all.B[2], all.B[3]);
+        }
+        __syncthreads();
+        if ((int)threadIdx.x < CG * 4 && c0 + threadIdx.x < D)
+            enter_tile(ch, tile, D, c0 + threadIdx.x, &own[0][0].x, &own[1][0].x, &sIn[0].x, threadIdx.x);
+        __syncthreads();
+        const float4 v = sIn[cg];
+        s[0] = v.x; s[1] = v.y; s[2] = v.z; s[3] = v.w;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s[e] = apply(f.A[e], f.B[e], s[e]);
+    if (heads && rg == 0) st_state(heads, tile, D, c, l.nv, s);
+    if (!any) {
+#pragma unroll
+        for (int i = 0; i < kRows; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) b[i][e] = s[e] = fmaf(a[i][e], s[e], b[i][e]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < kRows; ++i) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) b[i][e] = s[e] = apply(a[i][e], b[i][e], s[e]);
+            if (((m >> 8) >> i) & 1 && h_last) st_state(h_last, last[r0 + i], D, c, l.nv, s);
         }
     }
-    if (cuts)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) f.A[e] = -1.f;
-    const Map all = before_group<false>(f, CG, cg, wm);
-    if (n_tiles > 1) enter_tile(ch, tile, D, c, l.nv, CG, cg, rg, rg == RG - 1, all, nb, own, sIn);
-    float s[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) s[e] = apply(f.A[e], f.B[e], n_tiles > 1 ? sIn[cg * 4 + e] : 0.f);
-    if (heads && (rg == 0 || rg == RG / 2) && row0 + r0 < g.N) st_state(heads, 2 * tile + (rg != 0), D, c, l.nv, s);
-    const uint32_t oh = row_off<REV>(r0, rows, ldh, cg * 4);
-    const int32_t sh = REV ? -(int32_t)ldh : (int32_t)ldh;
-    T* hb = h + low * ldh + c0;
-#pragma unroll
-    for (int i = 0; i < kRows; ++i) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s[e] = apply(a[i][e], b[i][e], s[e]);
-        store_row(hb, oh + i * sh, l, i, s);
-        if (((m >> 8) >> i) & 1 && h_last) st_state(h_last, last[r0 + i], D, c, l.nv, s);
-    }
+    store_rows(h + low * ldh + c0, row_off<T, REV>(r0, rows, ldh, cg * 4), row_step<T, REV>(ldh), l, b);
     if (h_last && rg == 0)                                               // segments without rows: the state passes through
         for (int64_t k = tile; k < g.S; k += n_tiles)
             if (seg_lo<REV>(g, k) >= seg_lo<REV>(g, k + 1)) {
@@ -398,67 +431,58 @@ __global__ __launch_bounds__(kFwdThreads) void k_scan_fwd(const T* __restrict__ 
 // The walk for mu goes from the last tile to the first; h inside the tile comes from heads.  Kept per element: a, c, dh and
 // q = (h_before - x) a c, so dx = c lam and dgate = q lam.
 template <class T, bool REV>
-__global__ __launch_bounds__(kBwdThreads) void k_scan_bwd(const T* __restrict__ x, int64_t ldx, const T* __restrict__ gate, int64_t ldg,
-                                                          const T* __restrict__ dh, int64_t lddh, const float* __restrict__ dlast, Segs g,
-                                                          int64_t D, const float* __restrict__ h0, int CG, Chain ch, int64_t n_tiles,
-                                                          const float* __restrict__ heads, T* __restrict__ dx, int64_t lddx,
-                                                          T* __restrict__ dgate, int64_t lddg, float* __restrict__ dh0) {
-    __shared__ int32_t first[2048 / 8], last[2048 / 8];
-    __shared__ uint32_t mask[kBwdThreads / 8];
+__global__ __launch_bounds__(kThreads) void k_scan_bwd(const T* __restrict__ x, int64_t ldx, const T* __restrict__ gate, int64_t ldg,
+                                                             const T* __restrict__ dh, int64_t lddh, const float* __restrict__ dlast,
+                                                             Segs g, int64_t D, const float* __restrict__ h0, int CG, Chain ch,
+                                                             int64_t n_tiles, const float* __restrict__ heads, T* __restrict__ dx,
+                                                             int64_t lddx, T* __restrict__ dgate, int64_t lddg, float* __restrict__ dh0) {
+    __shared__ int32_t first[2 * kThreads], last[2 * kThreads];
+    __shared__ uint32_t mask[kThreads / 4];
     __shared__ WaveMaps wm;
-    __shared__ Neighbours nb;
-    __shared__ float own[2][128], sIn[128];
+    __shared__ float4 own[2][kMaxCols / 4], sIn[kMaxCols / 4];
     int64_t k;
     int cb;
     if (!take_tile(ch, n_tiles, k, cb)) return;
     const int64_t tile = n_tiles - 1 - k;
-    const int RG = kBwdThreads / CG, cg = threadIdx.x & (CG - 1), rg = threadIdx.x / CG, rows = RG * kRows, r0 = rg * kRows;
+    const int RG = kThreads / CG, cg = threadIdx.x & (CG - 1), rg = threadIdx.x / CG, rows = RG * kRows, r0 = rg * kRows;
     const int64_t row0 = tile * rows, c0 = (int64_t)cb * (CG * 4), c = c0 + cg * 4, low = REV ? g.N - row0 - rows : row0;
     const int64_t left = g.N - row0 - r0;
     const Lane l{c + 4 <= D ? 4 : c < D ? (int)(D - c) : 0, left >= kRows ? kRows : left > 0 ? (int)left : 0};
-    float a[kRows][4], cc[kRows][4], q[kRows][4], d[kRows][4];
-    load_rows(gate + low * ldg + c0, row_off<REV>(r0, rows, ldg, cg * 4), REV ? -(int32_t)ldg : (int32_t)ldg, l, a);
-    load_rows(x + low * ldx + c0, row_off<REV>(r0, rows, ldx, cg * 4), REV ? -(int32_t)ldx : (int32_t)ldx, l, q);
-    if (dh) load_rows(dh + low * lddh + c0, row_off<REV>(r0, rows, lddh, cg * 4), REV ? -(int32_t)lddh : (int32_t)lddh, l, d);
+    if (threadIdx.x < 64) mark_tile<REV>(g, row0, RG, mask, first, last);
+    float a[kRows][4], cc[kRows][4], q[kRows][4], d[kRows][4], s[4];
+    load_rows(gate + low * ldg + c0, row_off<T, REV>(r0, rows, ldg, cg * 4), row_step<T, REV>(ldg), l, __builtin_inff(), a);
+    load_rows(x + low * ldx + c0, row_off<T, REV>(r0, rows, ldx, cg * 4), row_step<T, REV>(ldx), l, 0.f, q);
+    if (dh) load_rows(dh + low * lddh + c0, row_off<T, REV>(r0, rows, lddh, cg * 4), row_step<T, REV>(lddh), l, 0.f, d);
     else
 #pragma unroll
         for (int i = 0; i < kRows; ++i)
 #pragma unroll
             for (int e = 0; e < 4; ++e) d[i][e] = 0.f;
-    float s[4];
     ld_state(heads, tile, D, c, l.nv, s);
-    mark_tile<REV>(g, row0, RG, mask, first, last);
-    const uint32_t m = mask[rg], none = m >> 16, fcut = (m | none) & 0xFF, lcut = (m >> 8 | none) & 0xFF;
-    Map f, u;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) { f.A[e] = u.A[e] = 1.f; f.B[e] = u.B[e] = 0.f; }
-    // h, to the row group's end
-#pragma unroll
-    for (int i = 0; i < kRows; ++i) {
+    for (int i = 0; i < kRows; ++i)
 #pragma unroll
         for (int e = 0; e < 4; ++e) gate_pair(a[i][e], a[i][e], cc[i][e]);
-        if (i >= l.nrows) {
+    __syncthreads();
+    const uint32_t m = mask[rg], none = m >> 16, fcut = (m | none) & 0xFF, lcut = (m >> 8 | none) & 0xFF;
+    const bool any = __builtin_expect(__any(m != 0), 0);
+    Map f{{1.f, 1.f, 1.f, 1.f}, {0.f, 0.f, 0.f, 0.f}}, u;                // of h down to the group's end, of mu up to its head
 #pragma unroll
-            for (int e = 0; e < 4; ++e) { a[i][e] = 1.f; cc[i][e] = 0.f; }
-        }
-        if ((fcut >> i) & 1) {
-            ld_state((m >> i) & 1 ? h0 : nullptr, (m >> i) & 1 ? first[r0 + i] : 0, D, c, l.nv, f.B);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) f.A[e] = -1.f;
-        }
+    for (int i = 0; i < kRows; ++i) {
+        if (any && (fcut >> i) & 1) ld_state((m >> i) & 1 ? h0 : nullptr, (m >> i) & 1 ? first[r0 + i] : 0, D, c, l.nv, f.B);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             f.B[e] = fmaf(a[i][e], f.B[e], cc[i][e] * q[i][e]);
             f.A[e] *= a[i][e];
         }
     }
-    if (fcut)
+    forget(a);
+    u = f;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) f.A[e] = -1.f;
-    // mu, to the row group's head
+    for (int e = 0; e < 4; ++e) u.B[e] = 0.f;
 #pragma unroll
     for (int i = kRows - 1; i >= 0; --i) {
-        if ((lcut >> i) & 1) {
+        if (any && (lcut >> i) & 1) {
             float ds[4] = {0.f, 0.f, 0.f, 0.f};
             if (((m >> 8) >> i) & 1) ld_state(dlast, last[r0 + i], D, c, l.nv, ds);
 #pragma unroll
@@ -468,57 +492,70 @@ __global__ __launch_bounds__(kBwdThreads) void k_scan_bwd(const T* __restrict__ 
             }
         }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            u.B[e] = a[i][e] * (d[i][e] + u.B[e]);
-            u.A[e] *= a[i][e];
-        }
+        for (int e = 0; e < 4; ++e) u.B[e] = a[i][e] * (d[i][e] + u.B[e]);
     }
-    if (lcut)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) u.A[e] = -1.f;
+    for (int e = 0; e < 4; ++e) {
+        if (fcut) f.A[e] = -1.f;
+        if (lcut) u.A[e] = -1.f;
+    }
     before_group<false>(f, CG, cg, wm);
 #pragma unroll
     for (int e = 0; e < 4; ++e) s[e] = apply(f.A[e], f.B[e], s[e]);
     __syncthreads();                                                     // wm is written again
     const Map all = before_group<true>(u, CG, cg, wm);
+    forget(cc);
 #pragma unroll
     for (int i = 0; i < kRows; ++i) {
-        if ((fcut >> i) & 1) ld_state((m >> i) & 1 ? h0 : nullptr, (m >> i) & 1 ? first[r0 + i] : 0, D, c, l.nv, s);
+        if (any && (fcut >> i) & 1) ld_state((m >> i) & 1 ? h0 : nullptr, (m >> i) & 1 ? first[r0 + i] : 0, D, c, l.nv, s);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const float xi = q[i][e], hb = s[e];
             s[e] = fmaf(a[i][e], hb, cc[i][e] * xi);
             q[i][e] = (hb - xi) * (a[i][e] * cc[i][e]);
         }
-        if ((none >> i) & 1) {
+        if (any && (none >> i) & 1) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) q[i][e] = cc[i][e] = 0.f;
         }
     }
-    if (n_tiles > 1) enter_tile(ch, k, D, c, l.nv, CG, cg, rg, rg == 0, all, nb, own, sIn);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) s[e] = apply(u.A[e], u.B[e], n_tiles > 1 ? sIn[cg * 4 + e] : 0.f);
-    const uint32_t ox = row_off<REV>(r0, rows, lddx, cg * 4), og = row_off<REV>(r0, rows, lddg, cg * 4);
-    const int32_t sx = REV ? -(int32_t)lddx : (int32_t)lddx, sg = REV ? -(int32_t)lddg : (int32_t)lddg;
-    T *xb = dx + low * lddx + c0, *gb = dgate + low * lddg + c0;
+    for (int e = 0; e < 4; ++e) s[e] = 0.f;
+    if (n_tiles > 1) {
+        if (rg == 0) {
+            own[0][cg] = make_float4(all.A[0], all.A[1], all.A[2], all.A[3]);
+            own[1][cg] = make_float4(all.B[0], all.B[1], all.B[2], all.B[3]);
+        }
+        __syncthreads();
+        if ((int)threadIdx.x < CG * 4 && c0 + threadIdx.x < D)
+            enter_tile(ch, k, D, c0 + threadIdx.x, &own[0][0].x, &own[1][0].x, &sIn[0].x, threadIdx.x);
+        __syncthreads();
+        const float4 v = sIn[cg];
+        s[0] = v.x; s[1] = v.y; s[2] = v.z; s[3] = v.w;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s[e] = apply(u.A[e], u.B[e], s[e]);
 #pragma unroll
     for (int i = kRows - 1; i >= 0; --i) {
-        float vx[4], vg[4];
-        if ((lcut >> i) & 1) {
+        if (any && (lcut >> i) & 1) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) s[e] = 0.f;
         }
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const float lam = d[i][e] + s[e];
-            vx[e] = cc[i][e] * lam;
-            vg[e] = q[i][e] * lam;
+            cc[i][e] *= lam;
+            q[i][e] *= lam;
             s[e] = a[i][e] * lam;
         }
-        store_row(xb, ox + i * sx, l, i, vx);
-        store_row(gb, og + i * sg, l, i, vg);
-        if ((m >> i) & 1 && dh0) st_state(dh0, first[r0 + i], D, c, l.nv, s);
+        if (any && (none >> i) & 1) {                                    // (a NaN of a row in no segment: 0 all the same)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) q[i][e] = cc[i][e] = 0.f;
+        }
+        if (any && (m >> i) & 1 && dh0) st_state(dh0, first[r0 + i], D, c, l.nv, s);
     }
+    store_rows(dx + low * lddx + c0, row_off<T, REV>(r0, rows, lddx, cg * 4), row_step<T, REV>(lddx), l, cc);
+    store_rows(dgate + low * lddg + c0, row_off<T, REV>(r0, rows, lddg, cg * 4), row_step<T, REV>(lddg), l, q);
     if (dh0 && rg == 0)
         for (int64_t j = tile; j < g.S; j += n_tiles)
             if (seg_lo<REV>(g, j) >= seg_lo<REV>(g, j + 1)) {
@@ -553,9 +590,9 @@ __global__ __launch_bounds__(256) void k_scan_step(const T* __restrict__ x, int6
 }
 
 // ------------------------------------------------------------------------------------------------ host side
-int column_groups(int64_t D) { return D > 64 ? 32 : D > 32 ? 16 : 8; }
-int64_t tiles_of(int64_t n, int64_t D, int threads) {
-    const int64_t rows = threads * kRows / column_groups(D);
+int column_groups(int64_t D) { return D > 32 ? 16 : D > 16 ? 8 : 4; }
+int64_t tiles_of(int64_t n, int64_t D) {
+    const int64_t rows = kThreads * kRows / column_groups(D);
     return (n + rows - 1) / rows;
 }
 unsigned column_blocks(int64_t D) { return (unsigned)((D + 4 * column_groups(D) - 1) / (4 * column_groups(D))); }
@@ -569,14 +606,14 @@ int check_scan(int dtype, int64_t n, int64_t D, int64_t S, const int32_t* rowptr
     if (!bg_elem_size(dtype) || n < 0 || D < 0 || S < 0) return BG_ERR_ARG;
     if (!rowptr && (S == 0 ? n != 0 : n % S != 0)) return BG_ERR_ARG;
     if (n > INT32_MAX || S >= INT32_MAX || D > (1 << 20)) return BG_ERR_SHAPE;
-    if (D > 0 && tiles_of(n, D, kBwdThreads) > (int64_t)(UINT32_MAX / kFwdThreads) / column_blocks(D)) return BG_ERR_SHAPE;   // work-items < 2^32
+    if (D > 0 && tiles_of(n, D) > (int64_t)(UINT32_MAX / kThreads) / column_blocks(D)) return BG_ERR_SHAPE;   // work-items < 2^32
     return BG_OK;
 }
 bool pitch_ok(int64_t ld) { return ld <= (1 << 21); }      // a tile's offsets (at most 512 rows) fit 32 bits, in bytes too
 
 struct ScanWs { int64_t tile, group, state, ticket, bytes; };
-ScanWs scan_ws(int64_t n, int64_t D) {                      // of the backward pass, whose tiles are the smaller ones
-    const int64_t t = tiles_of(n, D, kBwdThreads);
+ScanWs scan_ws(int64_t n, int64_t D) {
+    const int64_t t = tiles_of(n, D);
     ScanWs w;
     int64_t at = 0;
     auto take = [&](int64_t bytes) { const int64_t o = at; at += (bytes + 255) / 256 * 256; return o; };
@@ -600,17 +637,17 @@ Chain make_chain(void* ws, int64_t n, int64_t D, int64_t tiles, hipStream_t s) {
 template <class T, bool REV>
 void launch_scan_fwd(const T* x, int64_t ldx, const T* gate, int64_t ldg, Segs g, int64_t D, const float* h0, void* ws, T* h, int64_t ldh,
                      float* h_last, float* heads, hipStream_t s) {
-    const int64_t tiles = tiles_of(g.N, D, kFwdThreads);
+    const int64_t tiles = tiles_of(g.N, D);
     const Chain ch = make_chain(ws, g.N, D, tiles, s);
-    k_scan_fwd<T, REV><<<(unsigned)tiles * column_blocks(D), kFwdThreads, 0, s>>>(x, ldx, gate, ldg, g, D, h0, column_groups(D), ch, tiles, h,
+    k_scan_fwd<T, REV><<<(unsigned)tiles * column_blocks(D), kThreads, 0, s>>>(x, ldx, gate, ldg, g, D, h0, column_groups(D), ch, tiles, h,
                                                                                    ldh, h_last, heads);
 }
 template <class T, bool REV>
 void launch_scan_bwd(const T* x, int64_t ldx, const T* gate, int64_t ldg, const T* dh, int64_t lddh, const float* dlast, Segs g, int64_t D,
                      const float* h0, void* ws, const float* heads, T* dx, int64_t lddx, T* dgate, int64_t lddg, float* dh0, hipStream_t s) {
-    const int64_t tiles = tiles_of(g.N, D, kBwdThreads);
+    const int64_t tiles = tiles_of(g.N, D);
     const Chain ch = make_chain(ws, g.N, D, tiles, s);
-    k_scan_bwd<T, REV><<<(unsigned)tiles * column_blocks(D), kBwdThreads, 0, s>>>(x, ldx, gate, ldg, dh, lddh, dlast, g, D, h0,
+    k_scan_bwd<T, REV><<<(unsigned)tiles * column_blocks(D), kThreads, 0, s>>>(x, ldx, gate, ldg, dh, lddh, dlast, g, D, h0,
                                                                                    column_groups(D), ch, tiles, heads, dx, lddx, dgate, lddg, dh0);
 }
 
@@ -620,7 +657,7 @@ __global__ __launch_bounds__(256) void k_copy_or_zero(const float* __restrict__ 
 
 }  // namespace
 
-extern "C" int64_t bg_gated_scan_heads(int64_t n_rows, int64_t D) { return n_rows > 0 && D > 0 ? tiles_of(n_rows, D, kBwdThreads) * D : 0; }
+extern "C" int64_t bg_gated_scan_heads(int64_t n_rows, int64_t D) { return n_rows > 0 && D > 0 ? tiles_of(n_rows, D) * D : 0; }
 
 extern "C" int64_t bg_gated_scan_workspace(int64_t n_rows, int64_t D) { return n_rows > 0 && D > 0 ? scan_ws(n_rows, D).bytes : 0; }
 
