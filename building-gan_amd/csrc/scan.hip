@@ -37,10 +37,11 @@ __device__ __forceinline__ int64_t seg_lo(const Segs& g, int64_t j) {           
 }
 
 // mask[group]: bit i = row i of the group is a segment's first row, bit 8 + i = its last, bit 16 + i = in no segment;
-// first[row] / last[row] = that segment where the bit is set.  One wave does it: the segment of the tile's first row is
+// first[row] / last[row] = that segment where the bit is set; border: any bit at all.  One wave does it: the segment of the tile's first row is
 // found by a search 64 lanes wide.
 template <bool REV>
-__device__ __forceinline__ void mark_tile(const Segs& g, int64_t row0, int groups, uint32_t* mask, int32_t* first, int32_t* last) {
+__device__ __forceinline__ void mark_tile(const Segs& g, int64_t row0, int groups, uint32_t* mask, int32_t* first, int32_t* last,
+                                          int32_t& border) {
     const int t = threadIdx.x, rows = groups * kRows;
     const int64_t lo_all = seg_lo<REV>(g, 0), hi_all = seg_lo<REV>(g, g.S), end = row0 + rows;
     const bool inside = lo_all <= row0 && (hi_all >= end || hi_all == g.N);
@@ -63,6 +64,7 @@ __device__ __forceinline__ void mark_tile(const Segs& g, int64_t row0, int group
         hi = nhi < hi ? nhi : hi;
     }
     __builtin_amdgcn_wave_barrier();
+    bool found = !inside;
     for (int64_t j = (lo > 0 ? lo - 1 : 0) + t; j < g.S; j += 64) {
         const int64_t a = seg_lo<REV>(g, j), b = seg_lo<REV>(g, j + 1);
         if (a >= end) break;
@@ -71,23 +73,26 @@ __device__ __forceinline__ void mark_tile(const Segs& g, int64_t row0, int group
         if (a >= row0) {
             first[a - row0] = s;
             atomicOr(&mask[(a - row0) / kRows], 1u << ((a - row0) % kRows));
+            found = true;
         }
         if (b - 1 >= row0 && b - 1 < end) {
             last[b - 1 - row0] = s;
             atomicOr(&mask[(b - 1 - row0) / kRows], 0x100u << ((b - 1 - row0) % kRows));
+            found = true;
         }
     }
+    found = __any(found);
+    if (t == 0) border = found;
 }
 
 // a = sigmoid(g), c = sigmoid(-g) without cancellation: e = exp(-|g|) <= 1, r = 1 / (1 + e); one of them is r, the other e r.
-// The product |g| log2(e) is carried in two parts and the reciprocal takes one Newton step: v_exp_f32 and v_rcp_f32 alone are
-// off by up to an ulp to one side, which a product over a long memory's a's would add up.
+// What the rounding of |g| log2(e) leaves out is put back (e * (1 + rest)) and the reciprocal takes one Newton step: v_exp_f32
+// and v_rcp_f32 alone are off by up to an ulp to one side, which a product over a long memory's a's would add up.
 __device__ __forceinline__ void gate_pair(float g, float& a, float& c) {
     const float m = __builtin_elementwise_minimum(fabsf(g), 110.f);      // e^-110 is 0 in fp32; a NaN stays one
     const float p = m * -1.4426950408889634f;
-    const float lo = fmaf(m, -1.9259629911266175e-8f, fmaf(m, -1.4426950408889634f, -p));
     float e = __builtin_amdgcn_exp2f(p);
-    e = fmaf(e, lo * 0.6931471805599453f, e);
+    e = fmaf(e, fmaf(p, -0.6931471805599453f, -m), e);
     const float s = 1.f + e, r0 = __builtin_amdgcn_rcpf(s), r = fmaf(r0, fmaf(-s, r0, 1.f), r0), er = e * r;
     a = g < 0.f ? er : r;
     c = g < 0.f ? r : er;
@@ -153,6 +158,15 @@ __device__ __forceinline__ void st_state(float* __restrict__ p, int64_t row, int
 }
 
 // ------------------------------------------------------------------------------------------------ maps
+// The union of the wave's row groups' masks, the same in every lane: loops and branches over borders are the wave's, what a
+// lane does there is selection (a divergent branch would keep two copies of the rows).
+__device__ __forceinline__ uint32_t wave_mask(uint32_t m, int CG) {
+    uint32_t w = 0;
+    for (int l = 0; l < 64; l += CG) w |= (uint32_t)__builtin_amdgcn_readlane((int)m, l);
+    return w;
+}
+__device__ __forceinline__ bool bit(uint32_t m, int i) { return (m >> i) & 1; }
+
 struct Map { float A[4], B[4]; };
 // The values stay, what was computed from them does not: keeps the compiler from holding products of a walk over the rows in
 // registers until a later walk can use them again (a multiplication is cheaper than 32 registers).
@@ -162,25 +176,22 @@ __device__ __forceinline__ void forget(float (&v)[kRows][4]) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) asm("" : "+v"(v[i][e]));
 }
+template <bool CUTS>
 __device__ __forceinline__ void after(Map& m, const float (&A1)[4], const float (&B1)[4]) {          // m <- m o (A1, B1)
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-        m.B[e] = m.A[e] < 0.f ? m.B[e] : fmaf(m.A[e], B1[e], m.B[e]);
-        m.A[e] = m.A[e] < 0.f || A1[e] < 0.f ? -1.f : m.A[e] * A1[e];
+        m.B[e] = CUTS && m.A[e] < 0.f ? m.B[e] : fmaf(m.A[e], B1[e], m.B[e]);
+        m.A[e] = CUTS && (m.A[e] < 0.f || A1[e] < 0.f) ? -1.f : m.A[e] * A1[e];
     }
-}
-__device__ __forceinline__ void then(Map& m, float4 A, float4 B) {                   // m <- (A, B) o m
-    Map y{{A.x, A.y, A.z, A.w}, {B.x, B.y, B.z, B.w}};
-    after(y, m.A, m.B);
-    m = y;
 }
 __device__ __forceinline__ float apply(float A, float B, float s) { return A < 0.f ? B : fmaf(A, s, B); }
 
 // Maps of the workgroup's row groups: `m` becomes the map of everything before this thread's group (UP: the rows are walked
 // from the last group to the first).  In a wave by shuffles (64 / CG groups), then over the waves through LDS.  Returns the
-// map of the whole tile in the threads of the LAST group of the walk.
+// map of the whole tile in the threads of the LAST group of the walk.  CUTS: the tile has a border (a composition is then
+// seven instructions a column instead of two).
 struct WaveMaps { float4 A[kWaves][kMaxCols / 4], B[kWaves][kMaxCols / 4]; };
-template <bool UP>
+template <bool UP, bool CUTS>
 __device__ __forceinline__ Map before_group(Map& m, int CG, int cg, WaveMaps& w) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int at = UP ? 63 - lane : lane, edge = at / CG;                // this group's place in the wave's walk
@@ -190,18 +201,19 @@ __device__ __forceinline__ Map before_group(Map& m, int CG, int cg, WaveMaps& w)
         for (int e = 0; e < 4; ++e) {
             A1[e] = UP ? __shfl_down(m.A[e], o * CG, 64) : __shfl_up(m.A[e], o * CG, 64);
             B1[e] = UP ? __shfl_down(m.B[e], o * CG, 64) : __shfl_up(m.B[e], o * CG, 64);
+            if (edge < o) { A1[e] = 1.f; B1[e] = 0.f; }
         }
-        if (edge >= o) after(m, A1, B1);
+        after<CUTS>(m, A1, B1);
     }
     if (at >= 64 - CG) {
         w.A[wave][cg] = make_float4(m.A[0], m.A[1], m.A[2], m.A[3]);
         w.B[wave][cg] = make_float4(m.B[0], m.B[1], m.B[2], m.B[3]);
     }
-    const Map own = m;
+    Map all = m;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-        m.A[e] = UP ? __shfl_down(own.A[e], CG, 64) : __shfl_up(own.A[e], CG, 64);
-        m.B[e] = UP ? __shfl_down(own.B[e], CG, 64) : __shfl_up(own.B[e], CG, 64);
+        m.A[e] = UP ? __shfl_down(all.A[e], CG, 64) : __shfl_up(all.A[e], CG, 64);
+        m.B[e] = UP ? __shfl_down(all.B[e], CG, 64) : __shfl_up(all.B[e], CG, 64);
         if (edge == 0) { m.A[e] = 1.f; m.B[e] = 0.f; }
     }
     __syncthreads();
@@ -209,11 +221,15 @@ __device__ __forceinline__ Map before_group(Map& m, int CG, int cg, WaveMaps& w)
 #pragma unroll
     for (int k = 0; k < kWaves - 1; ++k) {
         const int x = UP ? kWaves - 1 - k : k;
-        if (UP ? x > wave : x < wave) then(pre, w.A[x][cg], w.B[x][cg]);
+        if (UP ? x > wave : x < wave) {
+            const float4 A = w.A[x][cg], B = w.B[x][cg];
+            Map y{{A.x, A.y, A.z, A.w}, {B.x, B.y, B.z, B.w}};
+            after<CUTS>(y, pre.A, pre.B);
+            pre = y;
+        }
     }
-    after(m, pre.A, pre.B);
-    Map all = own;
-    after(all, pre.A, pre.B);
+    after<CUTS>(m, pre.A, pre.B);
+    if (UP ? wave == 0 : wave == kWaves - 1) after<CUTS>(all, pre.A, pre.B);
     return all;
 }
 
@@ -224,7 +240,10 @@ __device__ __forceinline__ Map before_group(Map& m, int CG, int cg, WaveMaps& w)
 // per 64 tiles.  The products are always formed in this order, so the bits do not depend on who was first (a look-back
 // that takes the nearest state it finds would).  A word is its own flag: (A, B) travel as one 64-bit relaxed atomic,
 // B's bits never being kEmpty; no fences, no other memory is ordered by them.
-struct Chain { uint64_t *tile, *group; uint32_t *state, *ticket; };
+struct Chain {                       // for every column block: tile[group][8][64], group[block][8][64], state[block][64]
+    uint64_t *tile, *group;
+    uint32_t *state, *ticket, ncb;
+};
 __device__ __forceinline__ void publish(uint64_t* p, float A, float B) {
     uint32_t b = __float_as_uint(B);
     if (b == kEmpty) b = 0x7FC00000u;                                    // a NaN stays a NaN
@@ -242,54 +261,69 @@ __device__ __forceinline__ void then_words(float& A, float& B, const uint64_t (&
             A = A2 < 0.f || A < 0.f ? -1.f : A2 * A;
         }
 }
-__device__ __forceinline__ void await_words(const uint64_t* p, int64_t D, int n, uint64_t (&v)[kGroup - 1]) {
+// The words of a group lie side by side, so seven of them are one address and seven constants; those of tiles that are not
+// asked for are loaded and left alone.
+__device__ __forceinline__ void peek_words(const uint64_t* p, uint64_t (&v)[kGroup - 1]) {
+#pragma unroll
+    for (int i = 0; i < kGroup - 1; ++i) v[i] = peek(p + i * kMaxCols);
+}
+__device__ __forceinline__ void await_words(const uint64_t* p, int n, uint64_t (&v)[kGroup - 1]) {
+#pragma unroll 1
     for (int k = 0; k < kSpinLimit; ++k) {
         bool wait = false;
 #pragma unroll
-        for (int i = 0; i < kGroup - 1; ++i) v[i] = i < n ? peek(p + i * D) : 0;
-#pragma unroll
-        for (int i = 0; i < kGroup - 1; ++i) wait |= is_empty(v[i]);
-        if (!wait) break;
-        __builtin_amdgcn_s_sleep(1);
+        for (int i = 0; i < kGroup - 1; ++i) wait |= i < n && is_empty(v[i]);
+        if (!__any(wait)) break;
+        peek_words(p, v);
     }
 }
 
 // sIn[column] = the state that enters tile number `k` of the walk; own[0 / 1][column]: A / B of the tile's map.  The first
-// CG * 4 threads, one column each.  All that can be composed is composed before the state is waited for: a link of the chain
-// is one load, one fma and one store.
-__device__ __forceinline__ void enter_tile(const Chain& ch, int64_t k, int64_t D, int64_t c, const float* ownA, const float* ownB, float* sIn,
-                                           int col) {
+// CG * 4 threads, one column each.  Everything is asked for at once (a look at another workgroup's word takes about a
+// microsecond), and all that can be composed is composed before the state is waited for: a link of the chain is one load,
+// one fma and one store.
+__device__ __forceinline__ void enter_tile(const Chain& ch, uint32_t k, uint32_t cb, const float* ownA, const float* ownB, float* sIn,
+                                           uint32_t col) {
     const int p = (int)(k % kGroup), gp = (int)(k / kGroup % kGroup);
-    const int64_t block = k / (kGroup * kGroup);
+    const uint32_t group = k / kGroup, block = group / kGroup;
+    uint64_t *tiles = ch.tile + ((int64_t)group * ch.ncb + cb) * (kGroup * kMaxCols) + col;
+    uint64_t *groups = ch.group + ((int64_t)block * ch.ncb + cb) * (kGroup * kMaxCols) + col;
+    uint32_t* state = ch.state + ((int64_t)block * ch.ncb + cb) * kMaxCols + col;
+    const uint32_t* before = state - (block > 0 ? (int64_t)ch.ncb * kMaxCols : 0);
     const float oA = ownA[col], oB = ownB[col];
-    if (p < kGroup - 1) publish(ch.tile + k * D + c, oA, oB);
+    if (p < kGroup - 1) publish(tiles + p * kMaxCols, oA, oB);
+    uint64_t v[kGroup - 1], u[kGroup - 1];
+    uint32_t w = __hip_atomic_load(before, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    peek_words(groups, u);
+    peek_words(tiles, v);
     float A = 1.f, B = 0.f;                                              // of the group's tiles before this one
-    uint64_t v[kGroup - 1];
-    await_words(ch.tile + (k - p) * D + c, D, p, v);
+    await_words(tiles, p, v);
     then_words(A, B, v, p);
     if (p == kGroup - 1 && gp < kGroup - 1)
-        publish(ch.group + k / kGroup * D + c, A < 0.f || oA < 0.f ? -1.f : oA * A, apply(oA, oB, B));
+        publish(groups + gp * kMaxCols, A < 0.f || oA < 0.f ? -1.f : oA * A, apply(oA, oB, B));
     float gA = 1.f, gB = 0.f;                                            // of the block's groups before this one
-    await_words(ch.group + (k / kGroup - gp) * D + c, D, gp, v);
-    then_words(gA, gB, v, gp);
+    await_words(groups, gp, u);
+    then_words(gA, gB, u, gp);
     B = apply(A, B, gB);
     A = A < 0.f || gA < 0.f ? -1.f : A * gA;
-    float s = 0.f;
-    if (block > 0 && !(A < 0.f)) {                                       // behind a cut the state from further back is not needed
-        uint32_t w = 0;
-        for (int i = 0; i < kSpinLimit; ++i) {
-            w = __hip_atomic_load(ch.state + (block - 1) * D + c, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            if (w != kEmpty) break;
-        }
-        s = __uint_as_float(w);
-    }
-    s = apply(A, B, s);
+    if (block > 0 && !__all(A < 0.f))                                        // behind a cut the state from further back is not needed
+#pragma unroll 1
+        for (int i = 0; i < kSpinLimit && __any(w == kEmpty); ++i) w = __hip_atomic_load(before, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    const float s = apply(A, B, block > 0 ? __uint_as_float(w) : 0.f);
     if (p == kGroup - 1 && gp == kGroup - 1) {
         uint32_t b = __float_as_uint(apply(oA, oB, s));
         if (b == kEmpty) b = 0x7FC00000u;
-        __hip_atomic_store(ch.state + block * D + c, b, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __hip_atomic_store(state, b, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
     sIn[col] = s;
+}
+
+// v <- the state before a segment's first row, where this lane has one
+__device__ __forceinline__ void enter_row(bool here, const float* __restrict__ p, int64_t row, int64_t D, int64_t c, int nv, float (&v)[4]) {
+    float s0[4];
+    ld_state(p, row, D, c, nv, s0);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = here ? s0[e] : v[e];
 }
 
 // The next (tile, column block) in the order of the walk; with a single tile there is nothing to order.  false: none left
@@ -330,6 +364,7 @@ __global__ __launch_bounds__(kThreads) void k_scan_fwd(const T* __restrict__ x, 
                                                           float* __restrict__ heads) {
     __shared__ int32_t first[2 * kThreads], last[2 * kThreads];            // kThreads / CG * kRows rows, CG >= 4
     __shared__ uint32_t mask[kThreads / 4];
+    __shared__ int32_t border;
     __shared__ WaveMaps wm;
     __shared__ float4 own[2][kMaxCols / 4], sIn[kMaxCols / 4];
     int64_t tile;
@@ -339,7 +374,7 @@ __global__ __launch_bounds__(kThreads) void k_scan_fwd(const T* __restrict__ x, 
     const int64_t row0 = tile * rows, c0 = (int64_t)cb * (CG * 4), c = c0 + cg * 4, low = REV ? g.N - row0 - rows : row0;
     const int64_t left = g.N - row0 - r0;
     const Lane l{c + 4 <= D ? 4 : c < D ? (int)(D - c) : 0, left >= kRows ? kRows : left > 0 ? (int)left : 0};
-    if (threadIdx.x < 64) mark_tile<REV>(g, row0, RG, mask, first, last);
+    if (threadIdx.x < 64) mark_tile<REV>(g, row0, RG, mask, first, last, border);
     float a[kRows][4], b[kRows][4];
     // where there is no row: a = 1, b = 0, the map that changes nothing
     load_rows(gate + low * ldg + c0, row_off<T, REV>(r0, rows, ldg, cg * 4), row_step<T, REV>(ldg), l, __builtin_inff(), a);
@@ -354,39 +389,42 @@ __global__ __launch_bounds__(kThreads) void k_scan_fwd(const T* __restrict__ x, 
         }
     __syncthreads();
     const uint32_t m = mask[rg], cuts = (m | m >> 16) & 0xFF;
-    const bool any = __builtin_expect(__any(m != 0), 0);                 // most waves see no segment begin or end
+    const bool tile_any = __builtin_amdgcn_readfirstlane(border) != 0;
+    const bool any = __builtin_expect(tile_any && __any(m != 0), 0);     // most waves see no segment begin or end
     Map f{{1.f, 1.f, 1.f, 1.f}, {0.f, 0.f, 0.f, 0.f}};
     if (!any) {
 #pragma unroll
         for (int i = 0; i < kRows; ++i)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                f.B[e] = fmaf(a[i][e], f.B[e], b[i][e]);
-                f.A[e] *= a[i][e];
-            }
+            for (int e = 0; e < 4; ++e) f.B[e] = fmaf(a[i][e], f.B[e], b[i][e]);
     } else {
+        for (uint32_t todo = wave_mask(cuts, CG); todo; todo &= todo - 1) {          // one row after the other
+            const int at = __builtin_ctz(todo);
+            const bool here = bit(cuts, at), seg = bit(m, at);           // here, but not seg: a row in no segment
+            float s0[4];
+            ld_state(seg ? h0 : nullptr, seg ? first[r0 + at] : 0, D, c, l.nv, s0);
 #pragma unroll
-        for (int i = 0; i < kRows; ++i) {
-            if ((cuts >> i) & 1) {
-                float s0[4] = {0.f, 0.f, 0.f, 0.f};
-                if ((m >> i) & 1) ld_state(h0, first[r0 + i], D, c, l.nv, s0);
+            for (int i = 0; i < kRows; ++i)
+                if (i == at)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    b[i][e] = (m >> i) & 1 ? fmaf(a[i][e], s0[e], b[i][e]) : 0.f;
-                    a[i][e] = -1.f;
-                }
-            }
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                f.B[e] = apply(a[i][e], b[i][e], f.B[e]);
-                f.A[e] *= a[i][e];
-            }
+                    for (int e = 0; e < 4; ++e) {
+                        b[i][e] = !here ? b[i][e] : seg ? fmaf(a[i][e], s0[e], b[i][e]) : 0.f;
+                        a[i][e] = here ? -1.f : a[i][e];
+                    }
         }
-        if (cuts)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) f.A[e] = -1.f;
+        for (int i = 0; i < kRows; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) f.B[e] = apply(a[i][e], b[i][e], f.B[e]);
     }
-    const Map all = before_group<false>(f, CG, cg, wm);
+#pragma unroll
+    for (int i = 0; i < kRows; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) f.A[e] *= a[i][e];
+    if (cuts)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) f.A[e] = -1.f;
+    const Map all = tile_any ? before_group<false, true>(f, CG, cg, wm) : before_group<false, false>(f, CG, cg, wm);
     float s[4] = {0.f, 0.f, 0.f, 0.f};
     if (n_tiles > 1) {
         if (rg == RG - 1) {
@@ -395,7 +433,7 @@ __global__ __launch_bounds__(kThreads) void k_scan_fwd(const T* __restrict__ x, 
         }
         __syncthreads();
         if ((int)threadIdx.x < CG * 4 && c0 + threadIdx.x < D)
-            enter_tile(ch, tile, D, c0 + threadIdx.x, &own[0][0].x, &own[1][0].x, &sIn[0].x, threadIdx.x);
+            enter_tile(ch, (uint32_t)tile, (uint32_t)cb, &own[0][0].x, &own[1][0].x, &sIn[0].x, threadIdx.x);
         __syncthreads();
         const float4 v = sIn[cg];
         s[0] = v.x; s[1] = v.y; s[2] = v.z; s[3] = v.w;
@@ -410,11 +448,18 @@ __global__ __launch_bounds__(kThreads) void k_scan_fwd(const T* __restrict__ x, 
             for (int e = 0; e < 4; ++e) b[i][e] = s[e] = fmaf(a[i][e], s[e], b[i][e]);
     } else {
 #pragma unroll
-        for (int i = 0; i < kRows; ++i) {
+        for (int i = 0; i < kRows; ++i)
 #pragma unroll
             for (int e = 0; e < 4; ++e) b[i][e] = s[e] = apply(a[i][e], b[i][e], s[e]);
-            if (((m >> 8) >> i) & 1 && h_last) st_state(h_last, last[r0 + i], D, c, l.nv, s);
-        }
+        if (h_last)
+            for (uint32_t todo = wave_mask(m >> 8, CG) & 0xFF; todo; todo &= todo - 1) {
+                const int at = __builtin_ctz(todo);
+#pragma unroll
+                for (int i = 0; i < kRows; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[e] = i == at ? b[i][e] : s[e];
+                if (bit(m, 8 + at)) st_state(h_last, last[r0 + at], D, c, l.nv, s);
+            }
     }
     store_rows(h + low * ldh + c0, row_off<T, REV>(r0, rows, ldh, cg * 4), row_step<T, REV>(ldh), l, b);
     if (h_last && rg == 0)                                               // segments without rows: the state passes through
@@ -438,6 +483,7 @@ __global__ __launch_bounds__(kThreads) void k_scan_bwd(const T* __restrict__ x, 
                                                              int64_t lddx, T* __restrict__ dgate, int64_t lddg, float* __restrict__ dh0) {
     __shared__ int32_t first[2 * kThreads], last[2 * kThreads];
     __shared__ uint32_t mask[kThreads / 4];
+    __shared__ int32_t border;
     __shared__ WaveMaps wm;
     __shared__ float4 own[2][kMaxCols / 4], sIn[kMaxCols / 4];
     int64_t k;
@@ -448,7 +494,7 @@ __global__ __launch_bounds__(kThreads) void k_scan_bwd(const T* __restrict__ x, 
     const int64_t row0 = tile * rows, c0 = (int64_t)cb * (CG * 4), c = c0 + cg * 4, low = REV ? g.N - row0 - rows : row0;
     const int64_t left = g.N - row0 - r0;
     const Lane l{c + 4 <= D ? 4 : c < D ? (int)(D - c) : 0, left >= kRows ? kRows : left > 0 ? (int)left : 0};
-    if (threadIdx.x < 64) mark_tile<REV>(g, row0, RG, mask, first, last);
+    if (threadIdx.x < 64) mark_tile<REV>(g, row0, RG, mask, first, last, border);
     float a[kRows][4], cc[kRows][4], q[kRows][4], d[kRows][4], s[4];
     load_rows(gate + low * ldg + c0, row_off<T, REV>(r0, rows, ldg, cg * 4), row_step<T, REV>(ldg), l, __builtin_inff(), a);
     load_rows(x + low * ldx + c0, row_off<T, REV>(r0, rows, ldx, cg * 4), row_step<T, REV>(ldx), l, 0.f, q);
@@ -465,11 +511,13 @@ __global__ __launch_bounds__(kThreads) void k_scan_bwd(const T* __restrict__ x, 
         for (int e = 0; e < 4; ++e) gate_pair(a[i][e], a[i][e], cc[i][e]);
     __syncthreads();
     const uint32_t m = mask[rg], none = m >> 16, fcut = (m | none) & 0xFF, lcut = (m >> 8 | none) & 0xFF;
-    const bool any = __builtin_expect(__any(m != 0), 0);
+    uint32_t wf = 0, wl = 0;                                             // rows with a border in any of the wave's groups
+    const bool tile_any = __builtin_amdgcn_readfirstlane(border) != 0;
+    if (__builtin_expect(tile_any, 0)) { wf = wave_mask(fcut, CG); wl = wave_mask(lcut, CG); }
     Map f{{1.f, 1.f, 1.f, 1.f}, {0.f, 0.f, 0.f, 0.f}}, u;                // of h down to the group's end, of mu up to its head
 #pragma unroll
     for (int i = 0; i < kRows; ++i) {
-        if (any && (fcut >> i) & 1) ld_state((m >> i) & 1 ? h0 : nullptr, (m >> i) & 1 ? first[r0 + i] : 0, D, c, l.nv, f.B);
+        if (bit(wf, i)) enter_row(bit(fcut, i), bit(m, i) ? h0 : nullptr, bit(m, i) ? first[r0 + i] : 0, D, c, l.nv, f.B);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             f.B[e] = fmaf(a[i][e], f.B[e], cc[i][e] * q[i][e]);
@@ -482,13 +530,14 @@ __global__ __launch_bounds__(kThreads) void k_scan_bwd(const T* __restrict__ x, 
     for (int e = 0; e < 4; ++e) u.B[e] = 0.f;
 #pragma unroll
     for (int i = kRows - 1; i >= 0; --i) {
-        if (any && (lcut >> i) & 1) {
-            float ds[4] = {0.f, 0.f, 0.f, 0.f};
-            if (((m >> 8) >> i) & 1) ld_state(dlast, last[r0 + i], D, c, l.nv, ds);
+        if (bit(wl, i)) {
+            const bool seg = bit(m, 8 + i);
+            float ds[4];
+            ld_state(seg ? dlast : nullptr, seg ? last[r0 + i] : 0, D, c, l.nv, ds);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                d[i][e] = (none >> i) & 1 ? 0.f : d[i][e] + ds[e];
-                u.B[e] = 0.f;
+                d[i][e] = bit(none, i) ? 0.f : d[i][e] + ds[e];
+                u.B[e] = bit(lcut, i) ? 0.f : u.B[e];
             }
         }
 #pragma unroll
@@ -499,24 +548,21 @@ __global__ __launch_bounds__(kThreads) void k_scan_bwd(const T* __restrict__ x, 
         if (fcut) f.A[e] = -1.f;
         if (lcut) u.A[e] = -1.f;
     }
-    before_group<false>(f, CG, cg, wm);
+    if (tile_any) before_group<false, true>(f, CG, cg, wm);
+    else before_group<false, false>(f, CG, cg, wm);
 #pragma unroll
     for (int e = 0; e < 4; ++e) s[e] = apply(f.A[e], f.B[e], s[e]);
     __syncthreads();                                                     // wm is written again
-    const Map all = before_group<true>(u, CG, cg, wm);
+    const Map all = tile_any ? before_group<true, true>(u, CG, cg, wm) : before_group<true, false>(u, CG, cg, wm);
     forget(cc);
 #pragma unroll
     for (int i = 0; i < kRows; ++i) {
-        if (any && (fcut >> i) & 1) ld_state((m >> i) & 1 ? h0 : nullptr, (m >> i) & 1 ? first[r0 + i] : 0, D, c, l.nv, s);
+        if (bit(wf, i)) enter_row(bit(fcut, i), bit(m, i) ? h0 : nullptr, bit(m, i) ? first[r0 + i] : 0, D, c, l.nv, s);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const float xi = q[i][e], hb = s[e];
             s[e] = fmaf(a[i][e], hb, cc[i][e] * xi);
             q[i][e] = (hb - xi) * (a[i][e] * cc[i][e]);
-        }
-        if (any && (none >> i) & 1) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) q[i][e] = cc[i][e] = 0.f;
         }
     }
 #pragma unroll
@@ -528,7 +574,7 @@ __global__ __launch_bounds__(kThreads) void k_scan_bwd(const T* __restrict__ x, 
         }
         __syncthreads();
         if ((int)threadIdx.x < CG * 4 && c0 + threadIdx.x < D)
-            enter_tile(ch, k, D, c0 + threadIdx.x, &own[0][0].x, &own[1][0].x, &sIn[0].x, threadIdx.x);
+            enter_tile(ch, (uint32_t)k, (uint32_t)cb, &own[0][0].x, &own[1][0].x, &sIn[0].x, threadIdx.x);
         __syncthreads();
         const float4 v = sIn[cg];
         s[0] = v.x; s[1] = v.y; s[2] = v.z; s[3] = v.w;
@@ -537,9 +583,9 @@ __global__ __launch_bounds__(kThreads) void k_scan_bwd(const T* __restrict__ x, 
     for (int e = 0; e < 4; ++e) s[e] = apply(u.A[e], u.B[e], s[e]);
 #pragma unroll
     for (int i = kRows - 1; i >= 0; --i) {
-        if (any && (lcut >> i) & 1) {
+        if (bit(wl, i)) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s[e] = 0.f;
+            for (int e = 0; e < 4; ++e) s[e] = bit(lcut, i) ? 0.f : s[e];
         }
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -548,11 +594,14 @@ __global__ __launch_bounds__(kThreads) void k_scan_bwd(const T* __restrict__ x, 
             q[i][e] *= lam;
             s[e] = a[i][e] * lam;
         }
-        if (any && (none >> i) & 1) {                                    // (a NaN of a row in no segment: 0 all the same)
+        if (bit(wf, i)) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) q[i][e] = cc[i][e] = 0.f;
+            for (int e = 0; e < 4; ++e) {                                // rows in no segment: 0, whatever they hold
+                cc[i][e] = bit(none, i) ? 0.f : cc[i][e];
+                q[i][e] = bit(none, i) ? 0.f : q[i][e];
+            }
+            if (bit(m, i) && dh0) st_state(dh0, first[r0 + i], D, c, l.nv, s);
         }
-        if (any && (m >> i) & 1 && dh0) st_state(dh0, first[r0 + i], D, c, l.nv, s);
     }
     store_rows(dx + low * lddx + c0, row_off<T, REV>(r0, rows, lddx, cg * 4), row_step<T, REV>(lddx), l, cc);
     store_rows(dgate + low * lddg + c0, row_off<T, REV>(r0, rows, lddg, cg * 4), row_step<T, REV>(lddg), l, q);
@@ -617,9 +666,10 @@ ScanWs scan_ws(int64_t n, int64_t D) {
     ScanWs w;
     int64_t at = 0;
     auto take = [&](int64_t bytes) { const int64_t o = at; at += (bytes + 255) / 256 * 256; return o; };
-    w.tile = take(8 * t * D);
-    w.group = take(8 * (t / kGroup + 1) * D);
-    w.state = take(4 * (t / (kGroup * kGroup) + 1) * D);
+    const int64_t blocks = t / (kGroup * kGroup) + 1, lane = column_blocks(D) * kMaxCols;
+    w.tile = take(8 * (t / kGroup + 1) * kGroup * lane);
+    w.group = take(8 * blocks * kGroup * lane);
+    w.state = take(4 * blocks * lane);
     w.ticket = take(4);
     w.bytes = at;
     return w;
@@ -629,7 +679,7 @@ Chain make_chain(void* ws, int64_t n, int64_t D, int64_t tiles, hipStream_t s) {
     const ScanWs w = scan_ws(n, D);
     char* base = static_cast<char*>(ws);
     const Chain ch{reinterpret_cast<uint64_t*>(base + w.tile), reinterpret_cast<uint64_t*>(base + w.group),
-                   reinterpret_cast<uint32_t*>(base + w.state), reinterpret_cast<uint32_t*>(base + w.ticket)};
+                   reinterpret_cast<uint32_t*>(base + w.state), reinterpret_cast<uint32_t*>(base + w.ticket), column_blocks(D)};
     if (tiles > 1) k_scan_clear<<<bg_grid_for(w.ticket / 16, 256 * 4, 2048), 256, 0, s>>>(static_cast<uint4*>(ws), w.ticket / 16, ch.ticket);
     return ch;
 }
