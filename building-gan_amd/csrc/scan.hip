@@ -28,22 +28,22 @@ constexpr int kSpinLimit = 1 << 22;              // a wait of several seconds: o
 struct Segs { const int32_t* ptr; int64_t S, N, T; };      // ptr NULL: S segments of T rows
 
 // REV walks the rows upwards: LOGICAL row r is row N - 1 - r, logical segment j is segment S - 1 - j
-template <bool REV>
+template <bool REV, bool UNIFORM = false>
 __device__ __forceinline__ int64_t seg_lo(const Segs& g, int64_t j) {                // logical first row of logical segment j
+    typedef const int32_t __attribute__((address_space(4))) * Scalar;                // (j the same in every lane: a scalar load)
     const int64_t k = REV ? g.S - j : j;
-    int64_t p = g.ptr ? (int64_t)g.ptr[k] : k * g.T;
+    int64_t p = !g.ptr ? k * g.T : UNIFORM ? (int64_t)((Scalar)(uintptr_t)g.ptr)[k] : (int64_t)g.ptr[k];
     p = p < 0 ? 0 : p > g.N ? g.N : p;
     return REV ? g.N - p : p;
 }
 
 // mask[group]: bit i = row i of the group is a segment's first row, bit 8 + i = its last, bit 16 + i = in no segment;
-// first[row] / last[row] = that segment where the bit is set; border: any bit at all.  One wave does it: the segment of the tile's first row is
-// found by a search 64 lanes wide.
+// first[row] / last[row] = that segment where the bit is set; border: any bit at all.  One wave does it.
 template <bool REV>
 __device__ __forceinline__ void mark_tile(const Segs& g, int64_t row0, int groups, uint32_t* mask, int32_t* first, int32_t* last,
                                           int32_t& border) {
     const int t = threadIdx.x, rows = groups * kRows;
-    const int64_t lo_all = seg_lo<REV>(g, 0), hi_all = seg_lo<REV>(g, g.S), end = row0 + rows;
+    const int64_t lo_all = seg_lo<REV, true>(g, 0), hi_all = seg_lo<REV, true>(g, g.S), end = row0 + rows;
     const bool inside = lo_all <= row0 && (hi_all >= end || hi_all == g.N);
     for (int k = t; k < groups; k += 64) {
         uint32_t m = 0;
@@ -54,18 +54,19 @@ __device__ __forceinline__ void mark_tile(const Segs& g, int64_t row0, int group
             }
         mask[k] = m;
     }
-    int64_t lo = 0, hi = g.S;                    // lo -> how many segments begin at or before row0
+    // how many segments begin at or before row0: scalar loads (the same in every lane), so the search neither waits for the
+    // rows of the tile nor makes them wait
+    int64_t lo = 0, hi = g.S;
     if (!g.ptr) lo = hi = g.T > 0 ? row0 / g.T + 1 : 0;
     while (lo < hi) {
-        const int64_t step = (hi - lo + 63) / 64, j = lo + t * step;
-        const int c = __popcll(__ballot(j < hi && seg_lo<REV>(g, j) <= row0));
-        const int64_t nlo = c ? lo + (c - 1) * step + 1 : lo, nhi = c ? lo + c * step : lo;
-        lo = nlo;
-        hi = nhi < hi ? nhi : hi;
+        const int64_t mid = (lo + hi) >> 1;
+        if (seg_lo<REV, true>(g, mid) <= row0) lo = mid + 1; else hi = mid;
     }
     __builtin_amdgcn_wave_barrier();
     bool found = !inside;
-    for (int64_t j = (lo > 0 ? lo - 1 : 0) + t; j < g.S; j += 64) {
+    // nothing to mark where the segment that holds row0 began before it and goes on behind the tile
+    const bool plain = lo > 0 && seg_lo<REV, true>(g, lo - 1) < row0 && seg_lo<REV, true>(g, lo) > end;
+    for (int64_t j = plain ? g.S : (lo > 0 ? lo - 1 : 0) + t; j < g.S; j += 64) {
         const int64_t a = seg_lo<REV>(g, j), b = seg_lo<REV>(g, j + 1);
         if (a >= end) break;
         if (a >= b) continue;
@@ -464,7 +465,7 @@ __global__ __launch_bounds__(kThreads) void k_scan_fwd(const T* __restrict__ x, 
     store_rows(h + low * ldh + c0, row_off<T, REV>(r0, rows, ldh, cg * 4), row_step<T, REV>(ldh), l, b);
     if (h_last && rg == 0)                                               // segments without rows: the state passes through
         for (int64_t k = tile; k < g.S; k += n_tiles)
-            if (seg_lo<REV>(g, k) >= seg_lo<REV>(g, k + 1)) {
+            if (seg_lo<REV, true>(g, k) >= seg_lo<REV, true>(g, k + 1)) {
                 const int64_t sg = REV ? g.S - 1 - k : k;
                 float v[4];
                 ld_state(h0, sg, D, c, l.nv, v);
@@ -607,7 +608,7 @@ __global__ __launch_bounds__(kThreads) void k_scan_bwd(const T* __restrict__ x, 
     store_rows(dgate + low * lddg + c0, row_off<T, REV>(r0, rows, lddg, cg * 4), row_step<T, REV>(lddg), l, q);
     if (dh0 && rg == 0)
         for (int64_t j = tile; j < g.S; j += n_tiles)
-            if (seg_lo<REV>(g, j) >= seg_lo<REV>(g, j + 1)) {
+            if (seg_lo<REV, true>(g, j) >= seg_lo<REV, true>(g, j + 1)) {
                 const int64_t sgm = REV ? g.S - 1 - j : j;
                 float v[4];
                 ld_state(dlast, sgm, D, c, l.nv, v);
