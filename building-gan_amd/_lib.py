@@ -47,7 +47,7 @@ SIGNATURES = {
     "bg_plan_chunks": [_p, _i64, _i32, _p, _p],
     "bg_embedding_fwd": [_int, _p, _i64, _i64, _p, _int, _i64, _i64, _f, _p, _i64, _p],
     "bg_embedding_bwd": [_int, _p, _i64, _p, _int, _i64, _i64, _i64, _f, _p, _p, _i64, _p],
-    "bg_embedding_bwd_workspace": [_i64] * 3,
+    "bg_embedding_bwd_workspace": [_int, _i64, _i64, _i64],
     "bg_gated_scan_heads": [_i64] * 2,
     "bg_gated_scan_workspace": [_i64] * 2,
     "bg_gated_scan_fwd": [_int, _p, _i64, _p, _i64, _p, _i64, _i64, _i64, _p, _int, _p, _i64, _p, _p, _p, _i64, _p],

@@ -968,7 +968,7 @@ def embedding_grad_raw(g: torch.Tensor, ids: torch.Tensor, n_rows: int, scale: f
     g2 = _rows(g.reshape(i.numel(), D))
     with _lib.on_device(g):
         dw = torch.empty(n_rows, D, dtype=g.dtype, device=g.device)
-        size = lib.bg_embedding_bwd_workspace(i.numel(), n_rows, D)
+        size = lib.bg_embedding_bwd_workspace(code, i.numel(), n_rows, D)
         ws = torch.empty(size, dtype=torch.uint8, device=g.device) if size else None
         check(lib.bg_embedding_bwd(code, ptr(g2), _ld(g2), ptr(i), i.dtype == torch.int64, i.numel(), D, n_rows, scale, ptr(dw),
                                    ptr(ws), size, stream()), "bg_embedding_bwd")

@@ -127,19 +127,19 @@ int bg_plan_build(const bgPlanIn* in, int32_t* arena_i32, float* arena_f32, bgSt
 
 /* out[i,:] = scale * weight[ids[i],:] for a table weight[V, D] of `dtype` (row pitches in elements); ids are int64
  * (ids_is_64 != 0) or int32.  An id outside [0, V) is a missing token: its row of `out` is zero.  One fp32 product and
- * one rounding per element.  Rows are moved in the widest pieces (16 bytes down to one element) that D, the pitches and
- * the addresses allow.  D <= 2^15, n * D <= 2^33 (BG_ERR_SHAPE).
+ * one rounding per element.  Rows are moved in pieces of 16 bytes whatever their alignment.  D <= 2^15, n * D <= 2^33 (BG_ERR_SHAPE).
  * replaces: one-hot x Linear over a categorical node feature and the position table's gather, Model/models.py:25,84. */
 int bg_embedding_fwd(int dtype, const void* weight, int64_t ldw, int64_t V, const void* ids, int ids_is_64, int64_t n, int64_t D,
                      float scale, void* out, int64_t ldo, bgStream stream);
 
 /* The lookup's gradient: dw[v,:] = scale * sum over ids[i] == v of g[i,:], every row of dw[V, D] (contiguous, 16-byte
- * aligned) written, zero where a token does not occur.  Tokens are sorted (stable) and every row's terms are summed in
- * fp32 in an order that depends on the sizes and ids only, with no floating-point atomics: equal inputs give equal bits.
+ * aligned) written, zero where a token does not occur.  Tokens are sorted (stable; tables of up to 16 rows are summed without a sort) and
+ * every row's terms are summed in fp32 in an order that depends on the sizes and ids only, with no floating-point atomics:
+ * equal inputs give equal bits.
  * n <= 2^30, V < 2^31 - 1, D <= 2^15 (BG_ERR_SHAPE).  ws: bg_embedding_bwd_workspace(...) bytes, 16-byte aligned
  * (BG_ERR_SCRATCH when ws_bytes is less); its contents need no preparation.
  * replaces: the weight gradient of the Linear over a one-hot feature, Model/models.py:84 under autograd.            */
-int64_t bg_embedding_bwd_workspace(int64_t n, int64_t V, int64_t D);
+int64_t bg_embedding_bwd_workspace(int dtype, int64_t n, int64_t V, int64_t D);
 int bg_embedding_bwd(int dtype, const void* g, int64_t ldg, const void* ids, int ids_is_64, int64_t n, int64_t D, int64_t V,
                      float scale, void* dw, void* ws, int64_t ws_bytes, bgStream stream);
 

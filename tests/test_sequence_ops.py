@@ -64,8 +64,8 @@ def test_entry_points_refuse_bad_arguments_before_any_launch():
     assert fwd(ids=None) == -1 and fwd(out=None) == -1 and fwd(V=-1) == -1
     assert fwd(D=1 << 16, ldw=1 << 16, ldo=1 << 16) == -2 and fwd(n=1 << 40) == -2
     assert fwd(n=0) == 0 and fwd(D=0, ldw=0, ldo=0) == 0
-    size = lib.bg_embedding_bwd_workspace(3, 4, 8)
-    assert size > 0 and lib.bg_embedding_bwd_workspace(0, 4, 8) == 0
+    size = lib.bg_embedding_bwd_workspace(0, 3, 4, 8)
+    assert size > 0 and lib.bg_embedding_bwd_workspace(0, 0, 4, 8) == 0
     bwd = lambda **k: lib.bg_embedding_bwd(*{**dict(dt=0, g=p, ldg=8, ids=p, i64=1, n=3, D=8, V=4, scale=1.0, dw=p, ws=p, size=size, s=None), **k}.values())
     assert bwd(dt=-1) == -1 and bwd(ldg=7) == -1 and bwd(dw=None) == -1 and bwd(ws=None) == -1 and bwd(g=None) == -1
     assert bwd(dw=p + 4) == -3 and bwd(ws=p + 8) == -3 and bwd(size=size - 1) == -5
