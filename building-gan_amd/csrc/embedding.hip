@@ -64,7 +64,7 @@ __device__ __forceinline__ void st_sums(float* __restrict__ p, int D, const floa
 // The output is a flat row of n * nv pieces; a thread moves U pieces 256 apart, so stores are contiguous whatever the width.
 // Piece -> row needs a division by nv: the block's first row comes from one 64-bit division (scalar), the rest from a
 // multiplication by `magic` = ceil(2^32 / nv), exact while (256 U + nv) * nv < 2^32.
-template <class T, int U, bool I64, bool NARROW>
+template <class T, int U, bool I64, bool NARROW, bool STREAM>      // STREAM: an output that no cache holds
 __global__ __launch_bounds__(256) void k_embedding_fwd(const T* __restrict__ w, int64_t ldw, int64_t V, const void* __restrict__ ids,
                                                        int64_t n, uint32_t nv, uint32_t magic, int D, float scale, T* __restrict__ out,
                                                        int64_t ldo) {
@@ -94,53 +94,64 @@ __global__ __launch_bounds__(256) void k_embedding_fwd(const T* __restrict__ w, 
         if (p0 + threadIdx.x + 256 * u >= total) continue;
 #pragma unroll
         for (int k = 0; k < Piece<T>::W; ++k) x[u].v[k] = (T)((float)x[u].v[k] * scale);
-        st_piece<T, NARROW>(out + row[u] * ldo + col[u], D, x[u]);
+        T* p = out + row[u] * ldo + col[u];
+        if (STREAM) {
+            typedef uint32_t Words __attribute__((ext_vector_type(4), aligned(2)));
+            Words v;
+            __builtin_memcpy(&v, &x[u], 16);
+            __builtin_nontemporal_store(v, reinterpret_cast<Words*>(p));
+        } else st_piece<T, NARROW>(p, D, x[u]);
     }
 }
 
 // ------------------------------------------------------------------------------------------------ gradient of a few rows
-// LG lanes walk over rows of g (LG pieces of a row each); their sums of every table row stand in LDS, a slot of W floats per
-// table row and lane that no other lane touches.  The block's groups are added up in order and leave one partial table, the
-// blocks' tables are added up by a second launch.
-template <class T, bool I64, bool NARROW>
+// LG lanes walk over rows of g, four elements each (8 or 16 bytes; the last lane's begin four before the row's end); their
+// sums of every table row stand in LDS, a float4 for every table row and lane that no other lane touches.  The block's
+// groups are added up in order and leave one partial table, the blocks' tables are added up by a second launch.
+template <class T>
+struct __attribute__((packed, aligned(sizeof(T)))) Four { T v[4]; };
+template <class T, bool I64, bool NARROW>      // NARROW: D < 4
 __global__ __launch_bounds__(256) void k_embedding_few(const void* __restrict__ ids, int64_t n, int V, const T* __restrict__ g, int64_t ldg,
                                                        int D, float* __restrict__ part, int LG, int64_t chunk) {
-    constexpr int W = Piece<T>::W, U = 4;
-    extern __shared__ float4 table[];                    // [V][W / 4][256]
-    const int t = threadIdx.x, lane = t & (LG - 1), group = t / LG, groups = 256 / LG;
-    const int q = blockIdx.y * LG + lane, pieces = (D + W - 1) / W, col = piece_column<T, NARROW>(q, D);
-    for (int v = 0; v < V * (W / 4); ++v) table[v * 256 + t] = make_float4(0.f, 0.f, 0.f, 0.f);
+    constexpr int U = sizeof(T) == 4 ? 4 : 8;            // 64 bytes in flight a lane
+    extern __shared__ float4 table[];                    // [V][256]
+    const int t = threadIdx.x, lane = t & (LG - 1), group = t / LG, groups = 256 / LG, q = blockIdx.y * LG + lane;
+    const int col = NARROW ? 0 : 4 * q < D - 4 ? 4 * q : D - 4;
+    const bool here = 4 * q < D;
+    for (int v = 0; v < V; ++v) table[v * 256 + t] = make_float4(0.f, 0.f, 0.f, 0.f);
     const int64_t r0 = blockIdx.x * chunk, r1 = r0 + chunk < n ? r0 + chunk : n;
-    if (q < pieces)
+    if (here)
         for (int64_t r = r0 + group; r < r1; r += groups * U) {
             int64_t id[U];
-            Piece<T> x[U];
+            Four<T> x[U];
 #pragma unroll
             for (int u = 0; u < U; ++u) id[u] = r + u * groups < r1 ? ld_id<I64>(ids, r + u * groups) : -1;
 #pragma unroll
-            for (int u = 0; u < U; ++u)
-                if (id[u] >= 0 && id[u] < V) ld_piece<T, NARROW>(x[u], g + (r + u * groups) * ldg + col, D);
+            for (int u = 0; u < U; ++u) {
+                if (id[u] < 0 || id[u] >= V) continue;
+                const T* p = g + (r + u * groups) * ldg + col;
+                if (!NARROW) x[u] = *reinterpret_cast<const Four<T>*>(p);
+                else
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) x[u].v[k] = k < D ? p[k] : (T)0.f;
+            }
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 if (id[u] < 0 || id[u] >= V) continue;
-#pragma unroll
-                for (int k = 0; k < W / 4; ++k) {
-                    float4& s = table[((int)id[u] * (W / 4) + k) * 256 + t];
-                    s = bg_add4(s, make_float4((float)x[u].v[4 * k], (float)x[u].v[4 * k + 1], (float)x[u].v[4 * k + 2], (float)x[u].v[4 * k + 3]));
-                }
+                float4& s = table[(int)id[u] * 256 + t];
+                s = bg_add4(s, make_float4((float)x[u].v[0], (float)x[u].v[1], (float)x[u].v[2], (float)x[u].v[3]));
             }
         }
     __syncthreads();
-    if (group == 0 && q < pieces)
+    if (group == 0 && here)
         for (int v = 0; v < V; ++v) {
-            float acc[W];
-#pragma unroll
-            for (int k = 0; k < W / 4; ++k) {
-                float4 s = table[(v * (W / 4) + k) * 256 + lane];
-                for (int y = 1; y < groups; ++y) s = bg_add4(s, table[(v * (W / 4) + k) * 256 + y * LG + lane]);
-                acc[4 * k] = s.x; acc[4 * k + 1] = s.y; acc[4 * k + 2] = s.z; acc[4 * k + 3] = s.w;
-            }
-            st_sums<T, NARROW>(part + ((int64_t)blockIdx.x * V + v) * D + col, D, acc);
+            float4 s = table[v * 256 + lane];
+            for (int y = 1; y < groups; ++y) s = bg_add4(s, table[v * 256 + y * LG + lane]);
+            float* p = part + ((int64_t)blockIdx.x * V + v) * D + col;
+            p[0] = s.x;
+            if (!NARROW || D > 1) p[1] = s.y;
+            if (!NARROW || D > 2) p[2] = s.z;
+            if (!NARROW) p[3] = s.w;
         }
 }
 
@@ -248,7 +259,7 @@ __device__ __forceinline__ int wave_rank(int d, bool valid, int bits, int lane, 
 }
 
 // All passes of up to kSmall keys by one workgroup, keys and positions in registers and LDS; the other workgroups zero dW.
-constexpr int kSmallThreads = 1024, kSmallRounds = 8, kSmall = kSmallThreads * kSmallRounds;
+constexpr int kSmallThreads = 1024, kSmallRounds = 4, kSmall = kSmallThreads * kSmallRounds;
 template <int SRC>
 __global__ __launch_bounds__(kSmallThreads) void k_sort_small(const void* __restrict__ src, int n, int64_t V, int passes, int bits,
                                                               int32_t* __restrict__ key_out, int32_t* __restrict__ pos_out, Fill fill) {
@@ -412,7 +423,7 @@ __global__ __launch_bounds__(256) void k_embedding_runs(const int32_t* __restric
             for (int u = 0; u < U; ++u) {
                 kk[u] = pass_round(my_key, j + u, LG);
                 const int32_t p = pass_round(my_pos, j + u, LG);
-                if (kk[u] < V && here) ld_piece<T, NARROW>(x[u], g + (int64_t)p * ldg + col, D);
+                ld_piece<T, NARROW>(x[u], g + (int64_t)p * ldg + col, D);       // (also where it is not wanted: no branch)
             }
 #pragma unroll
             for (int u = 0; u < U; ++u) {
@@ -441,7 +452,7 @@ __global__ __launch_bounds__(256) void k_embedding_runs(const int32_t* __restric
 
 // The run that begins in tile blockIdx.x and goes on: its own partial and the following tiles' are added by kJoin threads a
 // column (strided over the tiles), those kJoin sums then in order.
-constexpr int kJoin = 4, kJoinCols = 64;
+constexpr int kJoin = 2, kJoinCols = 64;
 template <class T>
 __global__ __launch_bounds__(kJoin* kJoinCols) void k_embedding_join(const int32_t* __restrict__ key, int64_t n, int32_t V,
                                                                      const float* __restrict__ part, int C, int64_t D, float scale,
@@ -465,18 +476,19 @@ __global__ __launch_bounds__(kJoin* kJoinCols) void k_embedding_join(const int32
     const int tx = threadIdx.x % kJoinCols, ty = threadIdx.x / kJoinCols;
     const int64_t c0 = (int64_t)blockIdx.y * (kJoinCols * E) + tx;
     float s[E];
+    int64_t col[E];                                                      // (columns behind the last: the last once more, not stored)
 #pragma unroll
     for (int e = 0; e < E; ++e) {
         const int64_t c = c0 + e * kJoinCols;
-        s[e] = ty == 0 && c < D ? part[(2 * tile + 1) * D + c] : 0.f;
+        col[e] = c < D ? c : D - 1;
+        s[e] = ty == 0 ? part[(2 * tile + 1) * D + col[e]] : 0.f;
     }
+    const float* rows = part + (tile + 1 + ty) * 2 * D;
+    int64_t left = last - tile - ty;                                     // tiles of this thread: left / kJoin, rounded up
 #pragma unroll 4
-    for (int64_t t = tile + 1 + ty; t <= last; t += kJoin)
+    for (; left > 0; left -= kJoin, rows += 2 * kJoin * D)
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-            const int64_t c = c0 + e * kJoinCols;
-            if (c < D) s[e] += part[2 * t * D + c];
-        }
+        for (int e = 0; e < E; ++e) s[e] += rows[col[e]];
 #pragma unroll
     for (int e = 0; e < E; ++e) sum[ty][e][tx] = s[e];
     __syncthreads();
@@ -498,7 +510,7 @@ int lanes_per_row(int64_t pieces) {
     return best;
 }
 
-constexpr int64_t kFewRows = 16;       // table rows up to which the sums stand in LDS
+constexpr int64_t kFewRows = 20;       // table rows up to which the sums stand in LDS: 80 KB, two workgroups a compute unit
 
 struct BwdPlan {                       // pieces of the workspace (bytes) and the shape of the launches: functions of n, V, D only
     bool few;
@@ -510,13 +522,15 @@ BwdPlan bwd_plan(int64_t n, int64_t V, int64_t D, int elem) {
     BwdPlan p = {};
     int64_t at = 0;
     auto take = [&](int64_t bytes) { const int64_t o = at; at += (bytes + 255) / 256 * 256; return o; };
-    const int W = 16 / elem;
-    const int64_t pieces = (D + W - 1) / W;
-    p.LG = lanes_per_row(pieces);
-    const int64_t column_blocks = (pieces + p.LG - 1) / p.LG;
     p.few = V <= kFewRows;
+    const int W = p.few ? 4 : 16 / elem;
+    const int64_t pieces = (D + W - 1) / W;
+    // in the runs a whole wave for a row from 33 pieces on, though many of its lanes may be idle behind the last one: a row's
+    // lines are asked for together (65 pieces: 71 us with 64 lanes, 82 us with 16)
+    p.LG = !p.few && pieces > 32 ? 64 : lanes_per_row(pieces);
+    const int64_t column_blocks = (pieces + p.LG - 1) / p.LG;
     if (p.few) {
-        const int64_t step = 256 / p.LG * 4;             // rows a block takes at once
+        const int64_t step = 256 / p.LG * (elem == 4 ? 4 : 8);       // rows a block takes at once
         int64_t most = 1024 / column_blocks;
         if (most < 1) most = 1;
         p.blocks = (n + 4 * step - 1) / (4 * step);
@@ -531,10 +545,10 @@ BwdPlan bwd_plan(int64_t n, int64_t V, int64_t D, int elem) {
     while (V >> b) ++b;                                  // keys go up to V
     p.passes = (b + kDigitBits - 1) / kDigitBits;
     p.bits = (b + p.passes - 1) / p.passes;
-    p.rounds = n <= 65536 ? 2 : 8;
+    p.rounds = n <= 65536 ? 2 : n <= 131072 ? 4 : 8;     // up to 64 tiles, whose counts every workgroup adds up by itself
     p.n_tiles = (int)((n + kSortThreads * p.rounds - 1) / (kSortThreads * p.rounds));
     p.C = 128;
-    while (p.C > 16 && n * column_blocks * p.LG / ((int64_t)p.C * 64) < 4096) p.C /= 2;
+    while (p.C > 16 && n * column_blocks * p.LG / ((int64_t)p.C * 64) < 2048) p.C /= 2;
     p.run_tiles = (n + p.C - 1) / p.C;
     p.key_a = take(4 * n); p.key_b = take(4 * n); p.pos_a = take(4 * n); p.pos_b = take(4 * n);
     p.hist = take((int64_t)4 * kBins * p.n_tiles);
@@ -550,9 +564,12 @@ int launch_fwd(const T* w, int64_t ldw, int64_t V, const void* ids, int64_t n, i
     const uint32_t magic = nv == 1 ? 0u : (uint32_t)(((1ull << 32) + nv - 1) / nv);
     if (n > kMaxPieces / nv) return BG_ERR_SHAPE;
     const int64_t total = n * nv;
-    const bool small = total <= 1 << 16, narrow = D < Piece<T>::W;
-    const auto kernel = small ? (narrow ? k_embedding_fwd<T, 1, I64, true> : k_embedding_fwd<T, 1, I64, false>)
-                              : (narrow ? k_embedding_fwd<T, 4, I64, true> : k_embedding_fwd<T, 4, I64, false>);
+    // an output past the last-level cache is stored around the caches (537 MB: 99 us against 125 us; 33 MB: no difference,
+    // and whoever reads it next may find it there)
+    const bool small = total <= 1 << 16, narrow = D < Piece<T>::W, stream = !narrow && total * 16 > ((int64_t)256 << 20);
+    const auto kernel = narrow ? (small ? k_embedding_fwd<T, 1, I64, true, false> : k_embedding_fwd<T, 4, I64, true, false>)
+                      : small ? k_embedding_fwd<T, 1, I64, false, false>
+                      : stream ? k_embedding_fwd<T, 4, I64, false, true> : k_embedding_fwd<T, 4, I64, false, false>;
     kernel<<<bg_grid_for(total, small ? 256 : 1024, 1 << 30), 256, 0, s>>>(w, ldw, V, ids, n, nv, magic, (int)D, scale, out, ldo);
     BG_LAUNCH_CHECK();
     return BG_OK;
@@ -564,24 +581,12 @@ void launch_sort_pass(const BwdPlan& p, const void* src, const int32_t* pos_in, 
     const int bins = 1 << p.bits;
     const int b0 = f0.n16 ? bg_grid_for(f0.n16, kSortThreads * 4, 1024) : 0, b1 = f1.n16 ? bg_grid_for(f1.n16, kSortThreads * 4, 1024) : 0;
     const bool scanned = p.n_tiles > 64;
-    if (p.rounds == 2) k_sort_hist<SRC, 2><<<p.n_tiles + b0, kSortThreads, 0, s>>>(src, n, V, shift, bins, hist, p.n_tiles, scanned, f0);
-    else k_sort_hist<SRC, 8><<<p.n_tiles + b0, kSortThreads, 0, s>>>(src, n, V, shift, bins, hist, p.n_tiles, scanned, f0);
+    const auto hist_kernel = p.rounds == 2 ? k_sort_hist<SRC, 2> : p.rounds == 4 ? k_sort_hist<SRC, 4> : k_sort_hist<SRC, 8>;
+    hist_kernel<<<p.n_tiles + b0, kSortThreads, 0, s>>>(src, n, V, shift, bins, hist, p.n_tiles, scanned, f0);
     if (scanned) k_sort_scan<<<(bins + 3) / 4, 256, 0, s>>>(hist, p.n_tiles, bins, total);
-    if (p.rounds == 2)
-        k_sort_place<SRC, 2, false><<<p.n_tiles + b1, kSortThreads, 0, s>>>(src, pos_in, n, V, shift, p.bits, hist, total, p.n_tiles,
-                                                                           key_out, pos_out, f1);
-    else if (scanned)
-        k_sort_place<SRC, 8, true><<<p.n_tiles + b1, kSortThreads, 0, s>>>(src, pos_in, n, V, shift, p.bits, hist, total, p.n_tiles,
-                                                                          key_out, pos_out, f1);
-    else
-        k_sort_place<SRC, 8, false><<<p.n_tiles + b1, kSortThreads, 0, s>>>(src, pos_in, n, V, shift, p.bits, hist, total, p.n_tiles,
-                                                                           key_out, pos_out, f1);
-}
-
-template <class K>
-int allow_lds(K kernel, size_t bytes) {                  // dynamic LDS past 64 KB has to be asked for
-    if (bytes > 64 * 1024) BG_HIP(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
-    return BG_OK;
+    const auto place_kernel = p.rounds == 2 ? k_sort_place<SRC, 2, false> : p.rounds == 4 ? k_sort_place<SRC, 4, false>
+                            : scanned ? k_sort_place<SRC, 8, true> : k_sort_place<SRC, 8, false>;
+    place_kernel<<<p.n_tiles + b1, kSortThreads, 0, s>>>(src, pos_in, n, V, shift, p.bits, hist, total, p.n_tiles, key_out, pos_out, f1);
 }
 
 template <int SRC>
@@ -595,11 +600,10 @@ int launch_sort_small(const BwdPlan& p, const void* src, int64_t n, int64_t V, i
 template <class T, bool I64>
 int launch_few(const BwdPlan& p, const void* ids, int64_t n, int64_t V, const T* g, int64_t ldg, int64_t D, float scale, T* dw, float* part,
                hipStream_t s) {
-    const int64_t pieces = (D + Piece<T>::W - 1) / Piece<T>::W;
-    const size_t lds = (size_t)V * Piece<T>::W * 1024;
-    const auto kernel = D < Piece<T>::W ? k_embedding_few<T, I64, true> : k_embedding_few<T, I64, false>;
-    if (allow_lds(kernel, lds) != BG_OK) return BG_ERR_LAUNCH;
-    kernel<<<dim3((unsigned)p.blocks, (unsigned)((pieces + p.LG - 1) / p.LG)), 256, lds, s>>>(
+    const size_t lds = (size_t)V * 4096;
+    const auto kernel = D < 4 ? k_embedding_few<T, I64, true> : k_embedding_few<T, I64, false>;
+    if (lds > 64 * 1024) BG_HIP(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
+    kernel<<<dim3((unsigned)p.blocks, (unsigned)(((D + 3) / 4 + p.LG - 1) / p.LG)), 256, lds, s>>>(
         ids, n, (int)V, g, ldg, (int)D, part, p.LG, p.chunk);
     BG_LAUNCH_CHECK();
     k_embedding_few_join<T><<<bg_grid_for(V * D, kFewCols), kFewCols * kFewSplit, 0, s>>>(part, p.blocks, V * D, scale, dw);
