@@ -5,7 +5,6 @@ nothing here falls back to PyTorch or to the CPU oracle.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes as C
 import os
 from typing import Optional
@@ -283,15 +282,10 @@ def stream() -> int:
     return torch.cuda.current_stream().cuda_stream
 
 
-def on_device(t: torch.Tensor):
-    """Context in which launches and allocations go to ``t``'s device (and to its current stream), whichever device is the
-    current one: nothing to do -- and nothing paid -- where they are the same."""
-    if t.device.index == (_get_device() if _get_device is not None else torch.cuda.current_device()):
-        return _HERE_ALREADY
-    return torch.cuda.device(t.device)
-
-
-_HERE_ALREADY = contextlib.nullcontext()
+def elsewhere(t: torch.Tensor) -> bool:
+    """Whether ``t`` lives on another device than the current one: the launches and allocations of an operator go to its
+    operands' device (and to the current stream there), so it runs itself again under ``torch.cuda.device(t.device)``."""
+    return t.get_device() != (_get_device() if _get_device is not None else torch.cuda.current_device())
 
 
 def require_device(t: torch.Tensor, what: str) -> None:

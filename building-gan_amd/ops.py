@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes as C
+import functools
 import threading
 from typing import List, Optional, Sequence
 
@@ -936,22 +937,24 @@ def _token_ids(ids: torch.Tensor, like: torch.Tensor, what: str) -> torch.Tensor
         raise _lib.BganError(f"{what}: ids must be int64 or int32, got {ids.dtype}")
     if ids.device != like.device:
         raise _lib.BganError(f"{what}: ids on {ids.device}, rows on {like.device}")
-    return ids.reshape(-1).contiguous()
+    return ids if ids.is_contiguous() else ids.contiguous()
 
 
 def embedding_raw(weight: torch.Tensor, ids: torch.Tensor, scale: float = 1.0) -> torch.Tensor:
     """``scale * weight[ids]`` [*ids.shape, D], zero rows where an id is outside [0, V) (bg_embedding_fwd: one launch)."""
     lib = _lib.load()
     _lib.require_device(weight, "embedding")
+    if _lib.elsewhere(weight):
+        with torch.cuda.device(weight.device):
+            return embedding_raw(weight, ids, scale)
     if weight.dim() != 2:
         raise _lib.BganError(f"embedding: weight must be [V, D], got {tuple(weight.shape)}")
     code, w, i = _elem(weight, "embedding"), _rows(weight), _token_ids(ids, weight, "embedding")
     V, D = w.shape
-    with _lib.on_device(w):
-        out = torch.empty(i.numel(), D, dtype=w.dtype, device=w.device)
-        check(lib.bg_embedding_fwd(code, ptr(w), _ld(w), V, ptr(i), i.dtype == torch.int64, i.numel(), D, scale, ptr(out), D,
-                                   stream()), "bg_embedding_fwd")
-    return out.view(*ids.shape, D)
+    out = torch.empty((*ids.shape, D), dtype=w.dtype, device=w.device)
+    check(lib.bg_embedding_fwd(code, w.data_ptr(), _ld(w), V, i.data_ptr(), i.dtype == torch.int64, i.numel(), D, scale,
+                               out.data_ptr(), D, stream()), "bg_embedding_fwd")
+    return out
 
 
 def embedding_grad_raw(g: torch.Tensor, ids: torch.Tensor, n_rows: int, scale: float = 1.0) -> torch.Tensor:
@@ -959,19 +962,21 @@ def embedding_grad_raw(g: torch.Tensor, ids: torch.Tensor, n_rows: int, scale: f
     (bg_embedding_bwd: ids sorted, fp32 sums in a fixed order)."""
     lib = _lib.load()
     _lib.require_device(g, "embedding_grad")
+    if _lib.elsewhere(g):
+        with torch.cuda.device(g.device):
+            return embedding_grad_raw(g, ids, n_rows, scale)
     code, i = _elem(g, "embedding_grad"), _token_ids(ids, g, "embedding_grad")
     if g.dim() != ids.dim() + 1 or g.shape[:-1] != ids.shape:
         raise _lib.BganError(f"embedding_grad: rows {tuple(g.shape)} do not belong to ids {tuple(ids.shape)}")
     if n_rows < 0:
         raise _lib.BganError("embedding_grad: n_rows must not be negative")
-    D = g.shape[-1]
-    g2 = _rows(g.reshape(i.numel(), D))
-    with _lib.on_device(g):
-        dw = torch.empty(n_rows, D, dtype=g.dtype, device=g.device)
-        size = lib.bg_embedding_bwd_workspace(code, i.numel(), n_rows, D)
-        ws = torch.empty(size, dtype=torch.uint8, device=g.device) if size else None
-        check(lib.bg_embedding_bwd(code, ptr(g2), _ld(g2), ptr(i), i.dtype == torch.int64, i.numel(), D, n_rows, scale, ptr(dw),
-                                   ptr(ws), size, stream()), "bg_embedding_bwd")
+    n, D = i.numel(), g.shape[-1]
+    g2 = _rows(g if g.dim() == 2 else g.reshape(n, D))
+    dw = torch.empty(n_rows, D, dtype=g.dtype, device=g.device)
+    size = lib.bg_embedding_bwd_workspace(code, n, n_rows, D)
+    ws = torch.empty(size, dtype=torch.uint8, device=g.device) if size else None
+    check(lib.bg_embedding_bwd(code, g2.data_ptr(), _ld(g2), i.data_ptr(), i.dtype == torch.int64, n, D, n_rows, scale, dw.data_ptr(),
+                               ptr(ws), size, stream()), "bg_embedding_bwd")
     return dw
 
 
@@ -1021,8 +1026,7 @@ def embedding(weight: torch.Tensor, ids: torch.Tensor, scale: float = 1.0, valid
 
 # ------------------------------------------------------------------------------- scan along segments
 def _scan_operands(x, gate, rowptr, h0, what):
-    """(type code, x, gate, row pointer, segments) as bg_gated_scan_* take them; BganError for what they do not take."""
-    _lib.require_device(x, what)
+    """(type code, x, gate, row pointer, segments, h0) as bg_gated_scan_* take them; BganError for what they do not take."""
     code = _elem(x, what)
     if x.dim() != 2 or gate.shape != x.shape:
         raise _lib.BganError(f"{what}: x and gate must be [rows, D] alike, got {tuple(x.shape)} and {tuple(gate.shape)}")
@@ -1037,55 +1041,71 @@ def _scan_operands(x, gate, rowptr, h0, what):
         rowptr, n_seg = None, rowptr
         if n_seg < 0 or (x.shape[0] % n_seg if n_seg else x.shape[0]):
             raise _lib.BganError(f"{what}: {x.shape[0]} rows are not {n_seg} segments of equal length")
-    if h0 is not None and (h0.dtype != torch.float32 or h0.device != x.device or tuple(h0.shape) != (n_seg, x.shape[1])):
-        raise _lib.BganError(f"{what}: h0 must be float32 [{n_seg}, {x.shape[1]}] on {x.device}, got {h0.dtype} {tuple(h0.shape)}")
-    return code, _rows(x), _rows(gate), rowptr, n_seg
+    if h0 is not None:
+        if h0.dtype != torch.float32 or h0.device != x.device or tuple(h0.shape) != (n_seg, x.shape[1]):
+            raise _lib.BganError(f"{what}: h0 must be float32 [{n_seg}, {x.shape[1]}] on {x.device}, got {h0.dtype} {tuple(h0.shape)}")
+        h0 = h0.contiguous()
+    return code, _rows(x), _rows(gate), rowptr, n_seg, h0
+
+
+@functools.lru_cache(maxsize=1024)
+def _scan_sizes(n_rows: int, D: int):
+    """(floats of the tiles' states, workspace bytes) of a scan over [n_rows, D]."""
+    lib = _lib.load()
+    return lib.bg_gated_scan_heads(n_rows, D), lib.bg_gated_scan_workspace(n_rows, D)
 
 
 def gated_scan_raw(x, gate, rowptr, h0=None, reverse: bool = False, keep_heads: bool = False):
     """(h, h_last, heads) of ``gated_scan`` on [rows, D] operands (bg_gated_scan_fwd); ``rowptr`` is the segments' int32 row
     pointer or, for segments of equal length, their number; ``heads`` (None unless kept) is what the backward pass takes."""
     lib = _lib.load()
-    code, x2, g2, rp, n_seg = _scan_operands(x, gate, rowptr, h0, "gated_scan")
-    N, D = x2.shape
-    h0c = None if h0 is None else h0.contiguous()
-    dev = x.device
-    with _lib.on_device(x):
-        h = torch.empty(N, D, dtype=x.dtype, device=dev)
-        h_last = torch.empty(n_seg, D, dtype=torch.float32, device=dev)
-        heads = torch.empty(lib.bg_gated_scan_heads(N, D), dtype=torch.float32, device=dev) if keep_heads else None
-        size = lib.bg_gated_scan_workspace(N, D)
-        ws = torch.empty(size, dtype=torch.uint8, device=dev)
-        check(lib.bg_gated_scan_fwd(code, ptr(x2), _ld(x2), ptr(g2), _ld(g2), ptr(rp), n_seg, N, D, ptr(h0c), reverse, ptr(h),
-                                    max(D, 1), ptr(h_last), ptr(heads), ptr(ws), size, stream()), "bg_gated_scan_fwd")
+    _lib.require_device(x, "gated_scan")
+    if _lib.elsewhere(x):
+        with torch.cuda.device(x.device):
+            return gated_scan_raw(x, gate, rowptr, h0, reverse, keep_heads)
+    code, x, gate, rp, n_seg, h0 = _scan_operands(x, gate, rowptr, h0, "gated_scan")
+    (N, D), dev = x.shape, x.device
+    n_heads, size = _scan_sizes(N, D)
+    h = torch.empty(N, D, dtype=x.dtype, device=dev)
+    h_last = torch.empty(n_seg, D, dtype=torch.float32, device=dev)
+    heads = torch.empty(n_heads, dtype=torch.float32, device=dev) if keep_heads else None
+    ws = torch.empty(size, dtype=torch.uint8, device=dev)
+    check(lib.bg_gated_scan_fwd(code, x.data_ptr(), _ld(x), gate.data_ptr(), _ld(gate), ptr(rp), n_seg, N, D, ptr(h0), reverse,
+                                h.data_ptr(), max(D, 1), h_last.data_ptr(), ptr(heads), ws.data_ptr(), size, stream()),
+          "bg_gated_scan_fwd")
     return h, h_last, heads
 
 
 def gated_scan_grad_raw(x, gate, rowptr, h0, reverse: bool, heads, dh, dlast, need_dh0: bool = True):
     """(dx, dgate, dh0) from the gradients of h (``dh``, may be None) and h_last (``dlast``, may be None)
     (bg_gated_scan_bwd); ``heads`` is the forward call's."""
-    lib = _lib.load()
-    code, x2, g2, rp, n_seg = _scan_operands(x, gate, rowptr, h0, "gated_scan_grad")
-    N, D = x2.shape
+    _lib.require_device(x, "gated_scan_grad")
+    if _lib.elsewhere(x):
+        with torch.cuda.device(x.device):
+            return gated_scan_grad_raw(x, gate, rowptr, h0, reverse, heads, dh, dlast, need_dh0)
+    code, x, gate, rp, n_seg, h0 = _scan_operands(x, gate, rowptr, h0, "gated_scan_grad")
     if dh is not None and (dh.dtype != x.dtype or dh.shape != x.shape or dh.device != x.device):
         raise _lib.BganError("gated_scan_grad: dh must be like x")
-    if dlast is not None and (dlast.dtype != torch.float32 or tuple(dlast.shape) != (n_seg, D) or dlast.device != x.device):
-        raise _lib.BganError(f"gated_scan_grad: dlast must be float32 [{n_seg}, {D}]")
-    if heads.numel() != lib.bg_gated_scan_heads(N, D) or heads.dtype != torch.float32:
+    if dlast is not None and (dlast.dtype != torch.float32 or tuple(dlast.shape) != (n_seg, x.shape[1]) or dlast.device != x.device):
+        raise _lib.BganError(f"gated_scan_grad: dlast must be float32 [{n_seg}, {x.shape[1]}]")
+    if heads.numel() != _scan_sizes(*x.shape)[0] or heads.dtype != torch.float32 or heads.device != x.device or not heads.is_contiguous():
         raise _lib.BganError("gated_scan_grad: heads are not a forward call's over these rows")
-    d2 = None if dh is None else _rows(dh)
-    dl = None if dlast is None else dlast.contiguous()
-    h0c = None if h0 is None else h0.contiguous()
-    dev = x.device
-    with _lib.on_device(x):
-        dx = torch.empty(N, D, dtype=x.dtype, device=dev)
-        dgate = torch.empty(N, D, dtype=x.dtype, device=dev)
-        dh0 = torch.empty(n_seg, D, dtype=torch.float32, device=dev) if need_dh0 else None
-        size = lib.bg_gated_scan_workspace(N, D)
-        ws = torch.empty(size, dtype=torch.uint8, device=dev)
-        check(lib.bg_gated_scan_bwd(code, ptr(x2), _ld(x2), ptr(g2), _ld(g2), ptr(d2), _ld(d2) if d2 is not None else 0, ptr(dl),
-                                    ptr(rp), n_seg, N, D, ptr(h0c), reverse, ptr(heads), ptr(dx), max(D, 1), ptr(dgate), max(D, 1),
-                                    ptr(dh0), ptr(ws), size, stream()), "bg_gated_scan_bwd")
+    return _scan_backward(code, x, gate, rp, n_seg, h0, reverse, heads, dh, dlast, need_dh0)
+
+
+def _scan_backward(code, x, gate, rp, n_seg, h0, reverse, heads, dh, dlast, need_dh0):
+    lib = _lib.load()
+    (N, D), dev = x.shape, x.device
+    dh = None if dh is None else _rows(dh)
+    dlast = None if dlast is None else dlast.contiguous()
+    dx = torch.empty(N, D, dtype=x.dtype, device=dev)
+    dgate = torch.empty(N, D, dtype=x.dtype, device=dev)
+    dh0 = torch.empty(n_seg, D, dtype=torch.float32, device=dev) if need_dh0 else None
+    size = _scan_sizes(N, D)[1]
+    ws = torch.empty(size, dtype=torch.uint8, device=dev)
+    check(lib.bg_gated_scan_bwd(code, x.data_ptr(), _ld(x), gate.data_ptr(), _ld(gate), ptr(dh), 0 if dh is None else _ld(dh), ptr(dlast),
+                                ptr(rp), n_seg, N, D, ptr(h0), reverse, heads.data_ptr(), dx.data_ptr(), max(D, 1), dgate.data_ptr(),
+                                max(D, 1), ptr(dh0), ws.data_ptr(), size, stream()), "bg_gated_scan_bwd")
     return dx, dgate, dh0
 
 
@@ -1096,19 +1116,19 @@ class GatedScan(torch.autograd.Function):
     def forward(ctx, x, gate, h0, rowptr, reverse: bool):
         h, h_last, heads = gated_scan_raw(x, gate, rowptr, h0, reverse, keep_heads=True)
         ctx.reverse = reverse
-        ctx.n_seg = None if isinstance(rowptr, torch.Tensor) else rowptr
-        ctx.save_for_backward(x, gate, h0, rowptr if ctx.n_seg is None else None, heads)
+        ctx.n_seg = h_last.shape[0]
+        ctx.save_for_backward(x, gate, h0, rowptr if isinstance(rowptr, torch.Tensor) else None, heads)
         ctx.set_materialize_grads(False)
         return h, h_last
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dh, dlast):
-        x, gate, h0, rowptr, heads = ctx.saved_tensors
         if dh is None and dlast is None:
             return None, None, None, None, None
-        dx, dgate, dh0 = gated_scan_grad_raw(x, gate, rowptr if ctx.n_seg is None else ctx.n_seg, h0, ctx.reverse, heads, dh, dlast,
-                                             need_dh0=ctx.needs_input_grad[2])
+        x, gate, h0, rp, heads = ctx.saved_tensors      # (checked by the forward call; autograd runs this on x's device)
+        dx, dgate, dh0 = _scan_backward(_ELEM[x.dtype], _rows(x), _rows(gate), None if rp is None else rp.contiguous(), ctx.n_seg,
+                                        None if h0 is None else h0.contiguous(), ctx.reverse, heads, dh, dlast, ctx.needs_input_grad[2])
         return dx, dgate, dh0, None, None
 
 
@@ -1138,7 +1158,7 @@ def gated_scan(x: torch.Tensor, gate: torch.Tensor, rowptr: Optional[torch.Tenso
         h, h_last = GatedScan.apply(x, gate, h0, rowptr, bool(reverse))
     else:
         h, h_last, _ = gated_scan_raw(x, gate, rowptr, h0, bool(reverse))
-    return h.view(shape), h_last
+    return (h if h.shape == shape else h.view(shape)), h_last
 
 
 def _shifted_overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
@@ -1160,19 +1180,21 @@ def gated_scan_step(x: torch.Tensor, gate: torch.Tensor, state: torch.Tensor, st
         raise _lib.BganError("gated_scan_step: x and gate must be [n, D] of one type")
     if state.shape != x.shape or state.dtype != torch.float32 or state.device != x.device:
         raise _lib.BganError(f"gated_scan_step: state must be float32 {tuple(x.shape)} on {x.device}")
+    if _lib.elsewhere(x):
+        with torch.cuda.device(x.device):
+            return gated_scan_step(x, gate, state, state_out)
     n, D = x.shape
-    x2, g2, s2 = _rows(x), _rows(gate), _rows(state)
-    with _lib.on_device(x):
-        h = torch.empty(n, D, dtype=x.dtype, device=x.device)
-        if state_out is None:
-            state_out = torch.empty(n, D, dtype=torch.float32, device=x.device)
-        elif (state_out.shape != x.shape or state_out.dtype != torch.float32 or state_out.device != x.device
-              or _rows(state_out) is not state_out):
-            raise _lib.BganError(f"gated_scan_step: state_out must be float32 {tuple(x.shape)} with contiguous rows on {x.device}")
-        elif _shifted_overlap(state_out, state):
-            raise _lib.BganError("gated_scan_step: state_out shares memory with state without being the same rows")
-        check(lib.bg_gated_scan_step(code, ptr(x2), _ld(x2), ptr(g2), _ld(g2), ptr(s2), _ld(s2), n, D, ptr(h), max(D, 1),
-                                     ptr(state_out), _ld(state_out), stream()), "bg_gated_scan_step")
+    x, gate, state = _rows(x), _rows(gate), _rows(state)
+    h = torch.empty(n, D, dtype=x.dtype, device=x.device)
+    if state_out is None:
+        state_out = torch.empty(n, D, dtype=torch.float32, device=x.device)
+    elif (state_out.shape != x.shape or state_out.dtype != torch.float32 or state_out.device != x.device
+          or _rows(state_out) is not state_out):
+        raise _lib.BganError(f"gated_scan_step: state_out must be float32 {tuple(x.shape)} with contiguous rows on {x.device}")
+    elif _shifted_overlap(state_out, state):
+        raise _lib.BganError("gated_scan_step: state_out shares memory with state without being the same rows")
+    check(lib.bg_gated_scan_step(code, x.data_ptr(), _ld(x), gate.data_ptr(), _ld(gate), state.data_ptr(), _ld(state), n, D, h.data_ptr(),
+                                 max(D, 1), state_out.data_ptr(), _ld(state_out), stream()), "bg_gated_scan_step")
     return h, state_out
 
 
