@@ -11,7 +11,7 @@
 // Rows are cut into tiles whatever the segments are.  A workgroup reads its tile ONCE, keeps it in registers, composes its
 // rows' maps, publishes the tile's map, finds the state that enters the tile from what the tiles before it published, and
 // walks its rows from there.  h is never read back: the backward pass rebuilds it from the fp32 state kept at the head of
-// every tile.
+// every row group, an eighth of the rows.
 #include "common.h"
 
 namespace {
@@ -148,14 +148,21 @@ __device__ __forceinline__ void store_rows(T* __restrict__ base, uint32_t off, u
                 if (i < l.nrows && e < l.nv) reinterpret_cast<T*>(p + (uint32_t)(off + i * step))[e] = bg_round<T>(v[i][e]);
     }
 }
-// fp32 rows of [n, D] (states): rare, element by element
+// four columns of fp32 rows of [n, D] (states)
 __device__ __forceinline__ void ld_state(const float* __restrict__ p, int64_t row, int64_t D, int64_t c, int nv, float (&v)[4]) {
+    if (p && nv == 4) {
+        const Piece<float> x = *reinterpret_cast<const Piece<float>*>(p + row * D + c);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = p && e < nv ? p[row * D + c + e] : 0.f;
+        for (int e = 0; e < 4; ++e) v[e] = x.v[e];
+    } else
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = p && e < nv ? p[row * D + c + e] : 0.f;
 }
 __device__ __forceinline__ void st_state(float* __restrict__ p, int64_t row, int64_t D, int64_t c, int nv, const float (&v)[4]) {
+    if (nv == 4) *reinterpret_cast<Piece<float>*>(p + row * D + c) = Piece<float>{{v[0], v[1], v[2], v[3]}};
+    else
 #pragma unroll
-    for (int e = 0; e < 4; ++e) if (e < nv) p[row * D + c + e] = v[e];
+        for (int e = 0; e < 4; ++e) if (e < nv) p[row * D + c + e] = v[e];
 }
 
 // ------------------------------------------------------------------------------------------------ maps
@@ -169,13 +176,15 @@ __device__ __forceinline__ uint32_t wave_mask(uint32_t m, int CG) {
 __device__ __forceinline__ bool bit(uint32_t m, int i) { return (m >> i) & 1; }
 
 struct Map { float A[4], B[4]; };
-// The values stay, what was computed from them does not: keeps the compiler from holding products of a walk over the rows in
-// registers until a later walk can use them again (a multiplication is cheaper than 32 registers).
-__device__ __forceinline__ void forget(float (&v)[kRows][4]) {
+// The value is computed here and what follows is computed from it: left to itself, the compiler moves the last steps of a
+// sigmoid to where its result is used, or keeps products of one walk over the rows for a later one, and either way holds a
+// row's worth of registers more than the values it has.
+__device__ __forceinline__ void settle(float& v) { asm volatile("" : "+v"(v)); }
+__device__ __forceinline__ void settle(float (&v)[kRows][4]) {
 #pragma unroll
     for (int i = 0; i < kRows; ++i)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) asm("" : "+v"(v[i][e]));
+        for (int e = 0; e < 4; ++e) settle(v[i][e]);
 }
 template <bool CUTS>
 __device__ __forceinline__ void after(Map& m, const float (&A1)[4], const float (&B1)[4]) {          // m <- m o (A1, B1)
@@ -280,8 +289,8 @@ __device__ __forceinline__ void await_words(const uint64_t* p, int n, uint64_t (
 }
 
 // sIn[column] = the state that enters tile number `k` of the walk; own[0 / 1][column]: A / B of the tile's map.  The first
-// CG * 4 threads, one column each.  Everything is asked for at once (a look at another workgroup's word takes about a
-// microsecond), and all that can be composed is composed before the state is waited for: a link of the chain is one load,
+// CG * 4 threads, one column each.  The tiles' words are asked for together and then the groups' (a look at another
+// workgroup's word takes about a microsecond; both at once measured the same and cost 14 registers), and all that can be composed is composed before the state is waited for: a link of the chain is one load,
 // one fma and one store.
 __device__ __forceinline__ void enter_tile(const Chain& ch, uint32_t k, uint32_t cb, const float* ownA, const float* ownB, float* sIn,
                                            uint32_t col) {
@@ -293,9 +302,8 @@ __device__ __forceinline__ void enter_tile(const Chain& ch, uint32_t k, uint32_t
     const uint32_t* before = state - (block > 0 ? (int64_t)ch.ncb * kMaxCols : 0);
     const float oA = ownA[col], oB = ownB[col];
     if (p < kGroup - 1) publish(tiles + p * kMaxCols, oA, oB);
-    uint64_t v[kGroup - 1], u[kGroup - 1];
+    uint64_t v[kGroup - 1];
     uint32_t w = __hip_atomic_load(before, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    peek_words(groups, u);
     peek_words(tiles, v);
     float A = 1.f, B = 0.f;                                              // of the group's tiles before this one
     await_words(tiles, p, v);
@@ -303,8 +311,9 @@ __device__ __forceinline__ void enter_tile(const Chain& ch, uint32_t k, uint32_t
     if (p == kGroup - 1 && gp < kGroup - 1)
         publish(groups + gp * kMaxCols, A < 0.f || oA < 0.f ? -1.f : oA * A, apply(oA, oB, B));
     float gA = 1.f, gB = 0.f;                                            // of the block's groups before this one
-    await_words(groups, gp, u);
-    then_words(gA, gB, u, gp);
+    peek_words(groups, v);
+    await_words(groups, gp, v);
+    then_words(gA, gB, v, gp);
     B = apply(A, B, gB);
     A = A < 0.f || gA < 0.f ? -1.f : A * gA;
     if (block > 0 && !__all(A < 0.f))                                        // behind a cut the state from further back is not needed
@@ -317,14 +326,6 @@ __device__ __forceinline__ void enter_tile(const Chain& ch, uint32_t k, uint32_t
         __hip_atomic_store(state, b, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
     sIn[col] = s;
-}
-
-// v <- the state before a segment's first row, where this lane has one
-__device__ __forceinline__ void enter_row(bool here, const float* __restrict__ p, int64_t row, int64_t D, int64_t c, int nv, float (&v)[4]) {
-    float s0[4];
-    ld_state(p, row, D, c, nv, s0);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = here ? s0[e] : v[e];
 }
 
 // The next (tile, column block) in the order of the walk; with a single tile there is nothing to order.  false: none left
@@ -357,29 +358,119 @@ __device__ __forceinline__ uint32_t row_off(int r, int rows, int64_t ld, int c) 
 template <class T, bool REV>
 __device__ __forceinline__ uint32_t row_step(int64_t ld) { return (REV ? 0u - (uint32_t)ld : (uint32_t)ld) * (uint32_t)sizeof(T); }
 
+// What the threads of a tile share
+struct TileShared {
+    int32_t first[2 * kThreads], last[2 * kThreads];                     // kThreads / CG * kRows rows, CG >= 4
+    uint32_t mask[kThreads / 4];
+    int32_t border;
+    WaveMaps wm;
+    float4 own[2][kMaxCols / 4], in[kMaxCols / 4];
+};
+
+// Where a thread stands: rows r0 .. of tile `tile`, four columns from c on
+struct Place {
+    int RG, cg, rg, r0, rows, cb;
+    int64_t row0, c0, c, low;
+    Lane l;
+};
+template <bool REV>
+__device__ __forceinline__ Place place(const Segs& g, int64_t D, int CG, int64_t tile, int cb) {
+    Place p;
+    p.RG = kThreads / CG; p.cg = threadIdx.x & (CG - 1); p.rg = threadIdx.x / CG; p.rows = p.RG * kRows; p.r0 = p.rg * kRows; p.cb = cb;
+    p.row0 = tile * p.rows; p.c0 = (int64_t)cb * (CG * 4); p.c = p.c0 + p.cg * 4; p.low = REV ? g.N - p.row0 - p.rows : p.row0;
+    const int64_t left = g.N - p.row0 - p.r0;
+    p.l.nv = p.c + 4 <= D ? 4 : p.c < D ? (int)(D - p.c) : 0;
+    p.l.nrows = left >= kRows ? kRows : left > 0 ? (int)left : 0;
+    return p;
+}
+template <class T, bool REV>
+__device__ __forceinline__ void load_tile(const T* __restrict__ m, int64_t ld, const Place& p, float fill, float (&v)[kRows][4]) {
+    load_rows(m + p.low * ld + p.c0, row_off<T, REV>(p.r0, p.rows, ld, p.cg * 4), row_step<T, REV>(ld), p.l, fill, v);
+}
+template <class T, bool REV>
+__device__ __forceinline__ void store_tile(T* __restrict__ m, int64_t ld, const Place& p, const float (&v)[kRows][4]) {
+    store_rows(m + p.low * ld + p.c0, row_off<T, REV>(p.r0, p.rows, ld, p.cg * 4), row_step<T, REV>(ld), p.l, v);
+}
+
+// The state before this thread's row group, `pre` being the map of the tile's groups before it: through the chain, unless the
+// walk is a single tile.  What stands between `ask` and `answer` is done by the other waves while the first one waits.
+__device__ __forceinline__ void ask(const Chain& ch, int64_t k, int64_t n_tiles, int64_t D, int CG, const Place& p, bool last_group,
+                                    const Map& all, TileShared& sh) {
+    if (n_tiles == 1) return;
+    if (last_group) {
+        sh.own[0][p.cg] = make_float4(all.A[0], all.A[1], all.A[2], all.A[3]);
+        sh.own[1][p.cg] = make_float4(all.B[0], all.B[1], all.B[2], all.B[3]);
+    }
+    __syncthreads();
+    if ((int)threadIdx.x < CG * 4 && p.c0 + threadIdx.x < D)
+        enter_tile(ch, (uint32_t)k, (uint32_t)p.cb, &sh.own[0][0].x, &sh.own[1][0].x, &sh.in[0].x, threadIdx.x);
+}
+__device__ __forceinline__ void answer(int64_t n_tiles, const Place& p, const Map& pre, const TileShared& sh, float (&s)[4]) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s[e] = 0.f;
+    if (n_tiles > 1) {
+        __syncthreads();
+        const float4 v = sh.in[p.cg];
+        s[0] = v.x; s[1] = v.y; s[2] = v.z; s[3] = v.w;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s[e] = apply(pre.A[e], pre.B[e], s[e]);
+}
+
+// to[s] = from[s] (or 0) for the segments without rows, dealt out to the tiles
+template <bool REV>
+__device__ __forceinline__ void pass_through(const Segs& g, int64_t D, int64_t tile, int64_t n_tiles, const Place& p,
+                                             const float* __restrict__ from, float* __restrict__ to) {
+    if (!to || p.rg != 0) return;
+    for (int64_t j = tile; j < g.S; j += n_tiles)
+        if (seg_lo<REV, true>(g, j) >= seg_lo<REV, true>(g, j + 1)) {
+            const int64_t s = REV ? g.S - 1 - j : j;
+            float v[4];
+            ld_state(from, s, D, p.c, p.l.nv, v);
+            st_state(to, s, D, p.c, p.l.nv, v);
+        }
+}
+
+// Borders as a thread sees them: its own row group's first / last rows of segments and rows in no segment, and which rows
+// have one in any of the wave's groups (branches are the wave's, what a lane does there is selection).
+struct Borders {
+    uint32_t m, none, enter, leave, wave_enter, wave_leave;
+    __device__ __forceinline__ Borders(const TileShared& sh, const Place& p, int CG, bool border)
+        : m(0), none(0), enter(0), leave(0), wave_enter(0), wave_leave(0) {
+        if (__builtin_expect(border, 0)) {
+            m = sh.mask[p.rg];
+            none = m >> 16;
+            enter = (m | none) & 0xFF;
+            leave = (m >> 8 | none) & 0xFF;
+            wave_enter = wave_mask(enter, CG);
+            wave_leave = wave_mask(leave, CG);
+        }
+    }
+};
+// s <- the state before row i of the group where a segment begins there (0 where the row is in none)
+__device__ __forceinline__ void enter_row(const Borders& w, int i, const TileShared& sh, const Place& p, const float* __restrict__ h0, int64_t D,
+                                          float (&s)[4]) {
+    const bool seg = bit(w.m, i);
+    float s0[4];
+    ld_state(seg ? h0 : nullptr, seg ? sh.first[p.r0 + i] : 0, D, p.c, p.l.nv, s0);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s[e] = bit(w.enter, i) ? s0[e] : s[e];
+}
+
 // ------------------------------------------------------------------------------------------------ forward
 template <class T, bool REV>
-__global__ __launch_bounds__(kThreads) void k_scan_fwd(const T* __restrict__ x, int64_t ldx, const T* __restrict__ gate, int64_t ldg,
-                                                          Segs g, int64_t D, const float* __restrict__ h0, int CG, Chain ch,
-                                                          int64_t n_tiles, T* __restrict__ h, int64_t ldh, float* __restrict__ h_last,
-                                                          float* __restrict__ heads) {
-    __shared__ int32_t first[2 * kThreads], last[2 * kThreads];            // kThreads / CG * kRows rows, CG >= 4
-    __shared__ uint32_t mask[kThreads / 4];
-    __shared__ int32_t border;
-    __shared__ WaveMaps wm;
-    __shared__ float4 own[2][kMaxCols / 4], sIn[kMaxCols / 4];
+__global__ __launch_bounds__(kThreads, 4) void k_scan_fwd(const T* __restrict__ x, int64_t ldx, const T* __restrict__ gate, int64_t ldg, Segs g,
+                                                       int64_t D, const float* __restrict__ h0, int CG, Chain ch, int64_t n_tiles,
+                                                       T* __restrict__ h, int64_t ldh, float* __restrict__ h_last, float* __restrict__ heads) {
+    __shared__ TileShared sh;
     int64_t tile;
     int cb;
     if (!take_tile(ch, n_tiles, tile, cb)) return;
-    const int RG = kThreads / CG, cg = threadIdx.x & (CG - 1), rg = threadIdx.x / CG, rows = RG * kRows, r0 = rg * kRows;
-    const int64_t row0 = tile * rows, c0 = (int64_t)cb * (CG * 4), c = c0 + cg * 4, low = REV ? g.N - row0 - rows : row0;
-    const int64_t left = g.N - row0 - r0;
-    const Lane l{c + 4 <= D ? 4 : c < D ? (int)(D - c) : 0, left >= kRows ? kRows : left > 0 ? (int)left : 0};
-    if (threadIdx.x < 64) mark_tile<REV>(g, row0, RG, mask, first, last, border);
-    float a[kRows][4], b[kRows][4];
-    // where there is no row: a = 1, b = 0, the map that changes nothing
-    load_rows(gate + low * ldg + c0, row_off<T, REV>(r0, rows, ldg, cg * 4), row_step<T, REV>(ldg), l, __builtin_inff(), a);
-    load_rows(x + low * ldx + c0, row_off<T, REV>(r0, rows, ldx, cg * 4), row_step<T, REV>(ldx), l, 0.f, b);
+    const Place p = place<REV>(g, D, CG, tile, cb);
+    if (threadIdx.x < 64) mark_tile<REV>(g, p.row0, p.RG, sh.mask, sh.first, sh.last, sh.border);
+    float a[kRows][4], b[kRows][4];                                      // a row's map: s -> a s + b, b = c x
+    load_tile<T, REV>(gate, ldg, p, __builtin_inff(), a);                // where there is no row: a = 1, b = 0, the map that
+    load_tile<T, REV>(x, ldx, p, 0.f, b);                                // changes nothing
 #pragma unroll
     for (int i = 0; i < kRows; ++i)
 #pragma unroll
@@ -387,178 +478,111 @@ __global__ __launch_bounds__(kThreads) void k_scan_fwd(const T* __restrict__ x, 
             float ce;
             gate_pair(a[i][e], a[i][e], ce);
             b[i][e] *= ce;
+            settle(a[i][e]);
+            settle(b[i][e]);
         }
     __syncthreads();
-    const uint32_t m = mask[rg], cuts = (m | m >> 16) & 0xFF;
-    const bool tile_any = __builtin_amdgcn_readfirstlane(border) != 0;
-    const bool any = __builtin_expect(tile_any && __any(m != 0), 0);     // most waves see no segment begin or end
+    const bool border = __builtin_amdgcn_readfirstlane(sh.border) != 0;
+    const Borders w(sh, p, CG, border);
     Map f{{1.f, 1.f, 1.f, 1.f}, {0.f, 0.f, 0.f, 0.f}};
-    if (!any) {
 #pragma unroll
-        for (int i = 0; i < kRows; ++i)
+    for (int i = 0; i < kRows; ++i) {
+        if (bit(w.wave_enter, i)) {
+            enter_row(w, i, sh, p, h0, D, f.B);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) f.B[e] = fmaf(a[i][e], f.B[e], b[i][e]);
-    } else {
-        for (uint32_t todo = wave_mask(cuts, CG); todo; todo &= todo - 1) {          // one row after the other
-            const int at = __builtin_ctz(todo);
-            const bool here = bit(cuts, at), seg = bit(m, at);           // here, but not seg: a row in no segment
-            float s0[4];
-            ld_state(seg ? h0 : nullptr, seg ? first[r0 + at] : 0, D, c, l.nv, s0);
-#pragma unroll
-            for (int i = 0; i < kRows; ++i)
-                if (i == at)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        b[i][e] = !here ? b[i][e] : seg ? fmaf(a[i][e], s0[e], b[i][e]) : 0.f;
-                        a[i][e] = here ? -1.f : a[i][e];
-                    }
+            for (int e = 0; e < 4; ++e) {                                // a row in no segment: 0, whatever it holds
+                a[i][e] = bit(w.none, i) ? 0.f : a[i][e];
+                b[i][e] = bit(w.none, i) ? 0.f : b[i][e];
+            }
         }
 #pragma unroll
-        for (int i = 0; i < kRows; ++i)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) f.B[e] = apply(a[i][e], b[i][e], f.B[e]);
-    }
-#pragma unroll
-    for (int i = 0; i < kRows; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) f.A[e] *= a[i][e];
-    if (cuts)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) f.A[e] = -1.f;
-    const Map all = tile_any ? before_group<false, true>(f, CG, cg, wm) : before_group<false, false>(f, CG, cg, wm);
-    float s[4] = {0.f, 0.f, 0.f, 0.f};
-    if (n_tiles > 1) {
-        if (rg == RG - 1) {
-            own[0][cg] = make_float4(all.A[0], all.A[1], all.A[2], all.A[3]);
-            own[1][cg] = make_float4(all.B[0], all.B[1], all.B[2], all.B[3]);
+        for (int e = 0; e < 4; ++e) {
+            f.B[e] = fmaf(a[i][e], f.B[e], b[i][e]);
+            f.A[e] *= a[i][e];
         }
-        __syncthreads();
-        if ((int)threadIdx.x < CG * 4 && c0 + threadIdx.x < D)
-            enter_tile(ch, (uint32_t)tile, (uint32_t)cb, &own[0][0].x, &own[1][0].x, &sIn[0].x, threadIdx.x);
-        __syncthreads();
-        const float4 v = sIn[cg];
-        s[0] = v.x; s[1] = v.y; s[2] = v.z; s[3] = v.w;
     }
 #pragma unroll
-    for (int e = 0; e < 4; ++e) s[e] = apply(f.A[e], f.B[e], s[e]);
-    if (heads && rg == 0) st_state(heads, tile, D, c, l.nv, s);
-    if (!any) {
+    for (int e = 0; e < 4; ++e) f.A[e] = w.enter ? -1.f : f.A[e];
+    const Map all = border ? before_group<false, true>(f, CG, p.cg, sh.wm) : before_group<false, false>(f, CG, p.cg, sh.wm);
+    float s[4];
+    ask(ch, tile, n_tiles, D, CG, p, p.rg == p.RG - 1, all, sh);
+    answer(n_tiles, p, f, sh, s);
+    if (heads && p.l.nrows > 0) st_state(heads, tile * p.RG + p.rg, D, p.c, p.l.nv, s);
 #pragma unroll
-        for (int i = 0; i < kRows; ++i)
+    for (int i = 0; i < kRows; ++i) {
+        if (bit(w.wave_enter, i)) enter_row(w, i, sh, p, h0, D, s);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) b[i][e] = s[e] = fmaf(a[i][e], s[e], b[i][e]);
-    } else {
-#pragma unroll
-        for (int i = 0; i < kRows; ++i)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) b[i][e] = s[e] = apply(a[i][e], b[i][e], s[e]);
-        if (h_last)
-            for (uint32_t todo = wave_mask(m >> 8, CG) & 0xFF; todo; todo &= todo - 1) {
-                const int at = __builtin_ctz(todo);
-#pragma unroll
-                for (int i = 0; i < kRows; ++i)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) s[e] = i == at ? b[i][e] : s[e];
-                if (bit(m, 8 + at)) st_state(h_last, last[r0 + at], D, c, l.nv, s);
-            }
+        for (int e = 0; e < 4; ++e) b[i][e] = s[e] = fmaf(a[i][e], s[e], b[i][e]);
+        if (bit(w.wave_leave, i) && h_last && bit(w.m, 8 + i)) st_state(h_last, sh.last[p.r0 + i], D, p.c, p.l.nv, s);
     }
-    store_rows(h + low * ldh + c0, row_off<T, REV>(r0, rows, ldh, cg * 4), row_step<T, REV>(ldh), l, b);
-    if (h_last && rg == 0)                                               // segments without rows: the state passes through
-        for (int64_t k = tile; k < g.S; k += n_tiles)
-            if (seg_lo<REV, true>(g, k) >= seg_lo<REV, true>(g, k + 1)) {
-                const int64_t sg = REV ? g.S - 1 - k : k;
-                float v[4];
-                ld_state(h0, sg, D, c, l.nv, v);
-                st_state(h_last, sg, D, c, l.nv, v);
-            }
+    store_tile<T, REV>(h, ldh, p, b);
+    pass_through<REV>(g, D, tile, n_tiles, p, h0, h_last);
 }
 
 // ------------------------------------------------------------------------------------------------ backward
-// The walk for mu goes from the last tile to the first; h inside the tile comes from heads.  Kept per element: a, c, dh and
-// q = (h_before - x) a c, so dx = c lam and dgate = q lam.
+// The walk for mu goes from the last tile to the first.  h before a row group was kept by the forward pass, so
+// q = (h_before - x) a c is made while the tile's state is asked for; per element a, c, dh and q stay: dx = c lam,
+// dgate = q lam.
 template <class T, bool REV>
 __global__ __launch_bounds__(kThreads) void k_scan_bwd(const T* __restrict__ x, int64_t ldx, const T* __restrict__ gate, int64_t ldg,
-                                                             const T* __restrict__ dh, int64_t lddh, const float* __restrict__ dlast,
-                                                             Segs g, int64_t D, const float* __restrict__ h0, int CG, Chain ch,
-                                                             int64_t n_tiles, const float* __restrict__ heads, T* __restrict__ dx,
-                                                             int64_t lddx, T* __restrict__ dgate, int64_t lddg, float* __restrict__ dh0) {
-    __shared__ int32_t first[2 * kThreads], last[2 * kThreads];
-    __shared__ uint32_t mask[kThreads / 4];
-    __shared__ int32_t border;
-    __shared__ WaveMaps wm;
-    __shared__ float4 own[2][kMaxCols / 4], sIn[kMaxCols / 4];
+                                                       const T* __restrict__ dh, int64_t lddh, const float* __restrict__ dlast, Segs g,
+                                                       int64_t D, const float* __restrict__ h0, int CG, Chain ch, int64_t n_tiles,
+                                                       const float* __restrict__ heads, T* __restrict__ dx, int64_t lddx,
+                                                       T* __restrict__ dgate, int64_t lddg, float* __restrict__ dh0) {
+    __shared__ TileShared sh;
     int64_t k;
     int cb;
     if (!take_tile(ch, n_tiles, k, cb)) return;
     const int64_t tile = n_tiles - 1 - k;
-    const int RG = kThreads / CG, cg = threadIdx.x & (CG - 1), rg = threadIdx.x / CG, rows = RG * kRows, r0 = rg * kRows;
-    const int64_t row0 = tile * rows, c0 = (int64_t)cb * (CG * 4), c = c0 + cg * 4, low = REV ? g.N - row0 - rows : row0;
-    const int64_t left = g.N - row0 - r0;
-    const Lane l{c + 4 <= D ? 4 : c < D ? (int)(D - c) : 0, left >= kRows ? kRows : left > 0 ? (int)left : 0};
-    if (threadIdx.x < 64) mark_tile<REV>(g, row0, RG, mask, first, last, border);
+    const Place p = place<REV>(g, D, CG, tile, cb);
+    if (threadIdx.x < 64) mark_tile<REV>(g, p.row0, p.RG, sh.mask, sh.first, sh.last, sh.border);
     float a[kRows][4], cc[kRows][4], q[kRows][4], d[kRows][4], s[4];
-    load_rows(gate + low * ldg + c0, row_off<T, REV>(r0, rows, ldg, cg * 4), row_step<T, REV>(ldg), l, __builtin_inff(), a);
-    load_rows(x + low * ldx + c0, row_off<T, REV>(r0, rows, ldx, cg * 4), row_step<T, REV>(ldx), l, 0.f, q);
-    if (dh) load_rows(dh + low * lddh + c0, row_off<T, REV>(r0, rows, lddh, cg * 4), row_step<T, REV>(lddh), l, 0.f, d);
+    load_tile<T, REV>(gate, ldg, p, __builtin_inff(), a);
+    ld_state(heads, tile * p.RG + p.rg, D, p.c, p.l.nrows > 0 ? p.l.nv : 0, s);
+    load_tile<T, REV>(x, ldx, p, 0.f, q);
+    if (dh) load_tile<T, REV>(dh, lddh, p, 0.f, d);
     else
 #pragma unroll
         for (int i = 0; i < kRows; ++i)
 #pragma unroll
             for (int e = 0; e < 4; ++e) d[i][e] = 0.f;
-    ld_state(heads, tile, D, c, l.nv, s);
 #pragma unroll
     for (int i = 0; i < kRows; ++i)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) gate_pair(a[i][e], a[i][e], cc[i][e]);
-    __syncthreads();
-    const uint32_t m = mask[rg], none = m >> 16, fcut = (m | none) & 0xFF, lcut = (m >> 8 | none) & 0xFF;
-    uint32_t wf = 0, wl = 0;                                             // rows with a border in any of the wave's groups
-    const bool tile_any = __builtin_amdgcn_readfirstlane(border) != 0;
-    if (__builtin_expect(tile_any, 0)) { wf = wave_mask(fcut, CG); wl = wave_mask(lcut, CG); }
-    Map f{{1.f, 1.f, 1.f, 1.f}, {0.f, 0.f, 0.f, 0.f}}, u;                // of h down to the group's end, of mu up to its head
-#pragma unroll
-    for (int i = 0; i < kRows; ++i) {
-        if (bit(wf, i)) enter_row(bit(fcut, i), bit(m, i) ? h0 : nullptr, bit(m, i) ? first[r0 + i] : 0, D, c, l.nv, f.B);
-#pragma unroll
         for (int e = 0; e < 4; ++e) {
-            f.B[e] = fmaf(a[i][e], f.B[e], cc[i][e] * q[i][e]);
-            f.A[e] *= a[i][e];
+            gate_pair(a[i][e], a[i][e], cc[i][e]);
+            settle(a[i][e]);
+            settle(cc[i][e]);
         }
-    }
-    forget(a);
-    u = f;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) u.B[e] = 0.f;
+    __syncthreads();
+    const bool border = __builtin_amdgcn_readfirstlane(sh.border) != 0;
+    const Borders w(sh, p, CG, border);
+    Map u{{1.f, 1.f, 1.f, 1.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
     for (int i = kRows - 1; i >= 0; --i) {
-        if (bit(wl, i)) {
-            const bool seg = bit(m, 8 + i);
+        if (bit(w.wave_leave, i)) {
+            const bool seg = bit(w.m, 8 + i);
             float ds[4];
-            ld_state(seg ? dlast : nullptr, seg ? last[r0 + i] : 0, D, c, l.nv, ds);
+            ld_state(seg ? dlast : nullptr, seg ? sh.last[p.r0 + i] : 0, D, p.c, p.l.nv, ds);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                d[i][e] = bit(none, i) ? 0.f : d[i][e] + ds[e];
-                u.B[e] = bit(lcut, i) ? 0.f : u.B[e];
+                d[i][e] = bit(w.none, i) ? 0.f : d[i][e] + ds[e];
+                u.B[e] = bit(w.leave, i) ? 0.f : u.B[e];
             }
         }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) u.B[e] = a[i][e] * (d[i][e] + u.B[e]);
+        for (int e = 0; e < 4; ++e) {
+            u.B[e] = a[i][e] * (d[i][e] + u.B[e]);
+            u.A[e] *= a[i][e];
+        }
     }
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        if (fcut) f.A[e] = -1.f;
-        if (lcut) u.A[e] = -1.f;
-    }
-    if (tile_any) before_group<false, true>(f, CG, cg, wm);
-    else before_group<false, false>(f, CG, cg, wm);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) s[e] = apply(f.A[e], f.B[e], s[e]);
-    __syncthreads();                                                     // wm is written again
-    const Map all = tile_any ? before_group<true, true>(u, CG, cg, wm) : before_group<true, false>(u, CG, cg, wm);
-    forget(cc);
+    for (int e = 0; e < 4; ++e) u.A[e] = w.leave ? -1.f : u.A[e];
+    const Map all = border ? before_group<true, true>(u, CG, p.cg, sh.wm) : before_group<true, false>(u, CG, p.cg, sh.wm);
+    ask(ch, k, n_tiles, D, CG, p, p.rg == 0, all, sh);
 #pragma unroll
     for (int i = 0; i < kRows; ++i) {
-        if (bit(wf, i)) enter_row(bit(fcut, i), bit(m, i) ? h0 : nullptr, bit(m, i) ? first[r0 + i] : 0, D, c, l.nv, s);
+        if (bit(w.wave_enter, i)) enter_row(w, i, sh, p, h0, D, s);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const float xi = q[i][e], hb = s[e];
@@ -566,28 +590,12 @@ __global__ __launch_bounds__(kThreads) void k_scan_bwd(const T* __restrict__ x, 
             q[i][e] = (hb - xi) * (a[i][e] * cc[i][e]);
         }
     }
-#pragma unroll
-    for (int e = 0; e < 4; ++e) s[e] = 0.f;
-    if (n_tiles > 1) {
-        if (rg == 0) {
-            own[0][cg] = make_float4(all.A[0], all.A[1], all.A[2], all.A[3]);
-            own[1][cg] = make_float4(all.B[0], all.B[1], all.B[2], all.B[3]);
-        }
-        __syncthreads();
-        if ((int)threadIdx.x < CG * 4 && c0 + threadIdx.x < D)
-            enter_tile(ch, (uint32_t)k, (uint32_t)cb, &own[0][0].x, &own[1][0].x, &sIn[0].x, threadIdx.x);
-        __syncthreads();
-        const float4 v = sIn[cg];
-        s[0] = v.x; s[1] = v.y; s[2] = v.z; s[3] = v.w;
-    }
-#pragma unroll
-    for (int e = 0; e < 4; ++e) s[e] = apply(u.A[e], u.B[e], s[e]);
+    answer(n_tiles, p, u, sh, s);
 #pragma unroll
     for (int i = kRows - 1; i >= 0; --i) {
-        if (bit(wl, i)) {
+        if (bit(w.wave_leave, i))
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s[e] = bit(lcut, i) ? 0.f : s[e];
-        }
+            for (int e = 0; e < 4; ++e) s[e] = bit(w.leave, i) ? 0.f : s[e];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const float lam = d[i][e] + s[e];
@@ -595,25 +603,18 @@ __global__ __launch_bounds__(kThreads) void k_scan_bwd(const T* __restrict__ x, 
             q[i][e] *= lam;
             s[e] = a[i][e] * lam;
         }
-        if (bit(wf, i)) {
+        if (bit(w.wave_enter, i)) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {                                // rows in no segment: 0, whatever they hold
-                cc[i][e] = bit(none, i) ? 0.f : cc[i][e];
-                q[i][e] = bit(none, i) ? 0.f : q[i][e];
+                cc[i][e] = bit(w.none, i) ? 0.f : cc[i][e];
+                q[i][e] = bit(w.none, i) ? 0.f : q[i][e];
             }
-            if (bit(m, i) && dh0) st_state(dh0, first[r0 + i], D, c, l.nv, s);
+            if (bit(w.m, i) && dh0) st_state(dh0, sh.first[p.r0 + i], D, p.c, p.l.nv, s);
         }
     }
-    store_rows(dx + low * lddx + c0, row_off<T, REV>(r0, rows, lddx, cg * 4), row_step<T, REV>(lddx), l, cc);
-    store_rows(dgate + low * lddg + c0, row_off<T, REV>(r0, rows, lddg, cg * 4), row_step<T, REV>(lddg), l, q);
-    if (dh0 && rg == 0)
-        for (int64_t j = tile; j < g.S; j += n_tiles)
-            if (seg_lo<REV, true>(g, j) >= seg_lo<REV, true>(g, j + 1)) {
-                const int64_t sgm = REV ? g.S - 1 - j : j;
-                float v[4];
-                ld_state(dlast, sgm, D, c, l.nv, v);
-                st_state(dh0, sgm, D, c, l.nv, v);
-            }
+    store_tile<T, REV>(dx, lddx, p, cc);
+    store_tile<T, REV>(dgate, lddg, p, q);
+    pass_through<REV>(g, D, tile, n_tiles, p, dlast, dh0);
 }
 
 // ------------------------------------------------------------------------------------------------ one row per segment
@@ -708,7 +709,7 @@ __global__ __launch_bounds__(256) void k_copy_or_zero(const float* __restrict__ 
 
 }  // namespace
 
-extern "C" int64_t bg_gated_scan_heads(int64_t n_rows, int64_t D) { return n_rows > 0 && D > 0 ? tiles_of(n_rows, D) * D : 0; }
+extern "C" int64_t bg_gated_scan_heads(int64_t n_rows, int64_t D) { return n_rows > 0 && D > 0 ? tiles_of(n_rows, D) * (kThreads / column_groups(D)) * D : 0; }
 
 extern "C" int64_t bg_gated_scan_workspace(int64_t n_rows, int64_t D) { return n_rows > 0 && D > 0 ? scan_ws(n_rows, D).bytes : 0; }
 

@@ -152,7 +152,7 @@ int bg_embedding_bwd(int dtype, const void* g, int64_t ldg, const void* ids, int
  * after a segment's rows; a segment without rows passes h0 through.  Rows in no segment (before rowptr[0], from
  * rowptr[n_seg] on) are zero in h.  rowptr: int32 [n_seg + 1], non-decreasing; entries outside [0, n_rows] are taken as
  * the nearer end.  rowptr NULL: n_seg segments of n_rows / n_seg rows each.  The state is fp32; h is rounded once.
- * heads (may be NULL): fp32 [bg_gated_scan_heads(n_rows, D)], the state at the head of every tile of rows, which the
+ * heads (may be NULL): fp32 [bg_gated_scan_heads(n_rows, D)], the state before every eighth row, which the
  * backward pass takes.  ws: bg_gated_scan_workspace(n_rows, D) bytes, 16-byte aligned (BG_ERR_SCRATCH when ws_bytes is
  * less); it needs no preparation.  x, gate and h in pieces of four elements where D, the pitches and the addresses allow.
  * n_rows < 2^31, D <= 2^20 (BG_ERR_SHAPE).  Equal inputs give equal bits.

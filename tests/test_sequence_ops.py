@@ -73,7 +73,7 @@ def test_entry_points_refuse_bad_arguments_before_any_launch():
     assert bwd(V=0) == 0 and bwd(D=0, ldg=0) == 0
     size = lib.bg_gated_scan_workspace(10, 8)
     heads = lib.bg_gated_scan_heads(10, 8)
-    assert size > 0 and heads == 8 and lib.bg_gated_scan_workspace(0, 8) == 0
+    assert size > 0 and heads >= 2 * 8 and lib.bg_gated_scan_workspace(0, 8) == 0
     scan = lambda **k: lib.bg_gated_scan_fwd(*{**dict(dt=0, x=p, ldx=8, g=p, ldg=8, rp=p, S=2, N=10, D=8, h0=None, rev=0, h=p, ldh=8, hl=p,
                                                       heads=None, ws=p, size=size, s=None), **k}.values())
     assert scan(dt=7) == -1 and scan(ldx=7) == -1 and scan(ldg=7) == -1 and scan(ldh=7) == -1 and scan(x=None) == -1
