@@ -129,6 +129,26 @@ __device__ __forceinline__ void load_rows(const T* __restrict__ base, uint32_t o
                 v[i][e] = i < l.nrows && e < l.nv ? (float)reinterpret_cast<const T*>(p + (uint32_t)(off + i * step))[e] : fill;
     }
 }
+// Rows as they came from memory: 16-bit elements stay two to a register until they are used
+template <class T>
+struct Raw {
+    Piece<T> v[kRows];
+    __device__ __forceinline__ float get(int i, int e) const { return (float)v[i].v[e]; }
+};
+template <class T>
+__device__ __forceinline__ void load_raw(const T* __restrict__ base, uint32_t off, uint32_t step, Lane l, Raw<T>& r) {
+    const char* p = reinterpret_cast<const char*>(base);
+    if (__builtin_expect(l.whole(), 1)) {
+#pragma unroll
+        for (int i = 0; i < kRows; ++i) r.v[i] = *reinterpret_cast<const Piece<T>*>(p + (uint32_t)(off + i * step));
+    } else {
+#pragma unroll
+        for (int i = 0; i < kRows; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                r.v[i].v[e] = i < l.nrows && e < l.nv ? reinterpret_cast<const T*>(p + (uint32_t)(off + i * step))[e] : (T)0.f;
+    }
+}
 template <class T>
 __device__ __forceinline__ void store_rows(T* __restrict__ base, uint32_t off, uint32_t step, Lane l, const float (&v)[kRows][4]) {
     char* p = reinterpret_cast<char*>(base);
@@ -180,6 +200,14 @@ struct Map { float A[4], B[4]; };
 // sigmoid to where its result is used, or keeps products of one walk over the rows for a later one, and either way holds a
 // row's worth of registers more than the values it has.
 __device__ __forceinline__ void settle(float& v) { asm volatile("" : "+v"(v)); }
+template <class T>
+__device__ __forceinline__ void settle(Raw<T>& r) {
+    uint32_t w[sizeof(T) * kRows];
+    __builtin_memcpy(w, &r, sizeof(w));
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) * kRows; ++i) asm volatile("" : "+v"(w[i]));
+    __builtin_memcpy(&r, w, sizeof(w));
+}
 __device__ __forceinline__ void settle(float (&v)[kRows][4]) {
 #pragma unroll
     for (int i = 0; i < kRows; ++i)
@@ -388,6 +416,10 @@ __device__ __forceinline__ void load_tile(const T* __restrict__ m, int64_t ld, c
     load_rows(m + p.low * ld + p.c0, row_off<T, REV>(p.r0, p.rows, ld, p.cg * 4), row_step<T, REV>(ld), p.l, fill, v);
 }
 template <class T, bool REV>
+__device__ __forceinline__ void load_tile(const T* __restrict__ m, int64_t ld, const Place& p, Raw<T>& r) {
+    load_raw(m + p.low * ld + p.c0, row_off<T, REV>(p.r0, p.rows, ld, p.cg * 4), row_step<T, REV>(ld), p.l, r);
+}
+template <class T, bool REV>
 __device__ __forceinline__ void store_tile(T* __restrict__ m, int64_t ld, const Place& p, const float (&v)[kRows][4]) {
     store_rows(m + p.low * ld + p.c0, row_off<T, REV>(p.r0, p.rows, ld, p.cg * 4), row_step<T, REV>(ld), p.l, v);
 }
@@ -455,6 +487,20 @@ __device__ __forceinline__ void enter_row(const Borders& w, int i, const TileSha
     ld_state(seg ? h0 : nullptr, seg ? sh.first[p.r0 + i] : 0, D, p.c, p.l.nv, s0);
 #pragma unroll
     for (int e = 0; e < 4; ++e) s[e] = bit(w.enter, i) ? s0[e] : s[e];
+}
+
+// Row i of the group from above: where a segment ends there (or the row is in none) nothing comes in, s <- 0, and the gradient
+// d of its h takes that of the segment's last state (or is 0)
+__device__ __forceinline__ void leave_row(const Borders& w, int i, const TileShared& sh, const Place& p, const float* __restrict__ dlast,
+                                          int64_t D, float (&d)[4], float (&s)[4]) {
+    const bool seg = bit(w.m, 8 + i);
+    float ds[4];
+    ld_state(seg ? dlast : nullptr, seg ? sh.last[p.r0 + i] : 0, D, p.c, p.l.nv, ds);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        d[e] = bit(w.none, i) ? 0.f : d[e] + ds[e];
+        s[e] = bit(w.leave, i) ? 0.f : s[e];
+    }
 }
 
 // ------------------------------------------------------------------------------------------------ forward
@@ -536,16 +582,17 @@ __global__ __launch_bounds__(kThreads) void k_scan_bwd(const T* __restrict__ x, 
     const int64_t tile = n_tiles - 1 - k;
     const Place p = place<REV>(g, D, CG, tile, cb);
     if (threadIdx.x < 64) mark_tile<REV>(g, p.row0, p.RG, sh.mask, sh.first, sh.last, sh.border);
-    float a[kRows][4], cc[kRows][4], q[kRows][4], d[kRows][4], s[4];
+    float a[kRows][4], cc[kRows][4], q[kRows][4], s[4];
+    Raw<T> xr, dr;
     load_tile<T, REV>(gate, ldg, p, __builtin_inff(), a);
-    ld_state(heads, tile * p.RG + p.rg, D, p.c, p.l.nrows > 0 ? p.l.nv : 0, s);
-    load_tile<T, REV>(x, ldx, p, 0.f, q);
-    if (dh) load_tile<T, REV>(dh, lddh, p, 0.f, d);
+    if (dh) load_tile<T, REV>(dh, lddh, p, dr);
     else
 #pragma unroll
         for (int i = 0; i < kRows; ++i)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) d[i][e] = 0.f;
+            for (int e = 0; e < 4; ++e) dr.v[i].v[e] = (T)0.f;
+    ld_state(heads, tile * p.RG + p.rg, D, p.c, p.l.nrows > 0 ? p.l.nv : 0, s);
+    load_tile<T, REV>(x, ldx, p, xr);
 #pragma unroll
     for (int i = 0; i < kRows; ++i)
 #pragma unroll
@@ -560,22 +607,18 @@ __global__ __launch_bounds__(kThreads) void k_scan_bwd(const T* __restrict__ x, 
     Map u{{1.f, 1.f, 1.f, 1.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
     for (int i = kRows - 1; i >= 0; --i) {
-        if (bit(w.wave_leave, i)) {
-            const bool seg = bit(w.m, 8 + i);
-            float ds[4];
-            ld_state(seg ? dlast : nullptr, seg ? sh.last[p.r0 + i] : 0, D, p.c, p.l.nv, ds);
+        float d[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                d[i][e] = bit(w.none, i) ? 0.f : d[i][e] + ds[e];
-                u.B[e] = bit(w.leave, i) ? 0.f : u.B[e];
-            }
-        }
+        for (int e = 0; e < 4; ++e) d[e] = dr.get(i, e);
+        if (bit(w.wave_leave, i)) leave_row(w, i, sh, p, dlast, D, d, u.B);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            u.B[e] = a[i][e] * (d[i][e] + u.B[e]);
+            u.B[e] = a[i][e] * (d[e] + u.B[e]);
             u.A[e] *= a[i][e];
         }
     }
+    settle(dr);
+    settle(xr);
 #pragma unroll
     for (int e = 0; e < 4; ++e) u.A[e] = w.leave ? -1.f : u.A[e];
     const Map all = border ? before_group<true, true>(u, CG, p.cg, sh.wm) : before_group<true, false>(u, CG, p.cg, sh.wm);
@@ -585,7 +628,7 @@ __global__ __launch_bounds__(kThreads) void k_scan_bwd(const T* __restrict__ x, 
         if (bit(w.wave_enter, i)) enter_row(w, i, sh, p, h0, D, s);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const float xi = q[i][e], hb = s[e];
+            const float xi = xr.get(i, e), hb = s[e];
             s[e] = fmaf(a[i][e], hb, cc[i][e] * xi);
             q[i][e] = (hb - xi) * (a[i][e] * cc[i][e]);
         }
@@ -593,12 +636,13 @@ __global__ __launch_bounds__(kThreads) void k_scan_bwd(const T* __restrict__ x, 
     answer(n_tiles, p, u, sh, s);
 #pragma unroll
     for (int i = kRows - 1; i >= 0; --i) {
-        if (bit(w.wave_leave, i))
+        float d[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s[e] = bit(w.leave, i) ? 0.f : s[e];
+        for (int e = 0; e < 4; ++e) d[e] = dr.get(i, e);
+        if (bit(w.wave_leave, i)) leave_row(w, i, sh, p, dlast, D, d, s);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const float lam = d[i][e] + s[e];
+            const float lam = d[e] + s[e];
             cc[i][e] *= lam;
             q[i][e] *= lam;
             s[e] = a[i][e] * lam;
