@@ -272,9 +272,9 @@ __device__ __forceinline__ Map before_group(Map& m, int CG, int cg, WaveMaps& w)
 }
 
 // ------------------------------------------------------------------------------------------------ from tile to tile
-// Tiles are taken in the order of the walk by a ticket, so whatever a tile waits for belongs to a workgroup that already
-// runs.  Every tile publishes its map, the last of 8 tiles their group's map, the last of 8 groups the STATE behind its 64
-// tiles: a tile reads at most 7 maps of tiles, 7 of groups and one state, and the only chain along the sequence has a link
+// The tiles of a column block are taken in the order of the walk by a ticket, so whatever a tile waits for belongs to a
+// workgroup that already runs (column blocks have nothing to do with each other).  Every tile publishes its map, the last of
+// 8 tiles their group's map, the last of 8 groups the STATE behind its 64 tiles: a tile reads at most 7 maps of tiles, 7 of groups and one state, and the only chain along the sequence has a link
 // per 64 tiles.  The products are always formed in this order, so the bits do not depend on who was first (a look-back
 // that takes the nearest state it finds would).  A word is its own flag: (A, B) travel as one 64-bit relaxed atomic,
 // B's bits never being kEmpty; no fences, no other memory is ordered by them.
@@ -318,8 +318,8 @@ __device__ __forceinline__ void await_words(const uint64_t* p, int n, uint64_t (
 
 // sIn[column] = the state that enters tile number `k` of the walk; own[0 / 1][column]: A / B of the tile's map.  The first
 // CG * 4 threads, one column each.  The tiles' words are asked for together and then the groups' (a look at another
-// workgroup's word takes about a microsecond; both at once measured the same and cost 14 registers), and all that can be composed is composed before the state is waited for: a link of the chain is one load,
-// one fma and one store.
+// workgroup's word takes about a microsecond; both at once measured the same and cost 14 registers), and all that can be
+// composed is composed before the state is waited for: a link of the chain is one load, one fma and one store.
 __device__ __forceinline__ void enter_tile(const Chain& ch, uint32_t k, uint32_t cb, const float* ownA, const float* ownB, float* sIn,
                                            uint32_t col) {
     const int p = (int)(k % kGroup), gp = (int)(k / kGroup % kGroup);
@@ -357,23 +357,33 @@ __device__ __forceinline__ void enter_tile(const Chain& ch, uint32_t k, uint32_t
 }
 
 // The next (tile, column block) in the order of the walk; with a single tile there is nothing to order.  false: none left
-// (a ticket that another call's workgroups also draw from).
+// (a ticket that another call's workgroups also draw from).  A counter answers about once in 17 ns, so workgroups that start
+// together wait for it: 1,024 of the forward pass for 17 us.  There the column blocks are dealt out to up to 8 counters, each
+// on a cache line of its own (16,384 x 2,048 bf16: 77 us with one, 62, 59 and 60 us with 2, 4 and 8; 262,144 x 512: 249, 241,
+// 240 and 238 us).  The backward pass starts half as many, waits longer for its rows, and loses more where the rows' column
+// blocks get out of step (16,384 x 2,048 fp32: 154 us with one counter, 164 us with 8; 1,048,576 x 128: 566 and 577 us).
+constexpr uint32_t kFwdTickets = 8, kBwdTickets = 1, kTicketStep = 32, kXcds = 8;
+template <uint32_t TICKETS>
 __device__ __forceinline__ bool take_tile(const Chain& ch, int64_t n_tiles, int64_t& tile, int& cb) {
     __shared__ uint32_t ticket;
-    uint32_t k = blockIdx.x;
-    const uint32_t ncb = gridDim.x / (uint32_t)n_tiles;
+    const uint32_t even = (uint32_t)n_tiles / kXcds * kXcds * ch.ncb;    // eight workgroups, one on every XCD, draw from a counter,
+    const uint32_t at = (blockIdx.x < even ? blockIdx.x / kXcds : blockIdx.x) % ch.ncb;   // so the counters stay in step
+    uint32_t k = blockIdx.x, set = 0, sets = 1;
     if (n_tiles > 1) {
-        if (threadIdx.x == 0) ticket = atomicAdd(ch.ticket, 1u);
+        sets = ch.ncb < TICKETS ? ch.ncb : TICKETS;
+        set = at % sets;
+        if (threadIdx.x == 0) ticket = atomicAdd(ch.ticket + set * kTicketStep, 1u);
         __syncthreads();
         k = __builtin_amdgcn_readfirstlane(ticket);                      // addresses of a tile are scalar arithmetic
     }
-    tile = k / ncb;
-    cb = (int)(k % ncb);
-    return k < gridDim.x;
+    const uint32_t size = (ch.ncb - set + sets - 1) / sets;              // column blocks set, set + sets, ..
+    tile = k / size;
+    cb = (int)(set + k % size * sets);
+    return k / size < (uint32_t)n_tiles;
 }
 
-__global__ __launch_bounds__(256) void k_scan_clear(uint4* p, int64_t n16, uint32_t* ticket) {
-    if (blockIdx.x == 0 && threadIdx.x == 0) *ticket = 0;
+__global__ __launch_bounds__(256) void k_scan_clear(uint4* p, int64_t n16, uint4* tickets, int64_t t16) {
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < t16; i += (int64_t)gridDim.x * 256) tickets[i] = make_uint4(0, 0, 0, 0);
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n16; i += (int64_t)gridDim.x * 256)
         p[i] = make_uint4(kEmpty, kEmpty, kEmpty, kEmpty);
 }
@@ -511,7 +521,7 @@ __global__ __launch_bounds__(kThreads, 4) void k_scan_fwd(const T* __restrict__ 
     __shared__ TileShared sh;
     int64_t tile;
     int cb;
-    if (!take_tile(ch, n_tiles, tile, cb)) return;
+    if (!take_tile<kFwdTickets>(ch, n_tiles, tile, cb)) return;
     const Place p = place<REV>(g, D, CG, tile, cb);
     if (threadIdx.x < 64) mark_tile<REV>(g, p.row0, p.RG, sh.mask, sh.first, sh.last, sh.border);
     float a[kRows][4], b[kRows][4];                                      // a row's map: s -> a s + b, b = c x
@@ -578,7 +588,7 @@ __global__ __launch_bounds__(kThreads) void k_scan_bwd(const T* __restrict__ x, 
     __shared__ TileShared sh;
     int64_t k;
     int cb;
-    if (!take_tile(ch, n_tiles, k, cb)) return;
+    if (!take_tile<kBwdTickets>(ch, n_tiles, k, cb)) return;
     const int64_t tile = n_tiles - 1 - k;
     const Place p = place<REV>(g, D, CG, tile, cb);
     if (threadIdx.x < 64) mark_tile<REV>(g, p.row0, p.RG, sh.mask, sh.first, sh.last, sh.border);
@@ -716,17 +726,18 @@ ScanWs scan_ws(int64_t n, int64_t D) {
     w.tile = take(8 * (t / kGroup + 1) * kGroup * lane);
     w.group = take(8 * blocks * kGroup * lane);
     w.state = take(4 * blocks * lane);
-    w.ticket = take(4);
+    w.ticket = take(4 * kTicketStep * kFwdTickets);
     w.bytes = at;
     return w;
 }
-// the words of `tiles` tiles emptied, the ticket at zero
+// the words of `tiles` tiles emptied, the tickets at zero
 Chain make_chain(void* ws, int64_t n, int64_t D, int64_t tiles, hipStream_t s) {
     const ScanWs w = scan_ws(n, D);
     char* base = static_cast<char*>(ws);
     const Chain ch{reinterpret_cast<uint64_t*>(base + w.tile), reinterpret_cast<uint64_t*>(base + w.group),
                    reinterpret_cast<uint32_t*>(base + w.state), reinterpret_cast<uint32_t*>(base + w.ticket), column_blocks(D)};
-    if (tiles > 1) k_scan_clear<<<bg_grid_for(w.ticket / 16, 256 * 4, 2048), 256, 0, s>>>(static_cast<uint4*>(ws), w.ticket / 16, ch.ticket);
+    if (tiles > 1) k_scan_clear<<<bg_grid_for(w.ticket / 16, 256 * 4, 2048), 256, 0, s>>>(static_cast<uint4*>(ws), w.ticket / 16,
+                                                                                            reinterpret_cast<uint4*>(ch.ticket), (w.bytes - w.ticket) / 16);
     return ch;
 }
 

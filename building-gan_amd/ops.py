@@ -992,7 +992,8 @@ class Embedding(torch.autograd.Function):
     @staticmethod
     def backward(ctx, g):
         (ids,) = ctx.saved_tensors
-        return EmbeddingGrad.apply(g, ids, ctx.n_rows, ctx.scale), None, None
+        grad = EmbeddingGrad.apply if torch.is_grad_enabled() else embedding_grad_raw    # grad mode: create_graph asked for it
+        return grad(g, ids, ctx.n_rows, ctx.scale), None, None
 
 
 class EmbeddingGrad(torch.autograd.Function):
