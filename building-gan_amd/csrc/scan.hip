@@ -21,7 +21,7 @@ namespace {
 constexpr int kRows = 8;
 constexpr int kThreads = 256, kWaves = kThreads / 64;
 constexpr int kMaxCols = 64;
-constexpr int kGroup = 8;                        // tiles of a group, groups of a block (see enter_tile)
+constexpr int kGroup = 8;                        // tiles of a group, groups of a block (see Chain)
 constexpr uint32_t kEmpty = 0xFFFFFFFFu;         // what unpublished words hold
 constexpr int kSpinLimit = 1 << 22;              // a wait of several seconds: only a workspace in use by another call gets there
 
@@ -274,10 +274,11 @@ __device__ __forceinline__ Map before_group(Map& m, int CG, int cg, WaveMaps& w)
 // ------------------------------------------------------------------------------------------------ from tile to tile
 // The tiles of a column block are taken in the order of the walk by a ticket, so whatever a tile waits for belongs to a
 // workgroup that already runs (column blocks have nothing to do with each other).  Every tile publishes its map, the last of
-// 8 tiles their group's map, the last of 8 groups the STATE behind its 64 tiles: a tile reads at most 7 maps of tiles, 7 of groups and one state, and the only chain along the sequence has a link
-// per 64 tiles.  The products are always formed in this order, so the bits do not depend on who was first (a look-back
-// that takes the nearest state it finds would).  A word is its own flag: (A, B) travel as one 64-bit relaxed atomic,
-// B's bits never being kEmpty; no fences, no other memory is ordered by them.
+// 8 tiles their group's map, the last of 8 groups the STATE behind its 64 tiles: a tile reads at most 7 maps of tiles, 7 of
+// groups and one state, and the only chain along the sequence has a link per 64 tiles.  The products are always formed in
+// this order, so the bits do not depend on who was first (a look-back that takes the nearest state it finds would).  A word
+// is its own flag: (A, B) travel as one 64-bit relaxed atomic, B's bits never being kEmpty; no fences, no other memory is
+// ordered by them.
 struct Chain {                       // for every column block: tile[group][8][64], group[block][8][64], state[block][64]
     uint64_t *tile, *group;
     uint32_t *state, *ticket, ncb;
@@ -299,69 +300,67 @@ __device__ __forceinline__ void then_words(float& A, float& B, const uint64_t (&
             A = A2 < 0.f || A < 0.f ? -1.f : A2 * A;
         }
 }
-// The words of a group lie side by side, so seven of them are one address and seven constants; those of tiles that are not
-// asked for are loaded and left alone.
-__device__ __forceinline__ void peek_words(const uint64_t* p, uint64_t (&v)[kGroup - 1]) {
-#pragma unroll
-    for (int i = 0; i < kGroup - 1; ++i) v[i] = peek(p + i * kMaxCols);
-}
+// The first n words of a group, side by side, each asked for until it is there and with a pause between: asking for all
+// seven again and again takes from the rows' share of the memory (1,048,576 x 128 fp32 forward 350 us, with this 333 us).
 __device__ __forceinline__ void await_words(const uint64_t* p, int n, uint64_t (&v)[kGroup - 1]) {
+#pragma unroll
+    for (int i = 0; i < kGroup - 1; ++i) v[i] = (uint64_t)kEmpty << 32;
 #pragma unroll 1
     for (int k = 0; k < kSpinLimit; ++k) {
         bool wait = false;
 #pragma unroll
+        for (int i = 0; i < kGroup - 1; ++i)
+            if (i < n && __any(is_empty(v[i]))) v[i] = peek(p + i * kMaxCols);
+#pragma unroll
         for (int i = 0; i < kGroup - 1; ++i) wait |= i < n && is_empty(v[i]);
         if (!__any(wait)) break;
-        peek_words(p, v);
+        __builtin_amdgcn_s_sleep(4);
     }
 }
 
-// sIn[column] = the state that enters tile number `k` of the walk; own[0 / 1][column]: A / B of the tile's map.  The first
-// CG * 4 threads, one column each.  The tiles' words are asked for together and then the groups' (a look at another
-// workgroup's word takes about a microsecond; both at once measured the same and cost 14 registers), and all that can be
-// composed is composed before the state is waited for: a link of the chain is one load, one fma and one store.
-__device__ __forceinline__ void enter_tile(const Chain& ch, uint32_t k, uint32_t cb, const float* ownA, const float* ownB, float* sIn,
-                                           uint32_t col) {
+// What enters tile number `k` of the walk, by two waves at once, a lane for each column (a look at another workgroup's word
+// takes about a microsecond, and the two levels would be two looks after one another: 16,384 x 2,048 bf16 backward 120 us, with
+// two waves 115 us).  The first wave publishes the tile's map (ownA, ownB) and composes the maps of its group's tiles before it ..
+__device__ __forceinline__ void enter_group(const Chain& ch, uint32_t k, uint32_t cb, uint32_t col, float oA, float oB, float& A, float& B) {
     const int p = (int)(k % kGroup), gp = (int)(k / kGroup % kGroup);
-    const uint32_t group = k / kGroup, block = group / kGroup;
-    uint64_t *tiles = ch.tile + ((int64_t)group * ch.ncb + cb) * (kGroup * kMaxCols) + col;
-    uint64_t *groups = ch.group + ((int64_t)block * ch.ncb + cb) * (kGroup * kMaxCols) + col;
-    uint32_t* state = ch.state + ((int64_t)block * ch.ncb + cb) * kMaxCols + col;
-    const uint32_t* before = state - (block > 0 ? (int64_t)ch.ncb * kMaxCols : 0);
-    const float oA = ownA[col], oB = ownB[col];
+    uint64_t *tiles = ch.tile + ((int64_t)(k / kGroup) * ch.ncb + cb) * (kGroup * kMaxCols) + col;
+    A = 1.f;
+    B = 0.f;
     if (p < kGroup - 1) publish(tiles + p * kMaxCols, oA, oB);
-    uint64_t v[kGroup - 1];
-    uint32_t w = __hip_atomic_load(before, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    peek_words(tiles, v);
-    float A = 1.f, B = 0.f;                                              // of the group's tiles before this one
-    await_words(tiles, p, v);
-    then_words(A, B, v, p);
+    if (p > 0) {
+        uint64_t v[kGroup - 1];
+        await_words(tiles, p, v);
+        then_words(A, B, v, p);
+    }
     if (p == kGroup - 1 && gp < kGroup - 1)
-        publish(groups + gp * kMaxCols, A < 0.f || oA < 0.f ? -1.f : oA * A, apply(oA, oB, B));
-    float gA = 1.f, gB = 0.f;                                            // of the block's groups before this one
-    peek_words(groups, v);
-    await_words(groups, gp, v);
-    then_words(gA, gB, v, gp);
-    B = apply(A, B, gB);
-    A = A < 0.f || gA < 0.f ? -1.f : A * gA;
-    if (block > 0 && !__all(A < 0.f))                                        // behind a cut the state from further back is not needed
+        publish(ch.group + ((int64_t)(k / (kGroup * kGroup)) * ch.ncb + cb) * (kGroup * kMaxCols) + gp * kMaxCols + col,
+                A < 0.f || oA < 0.f ? -1.f : oA * A, apply(oA, oB, B));
+}
+// .. and the second one finds the state behind the block's groups before that.
+__device__ __forceinline__ float enter_block(const Chain& ch, uint32_t k, uint32_t cb, uint32_t col) {
+    const int gp = (int)(k / kGroup % kGroup);
+    const uint32_t block = k / (kGroup * kGroup);
+    const uint64_t *groups = ch.group + ((int64_t)block * ch.ncb + cb) * (kGroup * kMaxCols) + col;
+    const uint32_t* before = ch.state + ((int64_t)(block - (block > 0)) * ch.ncb + cb) * kMaxCols + col;
+    uint32_t w = block > 0 ? __hip_atomic_load(before, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0u;
+    float A = 1.f, B = 0.f;
+    if (gp > 0) {
+        uint64_t v[kGroup - 1];
+        await_words(groups, gp, v);
+        then_words(A, B, v, gp);
+    }
+    if (!__all(A < 0.f))                                                 // behind a cut the state from further back is not needed
 #pragma unroll 1
         for (int i = 0; i < kSpinLimit && __any(w == kEmpty); ++i) w = __hip_atomic_load(before, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    const float s = apply(A, B, block > 0 ? __uint_as_float(w) : 0.f);
-    if (p == kGroup - 1 && gp == kGroup - 1) {
-        uint32_t b = __float_as_uint(apply(oA, oB, s));
-        if (b == kEmpty) b = 0x7FC00000u;
-        __hip_atomic_store(state, b, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    }
-    sIn[col] = s;
+    return apply(A, B, __uint_as_float(w));
 }
 
 // The next (tile, column block) in the order of the walk; with a single tile there is nothing to order.  false: none left
 // (a ticket that another call's workgroups also draw from).  A counter answers about once in 17 ns, so workgroups that start
 // together wait for it: 1,024 of the forward pass for 17 us.  There the column blocks are dealt out to up to 8 counters, each
-// on a cache line of its own (16,384 x 2,048 bf16: 77 us with one, 62, 59 and 60 us with 2, 4 and 8; 262,144 x 512: 249, 241,
-// 240 and 238 us).  The backward pass starts half as many, waits longer for its rows, and loses more where the rows' column
-// blocks get out of step (16,384 x 2,048 fp32: 154 us with one counter, 164 us with 8; 1,048,576 x 128: 566 and 577 us).
+// on a cache line of its own (16,384 x 2,048 bf16: 58 us, 74 us with one counter; 262,144 x 512 bf16: 235 and 246 us).  The
+// backward pass starts half as many, waits longer for its rows, and loses more where the column blocks of a row get out of
+// step (1,048,576 x 128 fp32: 562 us with one counter, 577 us with 2 and with 8; 16,384 x 2,048 fp32: 149, 149 and 155 us).
 constexpr uint32_t kFwdTickets = 8, kBwdTickets = 1, kTicketStep = 32, kXcds = 8;
 template <uint32_t TICKETS>
 __device__ __forceinline__ bool take_tile(const Chain& ch, int64_t n_tiles, int64_t& tile, int& cb) {
@@ -402,7 +401,7 @@ struct TileShared {
     uint32_t mask[kThreads / 4];
     int32_t border;
     WaveMaps wm;
-    float4 own[2][kMaxCols / 4], in[kMaxCols / 4];
+    float4 own[2][kMaxCols / 4], near[2][kMaxCols / 4], far[kMaxCols / 4];
 };
 
 // Where a thread stands: rows r0 .. of tile `tile`, four columns from c on
@@ -435,7 +434,7 @@ __device__ __forceinline__ void store_tile(T* __restrict__ m, int64_t ld, const 
 }
 
 // The state before this thread's row group, `pre` being the map of the tile's groups before it: through the chain, unless the
-// walk is a single tile.  What stands between `ask` and `answer` is done by the other waves while the first one waits.
+// walk is a single tile.  What stands between `ask` and `answer` is done by the other waves while the first two wait.
 __device__ __forceinline__ void ask(const Chain& ch, int64_t k, int64_t n_tiles, int64_t D, int CG, const Place& p, bool last_group,
                                     const Map& all, TileShared& sh) {
     if (n_tiles == 1) return;
@@ -444,28 +443,45 @@ __device__ __forceinline__ void ask(const Chain& ch, int64_t k, int64_t n_tiles,
         sh.own[1][p.cg] = make_float4(all.B[0], all.B[1], all.B[2], all.B[3]);
     }
     __syncthreads();
-    if ((int)threadIdx.x < CG * 4 && p.c0 + threadIdx.x < D)
-        enter_tile(ch, (uint32_t)k, (uint32_t)p.cb, &sh.own[0][0].x, &sh.own[1][0].x, &sh.in[0].x, threadIdx.x);
+    const uint32_t col = threadIdx.x & 63;
+    if (threadIdx.x < 128 && (int)col < CG * 4 && p.c0 + col < D) {
+        if (threadIdx.x < 64) {
+            float A, B;
+            enter_group(ch, (uint32_t)k, (uint32_t)p.cb, col, (&sh.own[0][0].x)[col], (&sh.own[1][0].x)[col], A, B);
+            (&sh.near[0][0].x)[col] = A;
+            (&sh.near[1][0].x)[col] = B;
+        } else
+            (&sh.far[0].x)[col] = enter_block(ch, (uint32_t)k, (uint32_t)p.cb, col);
+    }
 }
-__device__ __forceinline__ void answer(int64_t n_tiles, const Place& p, const Map& pre, const TileShared& sh, float (&s)[4]) {
+__device__ __forceinline__ void answer(const Chain& ch, int64_t k, int64_t n_tiles, int64_t D, int CG, const Place& p, const Map& pre,
+                                       const TileShared& sh, float (&s)[4]) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) s[e] = 0.f;
     if (n_tiles > 1) {
         __syncthreads();
-        const float4 v = sh.in[p.cg];
-        s[0] = v.x; s[1] = v.y; s[2] = v.z; s[3] = v.w;
+        const uint32_t col = threadIdx.x;
+        if (k % (kGroup * kGroup) == kGroup * kGroup - 1 && (int)col < CG * 4 && p.c0 + col < D) {   // the state behind the block
+            uint32_t b = __float_as_uint(apply((&sh.own[0][0].x)[col], (&sh.own[1][0].x)[col],
+                                               apply((&sh.near[0][0].x)[col], (&sh.near[1][0].x)[col], (&sh.far[0].x)[col])));
+            if (b == kEmpty) b = 0x7FC00000u;
+            __hip_atomic_store(ch.state + ((int64_t)(k / (kGroup * kGroup)) * ch.ncb + p.cb) * kMaxCols + col, b, __ATOMIC_RELAXED,
+                               __HIP_MEMORY_SCOPE_AGENT);
+        }
+        const float4 A = sh.near[0][p.cg], B = sh.near[1][p.cg], v = sh.far[p.cg];
+        s[0] = apply(A.x, B.x, v.x); s[1] = apply(A.y, B.y, v.y); s[2] = apply(A.z, B.z, v.z); s[3] = apply(A.w, B.w, v.w);
     }
 #pragma unroll
     for (int e = 0; e < 4; ++e) s[e] = apply(pre.A[e], pre.B[e], s[e]);
 }
 
-// to[s] = from[s] (or 0) for the segments without rows, dealt out to the tiles
+// to[s] = from[s] (or 0) for the segments without rows, dealt out to the tiles' row groups
 template <bool REV>
 __device__ __forceinline__ void pass_through(const Segs& g, int64_t D, int64_t tile, int64_t n_tiles, const Place& p,
                                              const float* __restrict__ from, float* __restrict__ to) {
-    if (!to || p.rg != 0) return;
-    for (int64_t j = tile; j < g.S; j += n_tiles)
-        if (seg_lo<REV, true>(g, j) >= seg_lo<REV, true>(g, j + 1)) {
+    if (!to) return;
+    for (int64_t j = tile * p.RG + p.rg; j < g.S; j += n_tiles * p.RG)
+        if (seg_lo<REV>(g, j) >= seg_lo<REV>(g, j + 1)) {
             const int64_t s = REV ? g.S - 1 - j : j;
             float v[4];
             ld_state(from, s, D, p.c, p.l.nv, v);
@@ -562,7 +578,7 @@ __global__ __launch_bounds__(kThreads, 4) void k_scan_fwd(const T* __restrict__ 
     const Map all = border ? before_group<false, true>(f, CG, p.cg, sh.wm) : before_group<false, false>(f, CG, p.cg, sh.wm);
     float s[4];
     ask(ch, tile, n_tiles, D, CG, p, p.rg == p.RG - 1, all, sh);
-    answer(n_tiles, p, f, sh, s);
+    answer(ch, tile, n_tiles, D, CG, p, f, sh, s);
     if (heads && p.l.nrows > 0) st_state(heads, tile * p.RG + p.rg, D, p.c, p.l.nv, s);
 #pragma unroll
     for (int i = 0; i < kRows; ++i) {
@@ -643,7 +659,7 @@ __global__ __launch_bounds__(kThreads) void k_scan_bwd(const T* __restrict__ x, 
             q[i][e] = (hb - xi) * (a[i][e] * cc[i][e]);
         }
     }
-    answer(n_tiles, p, u, sh, s);
+    answer(ch, k, n_tiles, D, CG, p, u, sh, s);
 #pragma unroll
     for (int i = kRows - 1; i >= 0; --i) {
         float d[4];
