@@ -1011,8 +1011,8 @@ class EmbeddingGrad(torch.autograd.Function):
 
 def embedding(weight: torch.Tensor, ids: torch.Tensor, scale: float = 1.0, validate: bool = False) -> torch.Tensor:
     """Rows of a learned table: ``scale * weight[ids]``, shape [*ids.shape, D], in the table's type (float32, float16,
-    bfloat16; int64 or int32 ids).  A categorical node feature (program class, floor level) as a vector without the
-    one-hot matrix of Model/models.py:84; its gradient sums each row's terms in fp32 in a fixed order.
+    bfloat16; int64 or int32 ids).  A categorical node feature (program class, floor level) as a vector without its
+    one-hot matrix; the gradient sums each row's terms in fp32 in a fixed order.
 
     An id outside [0, V) is a missing token: a zero row that takes no part in the gradient.  ``validate=True`` reads the
     ids back (one synchronisation) and raises IndexError on any id outside [0, V) instead."""
@@ -1143,7 +1143,9 @@ def gated_scan(x: torch.Tensor, gate: torch.Tensor, rowptr: Optional[torch.Tenso
     segment of all rows without it; or [B, T, D], B segments of T rows.  ``h0`` [S, D] float32 is the state before a
     segment's first row (default zero), ``h_last`` [S, D] float32 the one after its last; a segment without rows passes
     its state through.  Rows in no segment are zero in ``h`` and in the gradients.  ``reverse`` walks every segment from
-    its last row to its first.  The state is carried in fp32 and ``h`` rounded once; results are bit-reproducible."""
+    its last row to its first.  The state is carried in fp32 and ``h`` rounded once; results are bit-reproducible.  What is
+    not finite stays in its segment and column; there an infinite state may come out as a NaN some rows on (the rows' maps
+    are composed, and a long product of a's is 0)."""
     shape = x.shape
     if x.dim() == 3:
         if rowptr is not None:
@@ -1162,12 +1164,18 @@ def gated_scan(x: torch.Tensor, gate: torch.Tensor, rowptr: Optional[torch.Tenso
     return (h if h.shape == shape else h.view(shape)), h_last
 
 
-def _shifted_overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
-    """Whether two float32 matrices overlap in memory without holding every element at the same address."""
-    if a.numel() == 0 or (a.data_ptr() == b.data_ptr() and a.stride() == b.stride()):
+def _shifted_overlap(out: torch.Tensor, t: torch.Tensor) -> bool:
+    """Whether two [n, D] matrices of contiguous rows share memory without holding every element at the same address."""
+    eo, et = out.element_size(), t.element_size()
+    if out.numel() == 0 or (out.data_ptr() == t.data_ptr() and out.stride() == t.stride() and eo == et):
         return False
-    lo, hi = zip(*((t.data_ptr(), t.data_ptr() + 4 * sum((n - 1) * s for n, s in zip(t.shape, t.stride()))) for t in (a, b)))
-    return lo[0] <= hi[1] and lo[1] <= hi[0]
+    (n, D), a, b = out.shape, out.data_ptr(), t.data_ptr()
+    po, pt = eo * (out.stride(0) if n > 1 else D), et * (t.stride(0) if n > 1 else D)
+    if a >= b + pt * (n - 1) + et * D or b >= a + po * (n - 1) + eo * D:
+        return False
+    if po != pt:
+        return True
+    return (b - a) % po < eo * D or (a - b) % po < et * D                   # else: column ranges of one buffer, side by side
 
 
 def gated_scan_step(x: torch.Tensor, gate: torch.Tensor, state: torch.Tensor, state_out: Optional[torch.Tensor] = None):
@@ -1192,8 +1200,8 @@ def gated_scan_step(x: torch.Tensor, gate: torch.Tensor, state: torch.Tensor, st
     elif (state_out.shape != x.shape or state_out.dtype != torch.float32 or state_out.device != x.device
           or _rows(state_out) is not state_out):
         raise _lib.BganError(f"gated_scan_step: state_out must be float32 {tuple(x.shape)} with contiguous rows on {x.device}")
-    elif _shifted_overlap(state_out, state):
-        raise _lib.BganError("gated_scan_step: state_out shares memory with state without being the same rows")
+    elif any(_shifted_overlap(state_out, t) for t in (state, x, gate)):
+        raise _lib.BganError("gated_scan_step: state_out shares memory with an operand without being the same rows")
     check(lib.bg_gated_scan_step(code, x.data_ptr(), _ld(x), gate.data_ptr(), _ld(gate), state.data_ptr(), _ld(state), n, D, h.data_ptr(),
                                  max(D, 1), state_out.data_ptr(), _ld(state_out), stream()), "bg_gated_scan_step")
     return h, state_out

@@ -127,18 +127,19 @@ int bg_plan_build(const bgPlanIn* in, int32_t* arena_i32, float* arena_f32, bgSt
 
 /* out[i,:] = scale * weight[ids[i],:] for a table weight[V, D] of `dtype` (row pitches in elements); ids are int64
  * (ids_is_64 != 0) or int32.  An id outside [0, V) is a missing token: its row of `out` is zero.  One fp32 product and
- * one rounding per element.  Rows are moved in pieces of 16 bytes whatever their alignment.  D <= 2^15, n * D <= 2^33 (BG_ERR_SHAPE).
- * replaces: one-hot x Linear over a categorical node feature and the position table's gather, Model/models.py:25,84. */
+ * one rounding per element.  Rows are moved in pieces of 16 bytes whatever their alignment.
+ * D <= 2^15, pieces of 16 bytes in `out` <= 2^33 (BG_ERR_SHAPE).
+ * replaces: nothing in the reference, which multiplies one-hot features with a weight.                              */
 int bg_embedding_fwd(int dtype, const void* weight, int64_t ldw, int64_t V, const void* ids, int ids_is_64, int64_t n, int64_t D,
                      float scale, void* out, int64_t ldo, bgStream stream);
 
 /* The lookup's gradient: dw[v,:] = scale * sum over ids[i] == v of g[i,:], every row of dw[V, D] (contiguous, 16-byte
- * aligned) written, zero where a token does not occur.  Tokens are sorted (stable; tables of up to 16 rows are summed without a sort) and
- * every row's terms are summed in fp32 in an order that depends on the sizes and ids only, with no floating-point atomics:
- * equal inputs give equal bits.
+ * aligned) written, zero where a token does not occur.  Tokens are sorted (stable; tables of up to 20
+ * rows are summed without a sort) and every row's terms are summed in fp32 in an order that depends on the sizes and ids
+ * only, with no floating-point atomics: equal inputs give equal bits.
  * n <= 2^30, V < 2^31 - 1, D <= 2^15 (BG_ERR_SHAPE).  ws: bg_embedding_bwd_workspace(...) bytes, 16-byte aligned
- * (BG_ERR_SCRATCH when ws_bytes is less); its contents need no preparation.
- * replaces: the weight gradient of the Linear over a one-hot feature, Model/models.py:84 under autograd.            */
+ * (BG_ERR_SCRATCH when ws_bytes is less); its contents need no preparation, and no two calls at once may have the same.
+ * replaces: nothing in the reference (see bg_embedding_fwd).                                                        */
 int64_t bg_embedding_bwd_workspace(int dtype, int64_t n, int64_t V, int64_t D);
 int bg_embedding_bwd(int dtype, const void* g, int64_t ldg, const void* ids, int ids_is_64, int64_t n, int64_t D, int64_t V,
                      float scale, void* dw, void* ws, int64_t ws_bytes, bgStream stream);
@@ -154,8 +155,9 @@ int bg_embedding_bwd(int dtype, const void* g, int64_t ldg, const void* ids, int
  * the nearer end.  rowptr NULL: n_seg segments of n_rows / n_seg rows each.  The state is fp32; h is rounded once.
  * heads (may be NULL): fp32 [bg_gated_scan_heads(n_rows, D)], the state before every eighth row, which the
  * backward pass takes.  ws: bg_gated_scan_workspace(n_rows, D) bytes, 16-byte aligned (BG_ERR_SCRATCH when ws_bytes is
- * less); it needs no preparation.  x, gate and h in pieces of four elements where D, the pitches and the addresses allow.
- * n_rows < 2^31, D <= 2^20 (BG_ERR_SHAPE).  Equal inputs give equal bits.
+ * less); it needs no preparation, and no two calls at once may have the same.  Any alignment and pitch of x, gate and h
+ * is read and written in pieces of four elements.  n_rows < 2^31, D <= 2^20, n_rows * D (D rounded up to 16, 32 or a
+ * multiple of 64) < 2^37, pitches <= 2^21 (BG_ERR_SHAPE).  Equal inputs give equal bits.  Outputs overlap nothing.
  * replaces: nothing in the reference, whose only state along a building is the floor level of Model/models.py:22-25.    */
 int64_t bg_gated_scan_heads(int64_t n_rows, int64_t D);
 int64_t bg_gated_scan_workspace(int64_t n_rows, int64_t D);
@@ -173,7 +175,9 @@ int bg_gated_scan_bwd(int dtype, const void* x, int64_t ldx, const void* gate, i
                       int64_t ws_bytes, bgStream stream);
 
 /* One row for each of n segments whose states are kept: state_out = a state + (1 - a) x, h = state_out in `dtype`.
- * state, state_out: fp32 [n, D] with row pitches; state_out may be state.                                            */
+ * state, state_out: fp32 [n, D] with row pitches; state_out may be state (the same rows), and overlaps nothing else.
+ * D <= 2^20, n < 2^24 (BG_ERR_SHAPE).
+ * replaces: nothing in the reference.                                                                                */
 int bg_gated_scan_step(int dtype, const void* x, int64_t ldx, const void* gate, int64_t ldg, const float* state, int64_t lds, int64_t n,
                        int64_t D, void* h, int64_t ldh, float* state_out, int64_t ldso, bgStream stream);
 

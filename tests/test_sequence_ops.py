@@ -612,3 +612,156 @@ def test_on_another_stream_and_two_calls_at_once(cuda):
             outs.append((ops.gated_scan(x, gate, ptr)[0], ops.embedding_grad_raw(x, ids, 50)))
     torch.cuda.synchronize()
     assert all(torch.equal(a, want) and torch.equal(b, want_w) for a, b in outs)
+
+
+# ------------------------------------------------------------------------------------------------ further sizes and calls
+def test_pitches_past_32_bits_of_a_tile_are_refused():
+    from building_gan_amd import _lib
+    lib = _lib.load()
+    p, far = 1 << 20, (1 << 21) + 1
+    size = lib.bg_gated_scan_workspace(10, 8)
+    fwd = lambda ldx, ldg, ldh: lib.bg_gated_scan_fwd(0, p, ldx, p, ldg, p, 2, 10, 8, None, 0, p, ldh, p, None, p, size, None)
+    assert fwd(far, 8, 8) == -2 and fwd(8, far, 8) == -2 and fwd(8, 8, far) == -2
+    bwd = lambda ldx, ldg, lddh, lddx, lddg: lib.bg_gated_scan_bwd(0, p, ldx, p, ldg, p, lddh, None, p, 2, 10, 8, None, 0, p, p, lddx, p, lddg,
+                                                                   None, p, size, None)
+    for k in range(5):
+        assert bwd(*[far if i == k else 8 for i in range(5)]) == -2
+
+
+def test_overlap_of_a_step_s_states():
+    """Side by side in one buffer or the same rows: taken; anything else that shares memory: refused."""
+    from building_gan_amd.ops import _shifted_overlap
+    buf = torch.zeros(6, 24)
+    a, b = buf[:, :12], buf[:, 12:]
+    assert not _shifted_overlap(a, b) and not _shifted_overlap(b, a) and not _shifted_overlap(a, a)
+    assert _shifted_overlap(buf[:, :13], buf[:, 11:24]) and _shifted_overlap(a[:4], a[1:5]) and _shifted_overlap(buf[:, 4:16], buf[:, :12])
+    assert not _shifted_overlap(buf[:3], buf[3:]) and not _shifted_overlap(a, torch.zeros(6, 12))
+    assert _shifted_overlap(buf[:1, :12], buf[:1, 6:18]) and not _shifted_overlap(buf[:1, :12], buf[:1, 12:])
+    assert _shifted_overlap(a, buf.view(torch.float16)[:, :12])
+
+
+@pytest.mark.gpu
+def test_step_into_another_half_of_the_same_buffer(cuda):
+    from building_gan_amd import _lib, ops
+    buf, x = torch.randn(7, 64, device=cuda), torch.randn(7, 32, device=cuda)
+    want = ops.gated_scan_step(x, x, buf[:, :32].contiguous())[1]
+    keep = buf[:, :32].clone()
+    ops.gated_scan_step(x, x, buf[:, :32], state_out=buf[:, 32:])
+    assert torch.equal(buf[:, 32:], want) and torch.equal(buf[:, :32], keep)
+    with pytest.raises(_lib.BganError):
+        ops.gated_scan_step(x, x, buf[:, :32], state_out=buf[:, 16:48])
+    with pytest.raises(_lib.BganError):
+        ops.gated_scan_step(buf[:6, :32], x[:6], x[:6], state_out=buf[1:, :32])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("V,D,n,kind", [(7, 3, 5000, "uniform"), (20, 1, 999, "hot"), (5, 2, 70000, "missing"), (20, 132, 4097, "missing"),
+                                        (21, 132, 4097, "missing"), (5000, 16, 4096, "uniform"), (5000, 16, 4097, "hot"),
+                                        (900, 24, 8192, "uniform"), (900, 24, 8193, "missing"), (600, 2, 30000, "uniform")])
+def test_lookup_at_the_borders_of_its_variants(cuda, V, D, n, kind):
+    """Tables of a few rows with rows of less than a piece, and the token counts where the sort changes."""
+    for dtype in (torch.float32, torch.bfloat16):
+        w, ids, g = lookup_case(V, D, n, dtype, V * n + D, kind)
+        check_lookup(cuda, w, ids, g, 0.5)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("reverse,dtype,ptr", [(False, torch.float32, [0, 16900]), (True, torch.float32, [0, 8200, 16900]),
+                                               (False, torch.bfloat16, [0, 9000, 9001, 16900]), (True, torch.float16, [3, 16800])])
+def test_scan_over_several_blocks_of_tiles(cuda, reverse, dtype, ptr):
+    """More than 2 x 64 tiles of 128 rows: states handed from block to block, with and without a border in between."""
+    c = scan_case(16900, 36, ptr, dtype, 21, slow=True)
+    check_scan(cuda, c, ptr, reverse)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("reverse", [False, True])
+def test_scan_of_many_segments_without_rows(cuda, reverse):
+    """Their states pass through, in both directions, whatever the number of tiles."""
+    from building_gan_amd import ops
+    gen = torch.Generator().manual_seed(4)
+    S, N = 20000, 700
+    cuts = torch.randint(0, N + 1, (S - 1,), generator=gen).sort().values.tolist()
+    ptr = torch.tensor([0] + cuts + [N], dtype=torch.int32)
+    x, gate, h0 = torch.randn(N, 20, generator=gen), torch.randn(N, 20, generator=gen), torch.randn(S, 20, generator=gen)
+    xs, gs, hs = (t.to(cuda).requires_grad_(True) for t in (x, gate, h0))
+    h, hl = ops.gated_scan(xs, gs, ptr.to(cuda), hs, reverse)
+    dl = torch.randn(S, 20, generator=gen)
+    (d0,) = torch.autograd.grad(hl, hs, dl.to(cuda))
+    none = (ptr[1:] == ptr[:-1])
+    assert int(none.sum()) > S - N - 1
+    assert torch.equal(hl.cpu()[none], h0[none]) and torch.equal(d0.cpu()[none], dl[none])
+    some = torch.nonzero(~none).flatten().tolist()
+    short = [int(ptr[s]) for s in some] + [N]
+    h2, hl2 = ops.gated_scan(x.to(cuda), gate.to(cuda), torch.tensor(short, dtype=torch.int32, device=cuda), h0[some].to(cuda), reverse)
+    assert torch.equal(h, h2) and torch.equal(hl[some], hl2)
+
+
+@pytest.mark.gpu
+def test_rows_past_2_31_elements(cuda):
+    """The last rows of 2^31 and more elements (bf16, 4.3 GB a matrix): the same bits as a call on those rows alone."""
+    from building_gan_amd import ops
+    D, N0, n = 2048, 1 << 20, 300
+    N = N0 + n
+    gen = torch.Generator(device=cuda).manual_seed(6)
+    x = torch.randn(N, D, generator=gen, device=cuda, dtype=torch.bfloat16)
+    gate = torch.randn(N, D, generator=gen, device=cuda, dtype=torch.bfloat16)
+    dh = torch.randn(N, D, generator=gen, device=cuda, dtype=torch.bfloat16)
+    ptr = torch.tensor([0, N0, N], dtype=torch.int32, device=cuda)           # N0 is a border of 64 tiles: joined alike
+    h, hl, heads = ops.gated_scan_raw(x, gate, ptr, None, False, keep_heads=True)
+    own, ownl, own_heads = ops.gated_scan_raw(x[N0:], gate[N0:], 1, None, False, keep_heads=True)
+    assert torch.equal(h[N0:], own) and torch.equal(hl[1:], ownl)
+    dx, dg, _ = ops.gated_scan_grad_raw(x, gate, ptr, None, False, heads, dh, None, False)
+    odx, odg, _ = ops.gated_scan_grad_raw(x[N0:], gate[N0:], 1, None, False, own_heads, dh[N0:], None, False)
+    assert torch.equal(dx[N0:], odx) and torch.equal(dg[N0:], odg)
+    del h, heads, dx, dg, gate, dh
+    ids = torch.randint(0, 50, (N,), generator=gen, device=cuda)
+    w = torch.randn(50, D, generator=gen, device=cuda, dtype=torch.bfloat16)
+    out = ops.embedding(w, ids)                                              # (stored around the caches)
+    assert torch.equal(out[N0:], w[ids[N0:]]) and torch.equal(out[:n], w[ids[:n]])
+    del out
+    ids[:N0] = -1
+    g = x.sign()                                                             # sums of +-1: exact in any order
+    want = torch.zeros(50, D, device=cuda).index_add_(0, ids[N0:], g[N0:].float())
+    assert torch.equal(ops.embedding_grad_raw(g, ids, 50).float(), want)
+    assert torch.equal(ops.embedding_grad_raw(g[:, :24], ids % 7 - (ids < 0).long() * 9, 20)[:7].float(),
+                       torch.zeros(7, 24, device=cuda).index_add_(0, ids[N0:] % 7, g[N0:, :24].float()))
+
+
+@pytest.mark.gpu
+def test_autograd_captured_and_replayed(cuda):
+    """A step of training, forward and backward through autograd, captured once and replayed on changing inputs."""
+    from building_gan_amd import ops
+    B, T, V, D = 3, 150, 40, 48
+    gen = torch.Generator(device=cuda).manual_seed(1)
+    w = torch.randn(V, 2 * D, generator=gen, device=cuda).requires_grad_(True)
+    h0 = torch.randn(B, D, generator=gen, device=cuda).requires_grad_(True)
+    ids = torch.zeros(B, T, dtype=torch.int64, device=cuda)
+    cot = torch.zeros(B, T, D, device=cuda)
+
+    def step():
+        z = ops.embedding(w, ids, 0.5)
+        h, hl = ops.gated_scan(z[..., :D], z[..., D:], h0=h0, reverse=True)
+        grads = torch.autograd.grad((h, hl), (w, h0), (cot, h0.detach()))
+        return (h.detach(), hl.detach()) + grads             # (no graph of these leaves lives on)
+
+    def fill():
+        ids.copy_(torch.randint(-1, V, (B, T), generator=gen, device=cuda))
+        cot.copy_(torch.randn(B, T, D, generator=gen, device=cuda))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = step()
+    for k in range(4):
+        fill()
+        graph.replay()
+        if k % 2:
+            torch.cuda.synchronize()
+        got = [t.clone() for t in outs]
+        for i, (a, b) in enumerate(zip(got, step())):
+            assert torch.equal(a, b), (k, i)
