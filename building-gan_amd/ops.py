@@ -970,12 +970,22 @@ def embedding_grad_raw(g: torch.Tensor, ids: torch.Tensor, n_rows: int, scale: f
         raise _lib.BganError(f"embedding_grad: rows {tuple(g.shape)} do not belong to ids {tuple(ids.shape)}")
     if n_rows < 0:
         raise _lib.BganError("embedding_grad: n_rows must not be negative")
-    n, D = i.numel(), g.shape[-1]
+    return _embedding_backward(code, g, i, n_rows, scale)
+
+
+@functools.lru_cache(maxsize=1024)
+def _embedding_grad_size(code: int, n: int, n_rows: int, D: int) -> int:
+    return _lib.load().bg_embedding_bwd_workspace(code, n, n_rows, D)
+
+
+def _embedding_backward(code, g, ids, n_rows, scale):
+    lib = _lib.load()
+    n, D = ids.numel(), g.shape[-1]
     g2 = _rows(g if g.dim() == 2 else g.reshape(n, D))
     dw = torch.empty(n_rows, D, dtype=g.dtype, device=g.device)
-    size = lib.bg_embedding_bwd_workspace(code, n, n_rows, D)
+    size = _embedding_grad_size(code, n, n_rows, D)
     ws = torch.empty(size, dtype=torch.uint8, device=g.device) if size else None
-    check(lib.bg_embedding_bwd(code, g2.data_ptr(), _ld(g2), i.data_ptr(), i.dtype == torch.int64, n, D, n_rows, scale, dw.data_ptr(),
+    check(lib.bg_embedding_bwd(code, g2.data_ptr(), _ld(g2), ids.data_ptr(), ids.dtype == torch.int64, n, D, n_rows, scale, dw.data_ptr(),
                                ptr(ws), size, stream()), "bg_embedding_bwd")
     return dw
 
@@ -992,8 +1002,10 @@ class Embedding(torch.autograd.Function):
     @staticmethod
     def backward(ctx, g):
         (ids,) = ctx.saved_tensors
-        grad = EmbeddingGrad.apply if torch.is_grad_enabled() else embedding_grad_raw    # grad mode: create_graph asked for it
-        return grad(g, ids, ctx.n_rows, ctx.scale), None, None
+        if torch.is_grad_enabled():                      # create_graph asked for it
+            return EmbeddingGrad.apply(g, ids, ctx.n_rows, ctx.scale), None, None
+        # (checked by the forward call; autograd runs this on the weight's device)
+        return _embedding_backward(_ELEM[g.dtype], g, ids if ids.is_contiguous() else ids.contiguous(), ctx.n_rows, ctx.scale), None, None
 
 
 class EmbeddingGrad(torch.autograd.Function):
