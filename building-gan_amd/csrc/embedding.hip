@@ -64,6 +64,9 @@ __device__ __forceinline__ void st_sums(float* __restrict__ p, int D, const floa
 // The output is a flat row of n * nv pieces; a thread moves U pieces 256 apart, so stores are contiguous whatever the width.
 // Piece -> row needs a division by nv: the block's first row comes from one 64-bit division (scalar), the rest from a
 // multiplication by `magic` = ceil(2^32 / nv), exact while (256 U + nv) * nv < 2^32.
+// Bound by the bytes written (and read, where the table is larger than the caches): 1,048,576 x 128 fp32 from 7 rows 99 us
+// (5.4 TB/s), 65,537 x 520 fp16 from 131,071 rows 31 us (4.4 TB/s read and written, rows at any alignment), 16,384 x 1,024
+// bf16 10.8 us (33.6 MB: a launch's own 2.5 us count).
 template <class T, int U, bool I64, bool NARROW, bool STREAM>      // STREAM: an output that no cache holds
 __global__ __launch_bounds__(256) void k_embedding_fwd(const T* __restrict__ w, int64_t ldw, int64_t V, const void* __restrict__ ids,
                                                        int64_t n, uint32_t nv, uint32_t magic, int D, float scale, T* __restrict__ out,
@@ -108,6 +111,9 @@ __global__ __launch_bounds__(256) void k_embedding_fwd(const T* __restrict__ w, 
 // LG lanes walk over rows of g, four elements each (8 or 16 bytes; the last lane's begin four before the row's end); their
 // sums of every table row stand in LDS, a float4 for every table row and lane that no other lane touches.  The block's
 // groups are added up in order and leave one partial table, the blocks' tables are added up by a second launch.
+// g is read once and nothing else is large: 1,048,576 x 128 fp32 into 7 rows 94 us + 7 us for the blocks' tables (537 MB,
+// 5.3 TB/s).  LDS is what limits it: a row more is 4 KB a block, so with more rows fewer loads are in flight (20 rows 46 us
+// against 56 us sorted at 262,144 x 128 fp32, 32 rows 93 us against 54 us: the sort from 21 rows on).
 template <class T>
 struct __attribute__((packed, aligned(sizeof(T)))) Four { T v[4]; };
 template <class T, bool I64, bool NARROW>      // NARROW: D < 4
@@ -177,7 +183,8 @@ __global__ __launch_bounds__(kFewCols* kFewSplit) void k_embedding_few_join(cons
 // ------------------------------------------------------------------------------------------------ stable sort of the ids
 // Least significant digit first, one pass = a histogram per tile of keys and a placement.  The key of a missing token is
 // V, behind every row.  Both launches carry extra workgroups that zero a share of dW meanwhile: the sort of a batch's
-// tokens is bound by latency, not by memory.
+// tokens is bound by latency, not by memory (16,384 tokens of 32,000: four launches, 25 us, which the 65 MB of zeros fit
+// into; 65,537 of 131,071: 41 us and 136 MB).
 constexpr int kDigitBits = 9;
 constexpr int kBins = 1 << kDigitBits;
 constexpr int kSortThreads = 512;
@@ -259,6 +266,7 @@ __device__ __forceinline__ int wave_rank(int d, bool valid, int bits, int lane, 
 }
 
 // All passes of up to kSmall keys by one workgroup, keys and positions in registers and LDS; the other workgroups zero dW.
+// (One launch instead of two for every digit; four keys a thread measured as well as eight and sixteen.)
 constexpr int kSmallThreads = 1024, kSmallRounds = 4, kSmall = kSmallThreads * kSmallRounds;
 template <int SRC>
 __global__ __launch_bounds__(kSmallThreads) void k_sort_small(const void* __restrict__ src, int n, int64_t V, int passes, int bits,
@@ -389,6 +397,8 @@ __global__ __launch_bounds__(kSortThreads) void k_sort_place(const void* __restr
 // ------------------------------------------------------------------------------------------------ sums over the runs
 // LG lanes carry one tile of C slots over LG pieces of a row.  They read LG slots at a time, one each, and pass them round.
 // part[(2 * tile + which) * D + c]: which 0 = the run that began in an earlier tile, 1 = one that goes on into the next
+// Bound by the gather of g's rows: eight loads in flight a lane, asked for whether or not the slot's token exists (35.8 ->
+// 28.2 us at 65,537 x 520 fp16).  16,384 x 1,024 bf16: 10.9 us (33.6 MB read, 14.6 MB written: 4.4 TB/s).
 // (a scalar where the wave carries one tile)
 __device__ __forceinline__ int32_t pass_round(int32_t v, int lane, int LG) {
     return LG == 64 ? __builtin_amdgcn_readlane(v, lane) : __shfl(v, lane, LG);
@@ -451,7 +461,8 @@ __global__ __launch_bounds__(256) void k_embedding_runs(const int32_t* __restric
 }
 
 // The run that begins in tile blockIdx.x and goes on: its own partial and the following tiles' are added by kJoin threads a
-// column (strided over the tiles), those kJoin sums then in order.
+// column (strided over the tiles), those kJoin sums then in order.  Latency: the search for a long run's end and the walk
+// over its tiles (7.6 us where a fifteenth of 16,384 tokens are one; two threads a column measured best of 2, 4, 8, 16).
 constexpr int kJoin = 2, kJoinCols = 64;
 template <class T>
 __global__ __launch_bounds__(kJoin* kJoinCols) void k_embedding_join(const int32_t* __restrict__ key, int64_t n, int32_t V,

@@ -765,3 +765,27 @@ def test_autograd_captured_and_replayed(cuda):
         got = [t.clone() for t in outs]
         for i, (a, b) in enumerate(zip(got, step())):
             assert torch.equal(a, b), (k, i)
+
+
+@pytest.mark.gpu
+def test_one_token_and_broadcast_operands(cuda):
+    """A scalar id, no ids with a gradient asked for, and operands expanded over the batch: their gradients add up."""
+    from building_gan_amd import ops
+    w = torch.randn(6, 9, device=cuda, requires_grad=True)
+    one = ops.embedding(w, torch.tensor(4, device=cuda), 2.0)
+    assert one.shape == (9,) and torch.equal(torch.autograd.grad(one, w, torch.ones(9, device=cuda))[0][:, 0].cpu(), torch.tensor([0., 0, 0, 0, 2, 0]))
+    none = ops.embedding(w, torch.zeros(0, 3, dtype=torch.int64, device=cuda))
+    assert not torch.autograd.grad(none, w, torch.zeros(0, 3, 9, device=cuda))[0].any()
+    x = torch.randn(1, 40, 12, device=cuda, requires_grad=True)
+    gate = torch.randn(3, 40, 12, device=cuda, requires_grad=True)
+    h, hl = ops.gated_scan(x.expand(3, 40, 12), gate)
+    dx, dg = torch.autograd.grad(h.sum() + hl.sum(), (x, gate))
+    xs = x.detach().expand(3, 40, 12).contiguous().requires_grad_(True)
+    h2, hl2 = ops.gated_scan(xs, gate)
+    dx2, dg2 = torch.autograd.grad(h2.sum() + hl2.sum(), (xs, gate))
+    assert torch.equal(h, h2) and torch.equal(dg, dg2) and torch.equal(dx, dx2.sum(0, keepdim=True))
+    y = torch.randn(50, 8, device=cuda, requires_grad=True)              # one tensor as both operands
+    (dy,) = torch.autograd.grad(ops.gated_scan(y, y)[0].sum(), y)
+    y1, y2 = y.detach().clone().requires_grad_(True), y.detach().clone().requires_grad_(True)
+    a, b = torch.autograd.grad(ops.gated_scan(y1, y2)[0].sum(), (y1, y2))
+    assert torch.equal(dy, a + b)
