@@ -90,14 +90,28 @@ __device__ __forceinline__ void mark_tile(const Segs& g, int64_t row0, int group
 // a = sigmoid(g), c = sigmoid(-g) without cancellation: e = exp(-|g|) <= 1, r = 1 / (1 + e); one of them is r, the other e r.
 // What the rounding of |g| log2(e) leaves out is put back (e * (1 + rest)) and the reciprocal takes one Newton step: v_exp_f32
 // and v_rcp_f32 alone are off by up to an ulp to one side, which a product over a long memory's a's would add up.
-__device__ __forceinline__ void gate_pair(float g, float& a, float& c) {
+struct Sides { float r, er; };                       // the larger and the smaller of the two
+__device__ __forceinline__ Sides gate_sides(float g) {
     const float m = __builtin_elementwise_minimum(fabsf(g), 110.f);      // e^-110 is 0 in fp32; a NaN stays one
     const float p = m * -1.4426950408889634f;
     float e = __builtin_amdgcn_exp2f(p);
     e = fmaf(e, fmaf(p, -0.6931471805599453f, -m), e);
-    const float s = 1.f + e, r0 = __builtin_amdgcn_rcpf(s), r = fmaf(r0, fmaf(-s, r0, 1.f), r0), er = e * r;
-    a = g < 0.f ? er : r;
-    c = g < 0.f ? r : er;
+    const float s = 1.f + e, r0 = __builtin_amdgcn_rcpf(s), r = fmaf(r0, fmaf(-s, r0, 1.f), r0);
+    return {r, e * r};
+}
+__device__ __forceinline__ void gate_pair(float g, float& a, float& c) {
+    const Sides h = gate_sides(g);
+    a = g < 0.f ? h.er : h.r;
+    c = g < 0.f ? h.r : h.er;
+}
+// Both in one register: the smaller one with the sign of the gate; the larger one is 1 minus it, which is exact to its own
+// rounding (the smaller is at most 1/2).
+__device__ __forceinline__ float pack_gate(float g) { return copysignf(gate_sides(g).er, g); }
+__device__ __forceinline__ void unpack_gate(float p, float& a, float& c) {
+    const float t = fabsf(p), big = 1.f - t;
+    const bool low = __float_as_int(p) < 0;
+    a = low ? t : big;
+    c = low ? big : t;
 }
 
 // Four columns of a row as one access at whatever alignment the row has (the hardware takes any; the alignment promised to
@@ -358,11 +372,12 @@ __device__ __forceinline__ float enter_block(const Chain& ch, uint32_t k, uint32
 
 // The next (tile, column block) in the order of the walk; with a single tile there is nothing to order.  false: none left
 // (a ticket that another call's workgroups also draw from).  A counter answers about once in 17 ns, so workgroups that start
-// together wait for it: 1,024 of the forward pass for 17 us.  There the column blocks are dealt out to up to 8 counters, each
-// on a cache line of its own (16,384 x 2,048 bf16: 58 us, 74 us with one counter; 262,144 x 512 bf16: 235 and 246 us).  The
-// backward pass starts half as many, waits longer for its rows, and loses more where the column blocks of a row get out of
-// step (1,048,576 x 128 fp32: 562 us with one counter, 577 us with 2 and with 8; 16,384 x 2,048 fp32: 149, 149 and 155 us).
-constexpr uint32_t kFwdTickets = 8, kBwdTickets = 1, kTicketStep = 32, kXcds = 8;
+// together wait for it: 1,024 of the forward pass for 17 us, 768 of the 16-bit backward pass for 13 us.  There the column
+// blocks are dealt out to up to 8 counters, each on a cache line of its own (forward, 16,384 x 2,048 bf16: 58 us, 74 us with
+// one counter; 262,144 x 512 bf16: 235 and 246 us; backward 108 and 113 us, 394 and 394 us).  The fp32 backward pass starts 512,
+// waits for memory anyway, and loses where the column blocks of a row get out of step (1,048,576 x 128: 562 us with one
+// counter, 577 us with 2 and with 8; 16,384 x 2,048: 149, 149 and 155 us).
+constexpr uint32_t kTickets = 8, kTicketStep = 32, kXcds = 8;
 template <uint32_t TICKETS>
 __device__ __forceinline__ bool take_tile(const Chain& ch, int64_t n_tiles, int64_t& tile, int& cb) {
     __shared__ uint32_t ticket;
@@ -543,7 +558,7 @@ __global__ __launch_bounds__(kThreads, 4) void k_scan_fwd(const T* __restrict__ 
     __shared__ TileShared sh;
     int64_t tile;
     int cb;
-    if (!take_tile<kFwdTickets>(ch, n_tiles, tile, cb)) return;
+    if (!take_tile<kTickets>(ch, n_tiles, tile, cb)) return;
     const Place p = place<REV>(g, D, CG, tile, cb);
     if (threadIdx.x < 64) mark_tile<REV>(g, p.row0, p.RG, sh.mask, sh.first, sh.last, sh.border);
     float a[kRows][4], b[kRows][4];                                      // a row's map: s -> a s + b, b = c x
@@ -600,11 +615,30 @@ __global__ __launch_bounds__(kThreads, 4) void k_scan_fwd(const T* __restrict__ 
 // ------------------------------------------------------------------------------------------------ backward
 // The walk for mu goes from the last tile to the first.  h before a row group was kept by the forward pass, so
 // q = (h_before - x) a c is made while the tile's state is asked for; per element a, c, dh and q stay: dx = c lam,
-// dgate = q lam.  fp32 rows are bound by memory again (1,048,576 x 128: 562 us, 4.78 TB/s); 16-bit rows by two waves a SIMD
-// (190 registers: a, c, q of a row group in fp32), which hide less of the loads' and the look-back's latency: 262,144 x 512
-// bf16 436 us (3.1 TB/s; without the look-back 370 us; held to three waves by spilling 464 us).
+// dgate = q lam.  fp32 rows are bound by memory again (1,048,576 x 128: 562 us, 4.78 TB/s).  16-bit rows want waves to hide
+// the loads' and the look-back's latency: with a and c in one register three waves a SIMD fit (262,144 x 512 bf16 394 us, 3.4
+// TB/s; apart and two waves 436 us; apart and three waves by spilling 464 us).  For fp32 rows, whose x and dh take twice the
+// registers, taking them apart only costs (577 us for 562).
+// a and c of a thread's rows, made from the gates in v.  PACKED: both in v (32 registers less), taken apart where they are
+// used (and settled there, or the compiler would keep what it took apart).
+template <bool PACKED>
+struct Gates {
+    float v[kRows][4];
+    __device__ __forceinline__ void make(int i, int e) { v[i][e] = pack_gate(v[i][e]); settle(v[i][e]); }
+    __device__ __forceinline__ void get(int i, int e, float& a, float& c) { settle(v[i][e]); unpack_gate(v[i][e], a, c); }
+};
+template <>
+struct Gates<false> {
+    float v[kRows][4], a_[kRows][4];                                     // v: c
+    __device__ __forceinline__ void make(int i, int e) {
+        gate_pair(v[i][e], a_[i][e], v[i][e]);
+        settle(a_[i][e]);
+        settle(v[i][e]);
+    }
+    __device__ __forceinline__ void get(int i, int e, float& a, float& c) { a = a_[i][e]; c = v[i][e]; }
+};
 template <class T, bool REV>
-__global__ __launch_bounds__(kThreads) void k_scan_bwd(const T* __restrict__ x, int64_t ldx, const T* __restrict__ gate, int64_t ldg,
+__global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 3 : 2) void k_scan_bwd(const T* __restrict__ x, int64_t ldx, const T* __restrict__ gate, int64_t ldg,
                                                        const T* __restrict__ dh, int64_t lddh, const float* __restrict__ dlast, Segs g,
                                                        int64_t D, const float* __restrict__ h0, int CG, Chain ch, int64_t n_tiles,
                                                        const float* __restrict__ heads, T* __restrict__ dx, int64_t lddx,
@@ -612,13 +646,15 @@ __global__ __launch_bounds__(kThreads) void k_scan_bwd(const T* __restrict__ x, 
     __shared__ TileShared sh;
     int64_t k;
     int cb;
-    if (!take_tile<kBwdTickets>(ch, n_tiles, k, cb)) return;
+    if (!take_tile<sizeof(T) == 2 ? kTickets : 1>(ch, n_tiles, k, cb)) return;
     const int64_t tile = n_tiles - 1 - k;
     const Place p = place<REV>(g, D, CG, tile, cb);
     if (threadIdx.x < 64) mark_tile<REV>(g, p.row0, p.RG, sh.mask, sh.first, sh.last, sh.border);
-    float a[kRows][4], cc[kRows][4], q[kRows][4], s[4];
+    Gates<sizeof(T) == 2> gates;
+    float (&dxs)[kRows][4] = gates.v;                                    // the gates as read, then a and c, then dx
+    float q[kRows][4], s[4];
     Raw<T> xr, dr;
-    load_tile<T, REV>(gate, ldg, p, __builtin_inff(), a);
+    load_tile<T, REV>(gate, ldg, p, __builtin_inff(), gates.v);
     if (dh) load_tile<T, REV>(dh, lddh, p, dr);
     else
 #pragma unroll
@@ -630,11 +666,7 @@ __global__ __launch_bounds__(kThreads) void k_scan_bwd(const T* __restrict__ x, 
 #pragma unroll
     for (int i = 0; i < kRows; ++i)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            gate_pair(a[i][e], a[i][e], cc[i][e]);
-            settle(a[i][e]);
-            settle(cc[i][e]);
-        }
+        for (int e = 0; e < 4; ++e) gates.make(i, e);
     __syncthreads();
     const bool border = __builtin_amdgcn_readfirstlane(sh.border) != 0;
     const Borders w(sh, p, CG, border);
@@ -647,8 +679,10 @@ __global__ __launch_bounds__(kThreads) void k_scan_bwd(const T* __restrict__ x, 
         if (bit(w.wave_leave, i)) leave_row(w, i, sh, p, dlast, D, d, u.B);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            u.B[e] = a[i][e] * (d[e] + u.B[e]);
-            u.A[e] *= a[i][e];
+            float a, c;
+            gates.get(i, e, a, c);
+            u.B[e] = a * (d[e] + u.B[e]);
+            u.A[e] *= a;
         }
     }
     settle(dr);
@@ -663,8 +697,10 @@ __global__ __launch_bounds__(kThreads) void k_scan_bwd(const T* __restrict__ x, 
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const float xi = xr.get(i, e), hb = s[e];
-            s[e] = fmaf(a[i][e], hb, cc[i][e] * xi);
-            q[i][e] = (hb - xi) * (a[i][e] * cc[i][e]);
+            float a, c;
+            gates.get(i, e, a, c);
+            s[e] = fmaf(a, hb, c * xi);
+            q[i][e] = (hb - xi) * (a * c);
         }
     }
     answer(ch, k, n_tiles, D, CG, p, u, sh, s);
@@ -677,20 +713,22 @@ __global__ __launch_bounds__(kThreads) void k_scan_bwd(const T* __restrict__ x, 
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const float lam = d[e] + s[e];
-            cc[i][e] *= lam;
+            float a, c;
+            gates.get(i, e, a, c);
+            dxs[i][e] = c * lam;
             q[i][e] *= lam;
-            s[e] = a[i][e] * lam;
+            s[e] = a * lam;
         }
         if (bit(w.wave_enter, i)) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {                                // rows in no segment: 0, whatever they hold
-                cc[i][e] = bit(w.none, i) ? 0.f : cc[i][e];
+                dxs[i][e] = bit(w.none, i) ? 0.f : dxs[i][e];
                 q[i][e] = bit(w.none, i) ? 0.f : q[i][e];
             }
             if (bit(w.m, i) && dh0) st_state(dh0, sh.first[p.r0 + i], D, p.c, p.l.nv, s);
         }
     }
-    store_tile<T, REV>(dx, lddx, p, cc);
+    store_tile<T, REV>(dx, lddx, p, dxs);
     store_tile<T, REV>(dgate, lddg, p, q);
     pass_through<REV>(g, D, tile, n_tiles, p, dlast, dh0);
 }
@@ -751,7 +789,7 @@ ScanWs scan_ws(int64_t n, int64_t D) {
     w.tile = take(8 * (t / kGroup + 1) * kGroup * lane);
     w.group = take(8 * blocks * kGroup * lane);
     w.state = take(4 * blocks * lane);
-    w.ticket = take(4 * kTicketStep * kFwdTickets);
+    w.ticket = take(4 * kTicketStep * kTickets);
     w.bytes = at;
     return w;
 }
