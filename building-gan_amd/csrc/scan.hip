@@ -87,6 +87,11 @@ __device__ __forceinline__ void mark_tile(const Segs& g, int64_t row0, int group
     if (t == 0) border = found;
 }
 
+// The value is computed here and what follows is computed from it: left to itself, the compiler moves the last steps of a
+// sigmoid to where its result is used, or keeps products of one walk over the rows for a later one, and either way holds a
+// row's worth of registers more than the values it has.
+__device__ __forceinline__ void settle(float& v) { asm volatile("" : "+v"(v)); }
+
 // a = sigmoid(g), c = sigmoid(-g) without cancellation: e = exp(-|g|) <= 1, r = 1 / (1 + e); one of them is r, the other e r.
 // What the rounding of |g| log2(e) leaves out is put back (e * (1 + rest)) and the reciprocal takes one Newton step: v_exp_f32
 // and v_rcp_f32 alone are off by up to an ulp to one side, which a product over a long memory's a's would add up.
@@ -107,7 +112,8 @@ __device__ __forceinline__ void gate_pair(float g, float& a, float& c) {
 // Both in one register: the smaller one with the sign of the gate; the larger one is 1 minus it, which is exact to its own
 // rounding (the smaller is at most 1/2).
 __device__ __forceinline__ float pack_gate(float g) { return copysignf(gate_sides(g).er, g); }
-__device__ __forceinline__ void unpack_gate(float p, float& a, float& c) {
+__device__ __forceinline__ void unpack_gate(float& p, float& a, float& c) {
+    settle(p);                                       // (or what is taken apart here is kept for the next walk)
     const float t = fabsf(p), big = 1.f - t;
     const bool low = __float_as_int(p) < 0;
     a = low ? t : big;
@@ -211,17 +217,18 @@ __device__ __forceinline__ uint32_t wave_mask(uint32_t m, int CG) {
 __device__ __forceinline__ bool bit(uint32_t m, int i) { return (m >> i) & 1; }
 
 struct Map { float A[4], B[4]; };
-// The value is computed here and what follows is computed from it: left to itself, the compiler moves the last steps of a
-// sigmoid to where its result is used, or keeps products of one walk over the rows for a later one, and either way holds a
-// row's worth of registers more than the values it has.
-__device__ __forceinline__ void settle(float& v) { asm volatile("" : "+v"(v)); }
+template <class T>
+__device__ __forceinline__ void settle(Piece<T>& x) {
+    uint32_t w[sizeof(T)];
+    __builtin_memcpy(w, &x, sizeof(w));
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T); ++i) asm volatile("" : "+v"(w[i]));
+    __builtin_memcpy(&x, w, sizeof(w));
+}
 template <class T>
 __device__ __forceinline__ void settle(Raw<T>& r) {
-    uint32_t w[sizeof(T) * kRows];
-    __builtin_memcpy(w, &r, sizeof(w));
 #pragma unroll
-    for (int i = 0; i < (int)sizeof(T) * kRows; ++i) asm volatile("" : "+v"(w[i]));
-    __builtin_memcpy(&r, w, sizeof(w));
+    for (int i = 0; i < kRows; ++i) settle(r.v[i]);
 }
 __device__ __forceinline__ void settle(float (&v)[kRows][4]) {
 #pragma unroll
@@ -372,20 +379,17 @@ __device__ __forceinline__ float enter_block(const Chain& ch, uint32_t k, uint32
 
 // The next (tile, column block) in the order of the walk; with a single tile there is nothing to order.  false: none left
 // (a ticket that another call's workgroups also draw from).  A counter answers about once in 17 ns, so workgroups that start
-// together wait for it: 1,024 of the forward pass for 17 us, 768 of the 16-bit backward pass for 13 us.  There the column
-// blocks are dealt out to up to 8 counters, each on a cache line of its own (forward, 16,384 x 2,048 bf16: 58 us, 74 us with
-// one counter; 262,144 x 512 bf16: 235 and 246 us; backward 108 and 113 us, 394 and 394 us).  The fp32 backward pass starts 512,
-// waits for memory anyway, and loses where the column blocks of a row get out of step (1,048,576 x 128: 562 us with one
-// counter, 577 us with 2 and with 8; 16,384 x 2,048: 149, 149 and 155 us).
+// together wait for it: 1,024 of the forward pass for 17 us, 768 of the backward pass for 13 us.  So the column blocks are
+// dealt out to up to 8 counters, each on a cache line of its own (16,384 x 2,048 bf16 forward 58 us, 74 us with one counter,
+// backward 108 and 113 us; 262,144 x 512 bf16 forward 235 and 246 us; no difference where memory is the bound).
 constexpr uint32_t kTickets = 8, kTicketStep = 32, kXcds = 8;
-template <uint32_t TICKETS>
 __device__ __forceinline__ bool take_tile(const Chain& ch, int64_t n_tiles, int64_t& tile, int& cb) {
     __shared__ uint32_t ticket;
     const uint32_t even = (uint32_t)n_tiles / kXcds * kXcds * ch.ncb;    // eight workgroups, one on every XCD, draw from a counter,
     const uint32_t at = (blockIdx.x < even ? blockIdx.x / kXcds : blockIdx.x) % ch.ncb;   // so the counters stay in step
     uint32_t k = blockIdx.x, set = 0, sets = 1;
     if (n_tiles > 1) {
-        sets = ch.ncb < TICKETS ? ch.ncb : TICKETS;
+        sets = ch.ncb < kTickets ? ch.ncb : kTickets;
         set = at % sets;
         if (threadIdx.x == 0) ticket = atomicAdd(ch.ticket + set * kTicketStep, 1u);
         __syncthreads();
@@ -520,6 +524,10 @@ struct Borders {
             wave_leave = wave_mask(leave, CG);
         }
     }
+    // before the next walk over the rows: or the compiler keeps the tests of 8 rows' bits, a register each
+    __device__ __forceinline__ void again() {
+        asm volatile("" : "+v"(m), "+v"(none), "+v"(enter), "+v"(leave));
+    }
 };
 // s <- the state before row i of the group where a segment begins there (0 where the row is in none)
 __device__ __forceinline__ void enter_row(const Borders& w, int i, const TileShared& sh, const Place& p, const float* __restrict__ h0, int64_t D,
@@ -558,7 +566,7 @@ __global__ __launch_bounds__(kThreads, 4) void k_scan_fwd(const T* __restrict__ 
     __shared__ TileShared sh;
     int64_t tile;
     int cb;
-    if (!take_tile<kTickets>(ch, n_tiles, tile, cb)) return;
+    if (!take_tile(ch, n_tiles, tile, cb)) return;
     const Place p = place<REV>(g, D, CG, tile, cb);
     if (threadIdx.x < 64) mark_tile<REV>(g, p.row0, p.RG, sh.mask, sh.first, sh.last, sh.border);
     float a[kRows][4], b[kRows][4];                                      // a row's map: s -> a s + b, b = c x
@@ -576,7 +584,7 @@ __global__ __launch_bounds__(kThreads, 4) void k_scan_fwd(const T* __restrict__ 
         }
     __syncthreads();
     const bool border = __builtin_amdgcn_readfirstlane(sh.border) != 0;
-    const Borders w(sh, p, CG, border);
+    Borders w(sh, p, CG, border);
     Map f{{1.f, 1.f, 1.f, 1.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
     for (int i = 0; i < kRows; ++i) {
@@ -599,6 +607,7 @@ __global__ __launch_bounds__(kThreads, 4) void k_scan_fwd(const T* __restrict__ 
     const Map all = border ? before_group<false, true>(f, CG, p.cg, sh.wm) : before_group<false, false>(f, CG, p.cg, sh.wm);
     float s[4];
     ask(ch, tile, n_tiles, D, CG, p, p.rg == p.RG - 1, all, sh);
+    w.again();
     answer(ch, tile, n_tiles, D, CG, p, f, sh, s);
     if (heads && p.l.nrows > 0) st_state(heads, tile * p.RG + p.rg, D, p.c, p.l.nv, s);
 #pragma unroll
@@ -615,30 +624,12 @@ __global__ __launch_bounds__(kThreads, 4) void k_scan_fwd(const T* __restrict__ 
 // ------------------------------------------------------------------------------------------------ backward
 // The walk for mu goes from the last tile to the first.  h before a row group was kept by the forward pass, so
 // q = (h_before - x) a c is made while the tile's state is asked for; per element a, c, dh and q stay: dx = c lam,
-// dgate = q lam.  fp32 rows are bound by memory again (1,048,576 x 128: 562 us, 4.78 TB/s).  16-bit rows want waves to hide
-// the loads' and the look-back's latency: with a and c in one register three waves a SIMD fit (262,144 x 512 bf16 394 us, 3.4
-// TB/s; apart and two waves 436 us; apart and three waves by spilling 464 us).  For fp32 rows, whose x and dh take twice the
-// registers, taking them apart only costs (577 us for 562).
-// a and c of a thread's rows, made from the gates in v.  PACKED: both in v (32 registers less), taken apart where they are
-// used (and settled there, or the compiler would keep what it took apart).
-template <bool PACKED>
-struct Gates {
-    float v[kRows][4];
-    __device__ __forceinline__ void make(int i, int e) { v[i][e] = pack_gate(v[i][e]); settle(v[i][e]); }
-    __device__ __forceinline__ void get(int i, int e, float& a, float& c) { settle(v[i][e]); unpack_gate(v[i][e], a, c); }
-};
-template <>
-struct Gates<false> {
-    float v[kRows][4], a_[kRows][4];                                     // v: c
-    __device__ __forceinline__ void make(int i, int e) {
-        gate_pair(v[i][e], a_[i][e], v[i][e]);
-        settle(a_[i][e]);
-        settle(v[i][e]);
-    }
-    __device__ __forceinline__ void get(int i, int e, float& a, float& c) { a = a_[i][e]; c = v[i][e]; }
-};
+// dgate = q lam.  Three waves a SIMD hide the loads' and the look-back's latency, so registers are what counts: a and c in one,
+// x and dh as they came, nothing kept from one walk over the rows for the next (133 registers for 16-bit rows, 163 for fp32).
+// 1,048,576 x 128 fp32 525 us (5.1 TB/s; a and c apart, two waves: 553 us), 262,144 x 512 bf16 342 us (3.9 TB/s; apart, two
+// waves: 436 us; four waves by spilling ten registers: 346 us).
 template <class T, bool REV>
-__global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 3 : 2) void k_scan_bwd(const T* __restrict__ x, int64_t ldx, const T* __restrict__ gate, int64_t ldg,
+__global__ __launch_bounds__(kThreads, 3) void k_scan_bwd(const T* __restrict__ x, int64_t ldx, const T* __restrict__ gate, int64_t ldg,
                                                        const T* __restrict__ dh, int64_t lddh, const float* __restrict__ dlast, Segs g,
                                                        int64_t D, const float* __restrict__ h0, int CG, Chain ch, int64_t n_tiles,
                                                        const float* __restrict__ heads, T* __restrict__ dx, int64_t lddx,
@@ -646,15 +637,13 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 3 : 2) void k_scan_bwd(c
     __shared__ TileShared sh;
     int64_t k;
     int cb;
-    if (!take_tile<sizeof(T) == 2 ? kTickets : 1>(ch, n_tiles, k, cb)) return;
+    if (!take_tile(ch, n_tiles, k, cb)) return;
     const int64_t tile = n_tiles - 1 - k;
     const Place p = place<REV>(g, D, CG, tile, cb);
     if (threadIdx.x < 64) mark_tile<REV>(g, p.row0, p.RG, sh.mask, sh.first, sh.last, sh.border);
-    Gates<sizeof(T) == 2> gates;
-    float (&dxs)[kRows][4] = gates.v;                                    // the gates as read, then a and c, then dx
-    float q[kRows][4], s[4];
+    float ac[kRows][4], q[kRows][4], s[4];                               // ac: the gates as read, then a and c, then dx
     Raw<T> xr, dr;
-    load_tile<T, REV>(gate, ldg, p, __builtin_inff(), gates.v);
+    load_tile<T, REV>(gate, ldg, p, __builtin_inff(), ac);
     if (dh) load_tile<T, REV>(dh, lddh, p, dr);
     else
 #pragma unroll
@@ -666,10 +655,15 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 3 : 2) void k_scan_bwd(c
 #pragma unroll
     for (int i = 0; i < kRows; ++i)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) gates.make(i, e);
+        for (int e = 0; e < 4; ++e) {
+            ac[i][e] = pack_gate(ac[i][e]);
+            settle(ac[i][e]);
+        }
+    settle(dr);
+    settle(xr);
     __syncthreads();
     const bool border = __builtin_amdgcn_readfirstlane(sh.border) != 0;
-    const Borders w(sh, p, CG, border);
+    Borders w(sh, p, CG, border);
     Map u{{1.f, 1.f, 1.f, 1.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
     for (int i = kRows - 1; i >= 0; --i) {
@@ -680,13 +674,14 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 3 : 2) void k_scan_bwd(c
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             float a, c;
-            gates.get(i, e, a, c);
+            unpack_gate(ac[i][e], a, c);
             u.B[e] = a * (d[e] + u.B[e]);
             u.A[e] *= a;
         }
     }
     settle(dr);
     settle(xr);
+    w.again();
 #pragma unroll
     for (int e = 0; e < 4; ++e) u.A[e] = w.leave ? -1.f : u.A[e];
     const Map all = border ? before_group<true, true>(u, CG, p.cg, sh.wm) : before_group<true, false>(u, CG, p.cg, sh.wm);
@@ -698,15 +693,18 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 3 : 2) void k_scan_bwd(c
         for (int e = 0; e < 4; ++e) {
             const float xi = xr.get(i, e), hb = s[e];
             float a, c;
-            gates.get(i, e, a, c);
+            unpack_gate(ac[i][e], a, c);
             s[e] = fmaf(a, hb, c * xi);
             q[i][e] = (hb - xi) * (a * c);
+            settle(q[i][e]);
         }
     }
+    w.again();
     answer(ch, k, n_tiles, D, CG, p, u, sh, s);
 #pragma unroll
     for (int i = kRows - 1; i >= 0; --i) {
         float d[4];
+        settle(dr.v[i]);
 #pragma unroll
         for (int e = 0; e < 4; ++e) d[e] = dr.get(i, e);
         if (bit(w.wave_leave, i)) leave_row(w, i, sh, p, dlast, D, d, s);
@@ -714,21 +712,21 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 3 : 2) void k_scan_bwd(c
         for (int e = 0; e < 4; ++e) {
             const float lam = d[e] + s[e];
             float a, c;
-            gates.get(i, e, a, c);
-            dxs[i][e] = c * lam;
+            unpack_gate(ac[i][e], a, c);
+            ac[i][e] = c * lam;
             q[i][e] *= lam;
             s[e] = a * lam;
         }
         if (bit(w.wave_enter, i)) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {                                // rows in no segment: 0, whatever they hold
-                dxs[i][e] = bit(w.none, i) ? 0.f : dxs[i][e];
+                ac[i][e] = bit(w.none, i) ? 0.f : ac[i][e];
                 q[i][e] = bit(w.none, i) ? 0.f : q[i][e];
             }
             if (bit(w.m, i) && dh0) st_state(dh0, sh.first[p.r0 + i], D, p.c, p.l.nv, s);
         }
     }
-    store_tile<T, REV>(dx, lddx, p, dxs);
+    store_tile<T, REV>(dx, lddx, p, ac);
     store_tile<T, REV>(dgate, lddg, p, q);
     pass_through<REV>(g, D, tile, n_tiles, p, dlast, dh0);
 }
