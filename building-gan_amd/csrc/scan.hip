@@ -92,32 +92,26 @@ __device__ __forceinline__ void mark_tile(const Segs& g, int64_t row0, int group
 // row's worth of registers more than the values it has.
 __device__ __forceinline__ void settle(float& v) { asm volatile("" : "+v"(v)); }
 
-// a = sigmoid(g), c = sigmoid(-g) without cancellation: e = exp(-|g|) <= 1, r = 1 / (1 + e); one of them is r, the other e r.
-// What the rounding of |g| log2(e) leaves out is put back (e * (1 + rest)) and the reciprocal takes one Newton step: v_exp_f32
-// and v_rcp_f32 alone are off by up to an ulp to one side, which a product over a long memory's a's would add up.
-struct Sides { float r, er; };                       // the larger and the smaller of the two
-__device__ __forceinline__ Sides gate_sides(float g) {
+// a = sigmoid(g), c = sigmoid(-g) without cancellation: with e = exp(-|g|) <= 1 the smaller one is e / (1 + e), at most 1/2, and
+// the larger one is 1 minus it, which is exact to its own rounding: a memory that is long because its a's are near 1 adds up no
+// one-sided errors of the reciprocal.  What the rounding of |g| log2(e) leaves out is put back (e * (1 + rest)).
+// Packed, both are one register: the smaller one with the sign of the gate.
+__device__ __forceinline__ float pack_gate(float g) {
     const float m = __builtin_elementwise_minimum(fabsf(g), 110.f);      // e^-110 is 0 in fp32; a NaN stays one
     const float p = m * -1.4426950408889634f;
     float e = __builtin_amdgcn_exp2f(p);
     e = fmaf(e, fmaf(p, -0.6931471805599453f, -m), e);
-    const float s = 1.f + e, r0 = __builtin_amdgcn_rcpf(s), r = fmaf(r0, fmaf(-s, r0, 1.f), r0);
-    return {r, e * r};
+    return copysignf(e * __builtin_amdgcn_rcpf(1.f + e), g);
 }
-__device__ __forceinline__ void gate_pair(float g, float& a, float& c) {
-    const Sides h = gate_sides(g);
-    a = g < 0.f ? h.er : h.r;
-    c = g < 0.f ? h.r : h.er;
+__device__ __forceinline__ void gate_pair(float p, float& a, float& c) {
+    const float small = fabsf(p), large = 1.f - small;
+    const bool low = __float_as_int(p) < 0;
+    a = low ? small : large;
+    c = low ? large : small;
 }
-// Both in one register: the smaller one with the sign of the gate; the larger one is 1 minus it, which is exact to its own
-// rounding (the smaller is at most 1/2).
-__device__ __forceinline__ float pack_gate(float g) { return copysignf(gate_sides(g).er, g); }
 __device__ __forceinline__ void unpack_gate(float& p, float& a, float& c) {
     settle(p);                                       // (or what is taken apart here is kept for the next walk)
-    const float t = fabsf(p), big = 1.f - t;
-    const bool low = __float_as_int(p) < 0;
-    a = low ? t : big;
-    c = low ? big : t;
+    gate_pair(p, a, c);
 }
 
 // Four columns of a row as one access at whatever alignment the row has (the hardware takes any; the alignment promised to
@@ -555,10 +549,10 @@ __device__ __forceinline__ void leave_row(const Borders& w, int i, const TileSha
 
 // ------------------------------------------------------------------------------------------------ forward
 // x and gate are read once, h (and an eighth of it in fp32) written once.  fp32 rows are bound by memory: 1,048,576 x 128
-// 333 us, 4.84 TB/s, what a copy of 4 GiB reaches (4.81).  16-bit rows carry half the bytes for the same arithmetic, about
-// 35 instructions an element: 262,144 x 512 bf16 235 us (3.4 TB/s), of which the SIMDs issue for half; without the look-back
+// 332 us, 4.85 TB/s, what a copy of 4 GiB reaches (4.81).  16-bit rows carry half the bytes for the same arithmetic, about
+// 33 instructions an element: 262,144 x 512 bf16 230 us (3.5 TB/s), of which the SIMDs issue for half; without the look-back
 // the same rows took 186 us, what remains of it is a tile's wait of some 3 us that four waves a SIMD do not hide.  The
-// bound of 128 registers (four waves instead of three) is worth 273 -> 247 us there.
+// bound of 128 registers (four waves instead of three) was worth 273 -> 247 us there; five would take spills.
 template <class T, bool REV>
 __global__ __launch_bounds__(kThreads, 4) void k_scan_fwd(const T* __restrict__ x, int64_t ldx, const T* __restrict__ gate, int64_t ldg, Segs g,
                                                        int64_t D, const float* __restrict__ h0, int CG, Chain ch, int64_t n_tiles,
@@ -577,7 +571,7 @@ __global__ __launch_bounds__(kThreads, 4) void k_scan_fwd(const T* __restrict__ 
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             float ce;
-            gate_pair(a[i][e], a[i][e], ce);
+            gate_pair(pack_gate(a[i][e]), a[i][e], ce);
             b[i][e] *= ce;
             settle(a[i][e]);
             settle(b[i][e]);
@@ -626,7 +620,7 @@ __global__ __launch_bounds__(kThreads, 4) void k_scan_fwd(const T* __restrict__ 
 // q = (h_before - x) a c is made while the tile's state is asked for; per element a, c, dh and q stay: dx = c lam,
 // dgate = q lam.  Three waves a SIMD hide the loads' and the look-back's latency, so registers are what counts: a and c in one,
 // x and dh as they came, nothing kept from one walk over the rows for the next (133 registers for 16-bit rows, 163 for fp32).
-// 1,048,576 x 128 fp32 525 us (5.1 TB/s; a and c apart, two waves: 553 us), 262,144 x 512 bf16 342 us (3.9 TB/s; apart, two
+// 1,048,576 x 128 fp32 527 us (5.1 TB/s; a and c apart, two waves: 553 us), 262,144 x 512 bf16 342 us (3.9 TB/s; apart, two
 // waves: 436 us; four waves by spilling ten registers: 346 us).
 template <class T, bool REV>
 __global__ __launch_bounds__(kThreads, 3) void k_scan_bwd(const T* __restrict__ x, int64_t ldx, const T* __restrict__ gate, int64_t ldg,
@@ -747,7 +741,7 @@ __global__ __launch_bounds__(256) void k_scan_step(const T* __restrict__ x, int6
 #pragma unroll
     for (int e = 0; e < W; ++e) {
         float a, c;
-        gate_pair((float)gv.v[e], a, c);
+        gate_pair(pack_gate((float)gv.v[e]), a, c);
         sv.v[e] = fmaf(a, sv.v[e], c * (float)xv.v[e]);
         hv.v[e] = bg_round<T>(sv.v[e]);
     }
