@@ -789,3 +789,38 @@ def test_one_token_and_broadcast_operands(cuda):
     y1, y2 = y.detach().clone().requires_grad_(True), y.detach().clone().requires_grad_(True)
     a, b = torch.autograd.grad(ops.gated_scan(y1, y2)[0].sum(), (y1, y2))
     assert torch.equal(dy, a + b)
+
+
+@pytest.mark.gpu
+def test_two_captured_graphs_replayed_at_once(cuda):
+    """Each graph keeps its own workspaces: replays on two streams, at the same time, do not disturb each other."""
+    from building_gan_amd import ops
+    gen = torch.Generator(device=cuda).manual_seed(12)
+    sides = []
+    for k, (N, D, V) in enumerate(((20000, 128, 900), (15000, 200, 40))):
+        x, gate, dh = (torch.randn(N, D, generator=gen, device=cuda) for _ in range(3))
+        ids = torch.randint(-1, V, (N,), generator=gen, device=cuda)
+        ptr = torch.tensor([0, N // 3, N], dtype=torch.int32, device=cuda)
+
+        def passes(x=x, gate=gate, dh=dh, ids=ids, ptr=ptr, V=V, k=k):
+            h, last, heads = ops.gated_scan_raw(x, gate, ptr, None, k == 1, keep_heads=True)
+            dx, dg, _ = ops.gated_scan_grad_raw(x, gate, ptr, None, k == 1, heads, dh, None)
+            return h, last, dx, dg, ops.embedding_grad_raw(dx, ids, V)
+
+        want = passes()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs = passes()
+        sides.append((graph, outs, want, torch.cuda.Stream(), passes))       # (passes holds what the graph reads)
+    for r in range(4):
+        for _, outs, *_ in sides:
+            for t in outs:
+                t.fill_(float("nan"))
+        torch.cuda.synchronize()
+        for graph, _, _, stream, _ in sides:
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        for k, (_, outs, want, *_) in enumerate(sides):
+            assert all(torch.equal(a, b) for a, b in zip(outs, want)), (r, k)
