@@ -249,7 +249,7 @@ __global__ __launch_bounds__(256) void k_sort_scan(int32_t* __restrict__ hist, i
 // Rank of this lane's digit among the wave's equal digits of earlier rounds and lower lanes; counts them in cnt (the wave's own
 // row: LDS keeps a wave's accesses in order).  Ballots over the digit's bits find the lanes that have the same one.
 template <class Count>
-__device__ __forceinline__ int wave_rank(int d, bool valid, int bits, int lane, Count* cnt) {
+__device__ __forceinline__ int wave_rank(int d, bool valid, int bits, Count* cnt) {
     const uint64_t live = __ballot(valid);
     uint32_t lo = (uint32_t)live, hi = (uint32_t)(live >> 32);
     for (int b = 0; b < bits; ++b) {
@@ -296,7 +296,7 @@ __global__ __launch_bounds__(kSmallThreads) void k_sort_small(const void* __rest
         __syncthreads();
 #pragma unroll
         for (int r = 0; r < kSmallRounds; ++r)
-            if (r < rounds) rank[r] = wave_rank((key[r] >> shift) & (bins - 1), key[r] >= 0, bits, lane, cnt[wave]);
+            if (r < rounds) rank[r] = wave_rank((key[r] >> shift) & (bins - 1), key[r] >= 0, bits, cnt[wave]);
         __syncthreads();
         int32_t all = 0, x = 0;                          // exclusive sums: over the waves, then over the bins
         if (t < kBins) {
@@ -371,7 +371,7 @@ __global__ __launch_bounds__(kSortThreads) void k_sort_place(const void* __restr
     }
     __syncthreads();
 #pragma unroll
-    for (int r = 0; r < ROUNDS; ++r) rank[r] = wave_rank((key[r] >> shift) & (bins - 1), key[r] >= 0, bits, lane, cnt[wave]);
+    for (int r = 0; r < ROUNDS; ++r) rank[r] = wave_rank((key[r] >> shift) & (bins - 1), key[r] >= 0, bits, cnt[wave]);
     // exclusive sum of `all` over the bins
     int32_t x = all;
 #pragma unroll
@@ -406,7 +406,7 @@ __device__ __forceinline__ int32_t pass_round(int32_t v, int lane, int LG) {
 template <class T, bool NARROW, int WIDTH>      // WIDTH 64: LG is 64, known to the compiler
 __global__ __launch_bounds__(256) void k_embedding_runs(const int32_t* __restrict__ key, const int32_t* __restrict__ pos, int64_t n,
                                                         int32_t V, const T* __restrict__ g, int64_t ldg, int D, float scale,
-                                                        T* __restrict__ dw, float* __restrict__ part, int C, int lanes, int64_t n_tiles) {
+                                                        T* __restrict__ dw, float* __restrict__ part, int C, int lanes) {
     constexpr int W = Piece<T>::W, U = 8;
     const int LG = WIDTH ? WIDTH : lanes;
     const int lane = threadIdx.x & (LG - 1);
@@ -709,7 +709,7 @@ extern "C" int bg_embedding_bwd(int dtype, const void* g, int64_t ldg, const voi
         const int64_t pieces = (D + Piece<T>::W - 1) / Piece<T>::W;
         const dim3 grid((unsigned)((p.run_tiles + 256 / p.LG - 1) / (256 / p.LG)), (unsigned)((pieces + p.LG - 1) / p.LG));
         const auto kernel = D < Piece<T>::W ? k_embedding_runs<T, true, 0> : p.LG == 64 ? k_embedding_runs<T, false, 64> : k_embedding_runs<T, false, 0>;
-        kernel<<<grid, 256, 0, s>>>(k, ps, n, (int32_t)V, gg, ldg, (int)D, scale, d, part, p.C, p.LG, p.run_tiles);
+        kernel<<<grid, 256, 0, s>>>(k, ps, n, (int32_t)V, gg, ldg, (int)D, scale, d, part, p.C, p.LG);
         BG_LAUNCH_CHECK();
         if (p.run_tiles > 1) {
             k_embedding_join<T><<<dim3((unsigned)p.run_tiles, (unsigned)((D + 255) / 256)), kJoin * kJoinCols, 0, s>>>(k, n, (int32_t)V, part,

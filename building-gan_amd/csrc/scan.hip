@@ -224,12 +224,6 @@ __device__ __forceinline__ void settle(Raw<T>& r) {
 #pragma unroll
     for (int i = 0; i < kRows; ++i) settle(r.v[i]);
 }
-__device__ __forceinline__ void settle(float (&v)[kRows][4]) {
-#pragma unroll
-    for (int i = 0; i < kRows; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) settle(v[i][e]);
-}
 template <bool CUTS>
 __device__ __forceinline__ void after(Map& m, const float (&A1)[4], const float (&B1)[4]) {          // m <- m o (A1, B1)
 #pragma unroll
