@@ -1207,6 +1207,7 @@ def gated_scan_step(x: torch.Tensor, gate: torch.Tensor, state: torch.Tensor, st
     n, D = x.shape
     x, gate, state = _rows(x), _rows(gate), _rows(state)
     h = torch.empty(n, D, dtype=x.dtype, device=x.device)
+    callers = state_out is not None
     if state_out is None:
         state_out = torch.empty(n, D, dtype=torch.float32, device=x.device)
     elif (state_out.shape != x.shape or state_out.dtype != torch.float32 or state_out.device != x.device
@@ -1216,6 +1217,8 @@ def gated_scan_step(x: torch.Tensor, gate: torch.Tensor, state: torch.Tensor, st
         raise _lib.BganError("gated_scan_step: state_out shares memory with an operand without being the same rows")
     check(lib.bg_gated_scan_step(code, x.data_ptr(), _ld(x), gate.data_ptr(), _ld(gate), state.data_ptr(), _ld(state), n, D, h.data_ptr(),
                                  max(D, 1), state_out.data_ptr(), _ld(state_out), stream()), "bg_gated_scan_step")
+    if callers:                                  # written through its address: a backward pass that still wants the old values
+        torch.autograd.graph.increment_version(state_out)        # (a scan that began with them) has to find out
     return h, state_out
 
 

@@ -824,3 +824,55 @@ def test_two_captured_graphs_replayed_at_once(cuda):
         torch.cuda.synchronize()
         for k, (_, outs, want, *_) in enumerate(sides):
             assert all(torch.equal(a, b) for a, b in zip(outs, want)), (r, k)
+
+
+# ------------------------------------------------------------------------------------------------ autograd around the calls
+@pytest.fixture
+def no_launch(monkeypatch):
+    """The wrappers on CPU tensors with every launch left out (results are whatever the memory held): what they do before and
+    after one.  Yields the calls made, as (entry point, arguments)."""
+    from building_gan_amd import _lib, ops
+    real, calls = _lib.load(), []
+
+    class Library:
+        def __getattr__(self, name):
+            if name in _lib._SIZES:
+                return getattr(real, name)
+            return lambda *a: calls.append((name, a)) or 0
+
+    monkeypatch.setattr(_lib, "load", Library)
+    monkeypatch.setattr(_lib, "require_device", lambda *a: None)
+    monkeypatch.setattr(_lib, "elsewhere", lambda t: False)
+    monkeypatch.setattr(ops, "stream", lambda: 0)
+    return calls
+
+
+def step_in_place_before_the_backward_pass(dev):
+    """States that a scan's backward pass will read are overwritten by a step: autograd has to notice."""
+    from building_gan_amd import ops
+    x = torch.ones(4, 8, device=dev, requires_grad=True)
+    state = torch.zeros(2, 8, device=dev)
+    h, _ = ops.gated_scan(x, torch.zeros(4, 8, device=dev), torch.tensor([0, 1, 4], dtype=torch.int32, device=dev), state)
+    row = torch.ones(2, 8, device=dev)
+    seen = state._version
+    ops.gated_scan_step(row, row, torch.zeros(2, 8, device=dev))             # states of its own: nothing of ours changes
+    assert state._version == seen
+    ops.gated_scan_step(row, row, state, state_out=state)
+    assert state._version > seen
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        h.sum().backward()
+    buf = torch.zeros(2, 24, device=dev)                                     # a view's base knows too
+    ops.gated_scan_step(row, row, torch.zeros(2, 8, device=dev), state_out=buf[:, 8:16])
+    assert buf._version > 0
+    with torch.inference_mode():
+        kept = torch.zeros(2, 8, device=dev)
+        assert ops.gated_scan_step(row, row, kept, state_out=kept)[1] is kept
+
+
+def test_step_in_place_is_seen_by_autograd(no_launch):
+    step_in_place_before_the_backward_pass(torch.device("cpu"))
+
+
+@pytest.mark.gpu
+def test_step_in_place_is_seen_by_autograd_on_the_gpu(cuda):
+    step_in_place_before_the_backward_pass(cuda)
