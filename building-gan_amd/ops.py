@@ -1192,8 +1192,8 @@ def _shifted_overlap(out: torch.Tensor, t: torch.Tensor) -> bool:
 
 def gated_scan_step(x: torch.Tensor, gate: torch.Tensor, state: torch.Tensor, state_out: Optional[torch.Tensor] = None):
     """One row for each of n segments whose states are kept between calls: (h [n, D] in x's type, state' [n, D] float32)
-    with ``state' = a state + (1 - a) x``; ``state_out=state`` updates the states in place (bg_gated_scan_step, no
-    autograd)."""
+    with ``state' = a state + (1 - a) x``; ``state_out=state`` updates the states in place (bg_gated_scan_step).  It has no
+    gradient, and says so where an operand wants one."""
     lib = _lib.load()
     _lib.require_device(x, "gated_scan_step")
     code = _elem(x, "gated_scan_step")
@@ -1201,6 +1201,9 @@ def gated_scan_step(x: torch.Tensor, gate: torch.Tensor, state: torch.Tensor, st
         raise _lib.BganError("gated_scan_step: x and gate must be [n, D] of one type")
     if state.shape != x.shape or state.dtype != torch.float32 or state.device != x.device:
         raise _lib.BganError(f"gated_scan_step: state must be float32 {tuple(x.shape)} on {x.device}")
+    if torch.is_grad_enabled() and (x.requires_grad or gate.requires_grad or state.requires_grad
+                                    or (state_out is not None and state_out.requires_grad)):
+        raise _lib.BganError("gated_scan_step has no gradient: call it under torch.no_grad(), or gated_scan for one")
     if _lib.elsewhere(x):
         with torch.cuda.device(x.device):
             return gated_scan_step(x, gate, state, state_out)

@@ -876,3 +876,29 @@ def test_step_in_place_is_seen_by_autograd(no_launch):
 @pytest.mark.gpu
 def test_step_in_place_is_seen_by_autograd_on_the_gpu(cuda):
     step_in_place_before_the_backward_pass(cuda)
+
+
+def steps_that_would_lose_a_gradient(dev):
+    from building_gan_amd import _lib, ops
+    plain = lambda: torch.zeros(3, 8, device=dev)
+    wants = lambda: torch.zeros(3, 8, device=dev, requires_grad=True)
+    for call in (lambda: ops.gated_scan_step(wants(), plain(), plain()), lambda: ops.gated_scan_step(plain(), wants(), plain()),
+                 lambda: ops.gated_scan_step(plain(), plain(), wants()),
+                 lambda: ops.gated_scan_step(plain(), plain(), plain(), state_out=wants())):
+        with pytest.raises(_lib.BganError, match="no gradient"):
+            call()
+        with torch.no_grad():
+            call()
+    kept = wants()
+    with torch.no_grad():
+        assert ops.gated_scan_step(plain(), plain(), kept, state_out=kept)[1] is kept
+    assert not ops.gated_scan_step(wants().detach(), plain(), plain())[0].requires_grad
+
+
+def test_step_refuses_operands_that_want_a_gradient(no_launch):
+    steps_that_would_lose_a_gradient(torch.device("cpu"))
+
+
+@pytest.mark.gpu
+def test_step_refuses_operands_that_want_a_gradient_on_the_gpu(cuda):
+    steps_that_would_lose_a_gradient(cuda)
