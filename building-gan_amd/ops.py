@@ -13,6 +13,7 @@ import threading
 from typing import List, Optional, Sequence
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import check, ptr, stream
@@ -990,6 +991,12 @@ def _embedding_backward(code, g, ids, n_rows, scale):
     return dw
 
 
+def _forward_mode() -> bool:
+    """Whether forward-mode derivatives are being taken.  A tensor's tangent does not show in ``requires_grad``, and a launcher
+    called past autograd drops it; a Function that is applied raises NotImplementedError for it."""
+    return getattr(forward_ad, "_current_level", 0) >= 0
+
+
 class Embedding(torch.autograd.Function):
     """y = scale * weight[ids]; the backward is EmbeddingGrad (both are linear, so the pair is closed)."""
 
@@ -1032,7 +1039,7 @@ def embedding(weight: torch.Tensor, ids: torch.Tensor, scale: float = 1.0, valid
         lo, hi = (int(v) for v in torch.stack(torch.aminmax(ids)).tolist())
         if lo < 0 or hi >= weight.shape[0]:
             raise IndexError(f"embedding: ids span [{lo}, {hi}], the table has {weight.shape[0]} rows")
-    if torch.is_grad_enabled() and weight.requires_grad:
+    if (torch.is_grad_enabled() and weight.requires_grad) or _forward_mode():
         return Embedding.apply(weight, ids, float(scale))
     return embedding_raw(weight, ids, float(scale))
 
@@ -1169,7 +1176,7 @@ def gated_scan(x: torch.Tensor, gate: torch.Tensor, rowptr: Optional[torch.Tenso
             rowptr = torch.zeros(shape[0] + 1, dtype=torch.int32, device=x.device)
     elif rowptr is None:
         rowptr = 1 if x.dim() == 2 and x.shape[0] else torch.zeros(2, dtype=torch.int32, device=x.device)
-    if torch.is_grad_enabled() and (x.requires_grad or gate.requires_grad or (h0 is not None and h0.requires_grad)):
+    if (torch.is_grad_enabled() and (x.requires_grad or gate.requires_grad or (h0 is not None and h0.requires_grad))) or _forward_mode():
         h, h_last = GatedScan.apply(x, gate, h0, rowptr, bool(reverse))
     else:
         h, h_last, _ = gated_scan_raw(x, gate, rowptr, h0, bool(reverse))

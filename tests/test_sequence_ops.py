@@ -902,3 +902,28 @@ def test_step_refuses_operands_that_want_a_gradient(no_launch):
 @pytest.mark.gpu
 def test_step_refuses_operands_that_want_a_gradient_on_the_gpu(cuda):
     steps_that_would_lose_a_gradient(cuda)
+
+
+def forward_mode_calls(dev):
+    """Forward-mode derivatives are not offered: an operand's tangent is an error, never a result without one."""
+    import torch.autograd.forward_ad as fw
+    from building_gan_amd import ops
+    w, ids, h0 = torch.ones(4, 8, device=dev), torch.tensor([0, 3], device=dev), torch.zeros(1, 8, device=dev)
+    with fw.dual_level():
+        d, d0 = fw.make_dual(w, torch.ones_like(w)), fw.make_dual(h0, torch.ones_like(h0))
+        for grad in (True, False):
+            with torch.set_grad_enabled(grad):
+                for call in (lambda: ops.embedding(d, ids), lambda: ops.gated_scan(d, w), lambda: ops.gated_scan(w, d),
+                             lambda: ops.gated_scan(w, w, None, d0), lambda: ops.gated_scan(d.view(2, 2, 8), w.view(2, 2, 8))):
+                    with pytest.raises(RuntimeError):
+                        call()
+                assert ops.embedding(w, ids).shape == (2, 8) and ops.gated_scan(w, w, None, h0)[0].shape == (4, 8)     # no tangent
+
+
+def test_operands_with_tangents_are_refused(no_launch):
+    forward_mode_calls(torch.device("cpu"))
+
+
+@pytest.mark.gpu
+def test_operands_with_tangents_are_refused_on_the_gpu(cuda):
+    forward_mode_calls(cuda)
