@@ -1009,7 +1009,7 @@ class Embedding(torch.autograd.Function):
     @staticmethod
     def backward(ctx, g):
         (ids,) = ctx.saved_tensors
-        if torch.is_grad_enabled():                      # create_graph asked for it
+        if torch.is_grad_enabled() or _forward_mode():   # create_graph asked for it, or g may have a tangent
             return EmbeddingGrad.apply(g, ids, ctx.n_rows, ctx.scale), None, None
         # (checked by the forward call; autograd runs this on the weight's device)
         return _embedding_backward(_ELEM[g.dtype], g, ids if ids.is_contiguous() else ids.contiguous(), ctx.n_rows, ctx.scale), None, None
@@ -1146,6 +1146,8 @@ class GatedScan(torch.autograd.Function):
     def backward(ctx, dh, dlast):
         if dh is None and dlast is None:
             return None, None, None, None, None
+        if _forward_mode() and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in (dh, dlast)):
+            raise NotImplementedError("gated_scan's backward pass has no forward-mode derivative")
         x, gate, h0, rp, heads = ctx.saved_tensors      # (checked by the forward call; autograd runs this on x's device)
         dx, dgate, dh0 = _scan_backward(_ELEM[x.dtype], _rows(x), _rows(gate), None if rp is None else rp.contiguous(), ctx.n_seg,
                                         None if h0 is None else h0.contiguous(), ctx.reverse, heads, dh, dlast, ctx.needs_input_grad[2])

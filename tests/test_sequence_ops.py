@@ -927,3 +927,30 @@ def test_operands_with_tangents_are_refused(no_launch):
 @pytest.mark.gpu
 def test_operands_with_tangents_are_refused_on_the_gpu(cuda):
     forward_mode_calls(cuda)
+
+
+def forward_over_reverse(dev):
+    """The cotangent of a backward pass may carry a tangent too (a Hessian's product with a vector taken that way)."""
+    import torch.autograd.forward_ad as fw
+    from building_gan_amd import ops
+    w, ids = torch.ones(4, 8, device=dev, requires_grad=True), torch.tensor([0, 3], device=dev)
+    dual = lambda *s: fw.make_dual(torch.ones(*s, device=dev), torch.ones(*s, device=dev))
+    with fw.dual_level():
+        out = ops.embedding(w, ids)
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(out, w, dual(2, 8), retain_graph=True)
+        assert torch.autograd.grad(out, w, torch.ones(2, 8, device=dev))[0].shape == (4, 8)
+        h, last = ops.gated_scan(w, w.detach())
+        for outs, grads in ((h, dual(4, 8)), (last, dual(1, 8)), ((h, last), (torch.ones(4, 8, device=dev), dual(1, 8)))):
+            with pytest.raises(RuntimeError):
+                torch.autograd.grad(outs, w, grads, retain_graph=True)
+        assert torch.autograd.grad((h, last), w, (torch.ones(4, 8, device=dev), torch.ones(1, 8, device=dev)))[0].shape == (4, 8)
+
+
+def test_cotangents_with_tangents_are_refused(no_launch):
+    forward_over_reverse(torch.device("cpu"))
+
+
+@pytest.mark.gpu
+def test_cotangents_with_tangents_are_refused_on_the_gpu(cuda):
+    forward_over_reverse(cuda)
