@@ -1185,13 +1185,15 @@ def gated_scan(x: torch.Tensor, gate: torch.Tensor, rowptr: Optional[torch.Tenso
     return (h if h.shape == shape else h.view(shape)), h_last
 
 
-def _shifted_overlap(out: torch.Tensor, t: torch.Tensor) -> bool:
-    """Whether two [n, D] matrices of contiguous rows share memory without holding every element at the same address."""
-    eo, et = out.element_size(), t.element_size()
-    if out.numel() == 0 or (out.data_ptr() == t.data_ptr() and out.stride() == t.stride() and eo == et):
+def _shifted_overlap(out: torch.Tensor, t: torch.Tensor, same_rows: bool = True) -> bool:
+    """Whether two [n, D] matrices of contiguous rows share memory; not, with ``same_rows``, where they hold every element at the
+    same address."""
+    if out.numel() == 0:
         return False
-    (n, D), a, b = out.shape, out.data_ptr(), t.data_ptr()
-    po, pt = eo * (out.stride(0) if n > 1 else D), et * (t.stride(0) if n > 1 else D)
+    (n, D), a, b, eo, et = out.shape, out.data_ptr(), t.data_ptr(), out.element_size(), t.element_size()
+    po, pt = eo * _ld(out), et * _ld(t)
+    if a == b and po == pt and eo == et:
+        return not same_rows
     if a >= b + pt * (n - 1) + et * D or b >= a + po * (n - 1) + eo * D:
         return False
     if po != pt:
@@ -1225,8 +1227,8 @@ def gated_scan_step(x: torch.Tensor, gate: torch.Tensor, state: torch.Tensor, st
     elif (state_out.shape != x.shape or state_out.dtype != torch.float32 or state_out.device != x.device
           or _rows(state_out) is not state_out):
         raise _lib.BganError(f"gated_scan_step: state_out must be float32 {tuple(x.shape)} with contiguous rows on {x.device}")
-    elif any(_shifted_overlap(state_out, t) for t in (state, x, gate)):
-        raise _lib.BganError("gated_scan_step: state_out shares memory with an operand without being the same rows")
+    elif _shifted_overlap(state_out, state) or _shifted_overlap(state_out, x, False) or _shifted_overlap(state_out, gate, False):
+        raise _lib.BganError("gated_scan_step: state_out shares memory with x or gate, or with other rows of state")
     check(lib.bg_gated_scan_step(code, x.data_ptr(), _ld(x), gate.data_ptr(), _ld(gate), state.data_ptr(), _ld(state), n, D, h.data_ptr(),
                                  max(D, 1), state_out.data_ptr(), _ld(state_out), stream()), "bg_gated_scan_step")
     if callers:                                  # written through its address: a backward pass that still wants the old values

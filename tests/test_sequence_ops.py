@@ -954,3 +954,28 @@ def test_cotangents_with_tangents_are_refused(no_launch):
 @pytest.mark.gpu
 def test_cotangents_with_tangents_are_refused_on_the_gpu(cuda):
     forward_over_reverse(cuda)
+
+
+def test_overlap_of_a_step_s_state_and_rows(no_launch):
+    """The states may be written where they stand, an operand's rows may not; and the pitch of a single row means nothing."""
+    from building_gan_amd import _lib, ops
+    x, gate, state = torch.zeros(3, 8), torch.zeros(3, 8), torch.zeros(3, 8)
+    for out in (x, gate):
+        with pytest.raises(_lib.BganError, match="shares memory"):
+            ops.gated_scan_step(x, gate, state, state_out=out)
+    for same in (x, gate):                                                   # written as states, read as rows
+        with pytest.raises(_lib.BganError, match="shares memory"):
+            ops.gated_scan_step(x, gate, same, state_out=same)
+    assert ops.gated_scan_step(x, gate, state, state_out=state)[1] is state
+    buf = torch.zeros(2, 32)
+    row, again = buf[:1, :16], buf.as_strided((1, 16), (16, 1))              # the same row, told in two ways
+    assert row.stride() != again.stride()
+    one = torch.zeros(1, 16)
+    ops.gated_scan_step(one, one, row, state_out=again)
+    ops.gated_scan_step(one, one, again, state_out=row)
+    with pytest.raises(_lib.BganError, match="shares memory"):
+        ops.gated_scan_step(one, one, row, state_out=buf.as_strided((1, 16), (16, 1), 8))
+    with pytest.raises(_lib.BganError, match="shares memory"):
+        ops.gated_scan_step(again, one, one, state_out=row)
+    tall = buf.view(64, 1)                                                   # a single column: its inner stride means nothing
+    ops.gated_scan_step(torch.zeros(64, 1), torch.zeros(64, 1), tall, state_out=buf.as_strided((64, 1), (1, 7)))
