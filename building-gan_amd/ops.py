@@ -1045,6 +1045,14 @@ def embedding(weight: torch.Tensor, ids: torch.Tensor, scale: float = 1.0, valid
 
 
 # ------------------------------------------------------------------------------- scan along segments
+_SCAN_PITCH = 1 << 21      # the farthest rows whose offsets in a tile are 32-bit (include/bgan.h)
+
+
+def _scan_rows(t: torch.Tensor) -> torch.Tensor:
+    t = _rows(t)
+    return t.contiguous() if _ld(t) > _SCAN_PITCH else t
+
+
 def _scan_operands(x, gate, rowptr, h0, what):
     """(type code, x, gate, row pointer, segments, h0) as bg_gated_scan_* take them; BganError for what they do not take."""
     code = _elem(x, what)
@@ -1065,7 +1073,7 @@ def _scan_operands(x, gate, rowptr, h0, what):
         if h0.dtype != torch.float32 or h0.device != x.device or tuple(h0.shape) != (n_seg, x.shape[1]):
             raise _lib.BganError(f"{what}: h0 must be float32 [{n_seg}, {x.shape[1]}] on {x.device}, got {h0.dtype} {tuple(h0.shape)}")
         h0 = h0.contiguous()
-    return code, _rows(x), _rows(gate), rowptr, n_seg, h0
+    return code, _scan_rows(x), _scan_rows(gate), rowptr, n_seg, h0
 
 
 @functools.lru_cache(maxsize=1024)
@@ -1116,7 +1124,7 @@ def gated_scan_grad_raw(x, gate, rowptr, h0, reverse: bool, heads, dh, dlast, ne
 def _scan_backward(code, x, gate, rp, n_seg, h0, reverse, heads, dh, dlast, need_dh0):
     lib = _lib.load()
     (N, D), dev = x.shape, x.device
-    dh = None if dh is None else _rows(dh)
+    dh = None if dh is None else _scan_rows(dh)
     dlast = None if dlast is None else dlast.contiguous()
     dx = torch.empty(N, D, dtype=x.dtype, device=dev)
     dgate = torch.empty(N, D, dtype=x.dtype, device=dev)
@@ -1149,8 +1157,9 @@ class GatedScan(torch.autograd.Function):
         if _forward_mode() and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in (dh, dlast)):
             raise NotImplementedError("gated_scan's backward pass has no forward-mode derivative")
         x, gate, h0, rp, heads = ctx.saved_tensors      # (checked by the forward call; autograd runs this on x's device)
-        dx, dgate, dh0 = _scan_backward(_ELEM[x.dtype], _rows(x), _rows(gate), None if rp is None else rp.contiguous(), ctx.n_seg,
-                                        None if h0 is None else h0.contiguous(), ctx.reverse, heads, dh, dlast, ctx.needs_input_grad[2])
+        dx, dgate, dh0 = _scan_backward(_ELEM[x.dtype], _scan_rows(x), _scan_rows(gate), None if rp is None else rp.contiguous(),
+                                        ctx.n_seg, None if h0 is None else h0.contiguous(), ctx.reverse, heads, dh, dlast,
+                                        ctx.needs_input_grad[2])
         return dx, dgate, dh0, None, None
 
 

@@ -979,3 +979,42 @@ def test_overlap_of_a_step_s_state_and_rows(no_launch):
         ops.gated_scan_step(again, one, one, state_out=row)
     tall = buf.view(64, 1)                                                   # a single column: its inner stride means nothing
     ops.gated_scan_step(torch.zeros(64, 1), torch.zeros(64, 1), tall, state_out=buf.as_strided((64, 1), (1, 7)))
+
+
+def far_rows(dev, n=5, D=8, pitch=(1 << 21) + 4):
+    buf = torch.zeros(n, pitch, device=dev)
+    gen = torch.Generator().manual_seed(0)
+    for k in (0, D, 2 * D):
+        buf[:, k:k + D] = torch.randn(n, D, generator=gen).to(dev)
+    return buf[:, :D], buf[:, D:2 * D], buf[:, 2 * D:3 * D]
+
+
+def test_far_rows_are_copied_before_a_scan(no_launch):
+    """Rows farther apart than a tile's 32-bit offsets reach: the entry points refuse such a pitch, so the wrappers copy."""
+    from building_gan_amd import ops
+    x, gate, dh = far_rows(torch.device("cpu"))
+    x, gate = x.detach().requires_grad_(True), gate.detach().requires_grad_(True)
+    h, _ = ops.gated_scan(x, gate)
+    torch.autograd.grad(h, (x, gate), dh)
+    ops.gated_scan_grad_raw(x.detach(), gate.detach(), 1, None, False, torch.zeros(ops._scan_sizes(5, 8)[0]), dh, None)
+    (f, fa), (b, ba), (r, ra) = no_launch
+    assert f == "bg_gated_scan_fwd" and b == r == "bg_gated_scan_bwd"
+    assert [fa[2], fa[4]] == [8, 8] and [ba[2], ba[4], ba[6]] == [ra[2], ra[4], ra[6]] == [8, 8, 8]      # the pitches
+
+
+@pytest.mark.gpu
+def test_far_rows_are_scanned(cuda):
+    from building_gan_amd import ops
+    x, gate, dh = far_rows(cuda)
+    near = [t.contiguous() for t in (x, gate, dh)]
+    out = []
+    for xx, gg, dd in ((x, gate, dh), near):
+        xx, gg = xx.detach().requires_grad_(True), gg.detach().requires_grad_(True)
+        h, last = ops.gated_scan(xx, gg)
+        out.append((h, last) + torch.autograd.grad(h, (xx, gg), dd))
+    assert all(torch.equal(a, b) for a, b in zip(*out))
+    state = torch.zeros(5, 8, device=cuda)
+    assert torch.equal(ops.gated_scan_step(x, gate, state)[1], ops.gated_scan_step(near[0], near[1], state)[1])
+    ids = torch.tensor([0, 4, 2, 1, 3], device=cuda)
+    assert torch.equal(ops.embedding(x, ids), near[0][ids])
+    assert torch.equal(ops.embedding_grad_raw(x, ids, 30), ops.embedding_grad_raw(near[0], ids, 30))
