@@ -1018,3 +1018,25 @@ def test_far_rows_are_scanned(cuda):
     ids = torch.tensor([0, 4, 2, 1, 3], device=cuda)
     assert torch.equal(ops.embedding(x, ids), near[0][ids])
     assert torch.equal(ops.embedding_grad_raw(x, ids, 30), ops.embedding_grad_raw(near[0], ids, 30))
+
+
+# ------------------------------------------------------------------------------------------------ every variant of the sort, equal segments
+@pytest.mark.gpu
+@pytest.mark.parametrize("ids_dtype", [torch.int64, torch.int32])
+@pytest.mark.parametrize("V", [21, 700, 300000])                                 # one, two and three passes over the keys
+@pytest.mark.parametrize("n", [4096, 4097, 65536, 65537, 131072, 131073, 200001, 262144, 262145])
+def test_lookup_gradient_at_the_borders_of_the_sort(cuda, n, V, ids_dtype):
+    """Token counts at which the sort takes another form: one workgroup; 2, 4 and 8 keys a lane; the tiles' counts added up by
+    every workgroup, and scanned from 64 tiles on.  Sums of small whole numbers: exact in any order."""
+    from building_gan_amd import ops
+    gen = torch.Generator().manual_seed(n + V)
+    ids = torch.randint(0, V, (n,), generator=gen)
+    ids[torch.rand(n, generator=gen) < 0.3] = V // 3                         # a run over many tiles of slots
+    ids[torch.rand(n, generator=gen) < 0.1] = -1
+    ids[0], ids[n - 1], ids[n // 2] = V - 1, V - 1, V                        # the ends of the order, a missing token
+    g = torch.randint(-3, 4, (n, 8), generator=gen).float()
+    there = (ids >= 0) & (ids < V)
+    want = torch.zeros(V, 8, dtype=torch.float64).index_add_(0, ids[there], g[there].double()) * 0.5
+    for dtype in (torch.float32, torch.bfloat16):
+        got = ops.embedding_grad_raw(g.to(cuda).to(dtype), ids.to(cuda).to(ids_dtype), V, 0.5)
+        assert torch.equal(got.cpu(), want.to(dtype)), (dtype, int((got.cpu() != want.to(dtype)).sum()))
