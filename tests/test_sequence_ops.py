@@ -1040,3 +1040,21 @@ def test_lookup_gradient_at_the_borders_of_the_sort(cuda, n, V, ids_dtype):
     for dtype in (torch.float32, torch.bfloat16):
         got = ops.embedding_grad_raw(g.to(cuda).to(dtype), ids.to(cuda).to(ids_dtype), V, 0.5)
         assert torch.equal(got.cpu(), want.to(dtype)), (dtype, int((got.cpu() != want.to(dtype)).sum()))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("reverse", [False, True])
+@pytest.mark.parametrize("B,T,D", [(6, 77, 24), (1, 300, 12), (40, 1, 8), (3, 1001, 68), (9, 128, 64)])
+def test_scan_of_a_batch_and_its_gradients(cuda, B, T, D, reverse, dtype):
+    """[B, T, D] has no row pointer: values and gradients against float64 through the row pointer, and bit for bit alike."""
+    from building_gan_amd import ops
+    ptr = list(range(0, B * T + 1, T))
+    c = scan_case(B * T, D, ptr, dtype, B + T)
+    want = check_scan(cuda, c, ptr, reverse)
+    z, h0 = c["z"].to(cuda).view(B, T, 2 * D).requires_grad_(True), c["h0"].to(cuda).requires_grad_(True)
+    h, last = ops.gated_scan(z[..., :D], z[..., D:], None, h0, reverse)
+    dz, d0 = torch.autograd.grad((h, last), (z, h0), (c["dh"].to(cuda).view(B, T, D), c["dlast"].to(cuda)))
+    got = (h.reshape(B * T, D), last, dz[..., :D].reshape(B * T, D), dz[..., D:].reshape(B * T, D), d0)
+    for name, a, b in zip(("h", "h_last", "dx", "dgate", "dh0"), got, want):
+        assert torch.equal(a, b), name
