@@ -2,9 +2,9 @@
 //
 // The gradient of a table of a few rows sums into tables in LDS, one for every group of lanes that walks over rows.  That of
 // a larger one sorts the token ids (stable radix sort on (id, position) pairs) and sums the rows of g in sorted order: the
-// occurrences of one token become one RUN of neighbouring slots.  Slots are cut into tiles of equal length, so the work is
-// even however often a token occurs; a run inside one tile is finished there, a run over several tiles leaves one fp32
-// partial row per tile and a second launch joins them.  No floating-point atomics: the order of every sum depends on the
+// occurrences of one token become one RUN of neighbouring slots.  Slots are cut into tiles of equal length, so the reading of g
+// is even however often a token occurs; a run inside one tile is finished there, a run over several tiles leaves one fp32
+// partial row per tile and a second launch joins them, a workgroup for each run and 256 columns (slow for a run of very many).  No floating-point atomics: the order of every sum depends on the
 // sizes and the ids alone.
 #include "common.h"
 
@@ -462,7 +462,9 @@ __global__ __launch_bounds__(256) void k_embedding_runs(const int32_t* __restric
 
 // The run that begins in tile blockIdx.x and goes on: its own partial and the following tiles' are added by kJoin threads a
 // column (strided over the tiles), those kJoin sums then in order.  Latency: the search for a long run's end and the walk
-// over its tiles (7.6 us where a fifteenth of 16,384 tokens are one; two threads a column measured best of 2, 4, 8, 16).
+// over its tiles (7.6 us where a fifteenth of 16,384 tokens are one, some 70 tiles; two threads a column measured best of 2, 4,
+// 8, 16 there).  The walk grows with the longest run: 1,048,576 x 64 fp32 of 100 rows 11 us with even ones, 79 us where a
+// fifth of the tokens are one (1,638 tiles), 350 us where all are (8,192), beside 42 to 52 us for the sums themselves.
 constexpr int kJoin = 2, kJoinCols = 64;
 template <class T>
 __global__ __launch_bounds__(kJoin* kJoinCols) void k_embedding_join(const int32_t* __restrict__ key, int64_t n, int32_t V,

@@ -1,6 +1,6 @@
 // Gated linear recurrence along the rows of each segment, a scan over long sequences, and its backward pass.
 //
-//   a = sigmoid(gate), c = 1 - a = sigmoid(-gate)          (both from one exponential, each to full relative accuracy)
+//   a = sigmoid(gate), c = 1 - a = sigmoid(-gate)          (both from one exponential, each with a relative error of a few units)
 //   forward :  h_t = a_t h_{t-1} + c_t x_t                 h before a segment's first row = h0 (or 0)
 //   backward:  mu_t = a_t (dh_t + mu_{t+1})                mu after a segment's last row = dlast (or 0)
 //              dx_t = c_t (dh_t + mu_{t+1}),  dgate_t = (dh_t + mu_{t+1}) (h_{t-1} - x_t) a_t c_t,  dh0 = mu_first
@@ -94,10 +94,11 @@ __device__ __forceinline__ void settle(float& v) { asm volatile("" : "+v"(v)); }
 
 // a = sigmoid(g), c = sigmoid(-g) without cancellation: with e = exp(-|g|) <= 1 the smaller one is e / (1 + e), at most 1/2, and
 // the larger one is 1 minus it, which is exact to its own rounding: a memory that is long because its a's are near 1 adds up no
-// one-sided errors of the reciprocal.  What the rounding of |g| log2(e) leaves out is put back (e * (1 + rest)).
+// one-sided errors of the reciprocal.  What the rounding of |g| log2(e) leaves out is put back (e * (1 + rest)).  The hardware's
+// exponential makes no subnormal numbers: from |g| = 87.4 on the smaller one is 0 (it would be 1.1e-38) and the larger one 1.
 // Packed, both are one register: the smaller one with the sign of the gate.
 __device__ __forceinline__ float pack_gate(float g) {
-    const float m = __builtin_elementwise_minimum(fabsf(g), 110.f);      // e^-110 is 0 in fp32; a NaN stays one
+    const float m = __builtin_elementwise_minimum(fabsf(g), 110.f);      // (an inf gives no NaN below; a NaN stays one)
     const float p = m * -1.4426950408889634f;
     float e = __builtin_amdgcn_exp2f(p);
     e = fmaf(e, fmaf(p, -0.6931471805599453f, -m), e);
@@ -329,8 +330,8 @@ __device__ __forceinline__ void await_words(const uint64_t* p, int n, uint64_t (
 }
 
 // What enters tile number `k` of the walk, by two waves at once, a lane for each column (a look at another workgroup's word
-// takes about a microsecond, and the two levels would be two looks after one another: 16,384 x 2,048 bf16 backward 120 us, with
-// two waves 115 us).  The first wave publishes the tile's map (ownA, ownB) and composes the maps of its group's tiles before it ..
+// takes about a microsecond, and the two levels would be two looks after one another: worth 5 us of 120 at 16,384 x 2,048 bf16
+// backward, when that pass had two waves a SIMD).  The first wave publishes the tile's map (ownA, ownB) and composes the maps of its group's tiles before it ..
 __device__ __forceinline__ void enter_group(const Chain& ch, uint32_t k, uint32_t cb, uint32_t col, float oA, float oB, float& A, float& B) {
     const int p = (int)(k % kGroup), gp = (int)(k / kGroup % kGroup);
     uint64_t *tiles = ch.tile + ((int64_t)(k / kGroup) * ch.ncb + cb) * (kGroup * kMaxCols) + col;
@@ -368,8 +369,8 @@ __device__ __forceinline__ float enter_block(const Chain& ch, uint32_t k, uint32
 // The next (tile, column block) in the order of the walk; with a single tile there is nothing to order.  false: none left
 // (a ticket that another call's workgroups also draw from).  A counter answers about once in 17 ns, so workgroups that start
 // together wait for it: 1,024 of the forward pass for 17 us, 768 of the backward pass for 13 us.  So the column blocks are
-// dealt out to up to 8 counters, each on a cache line of its own (16,384 x 2,048 bf16 forward 58 us, 74 us with one counter,
-// backward 108 and 113 us; 262,144 x 512 bf16 forward 235 and 246 us; no difference where memory is the bound).
+// dealt out to up to 8 counters, each on a cache line of its own (16,384 x 2,048 bf16 forward 58 us, 73 us with one counter,
+// backward 93 and 96 us; 262,144 x 512 bf16 forward 235 and 245 us, backward 336 and 335 us; 100,003 x 333 forward 86 and 94 us).
 constexpr uint32_t kTickets = 8, kTicketStep = 32, kXcds = 8;
 __device__ __forceinline__ bool take_tile(const Chain& ch, int64_t n_tiles, int64_t& tile, int& cb) {
     __shared__ uint32_t ticket;
@@ -545,8 +546,12 @@ __device__ __forceinline__ void leave_row(const Borders& w, int i, const TileSha
 // x and gate are read once, h (and an eighth of it in fp32) written once.  fp32 rows are bound by memory: 1,048,576 x 128
 // 332 us, 4.85 TB/s, what a copy of 4 GiB reaches (4.81).  16-bit rows carry half the bytes for the same arithmetic, about
 // 33 instructions an element: 262,144 x 512 bf16 230 us (3.5 TB/s), of which the SIMDs issue for half; without the look-back
-// the same rows took 186 us, what remains of it is a tile's wait of some 3 us that four waves a SIMD do not hide.  The
-// bound of 128 registers (four waves instead of three) was worth 273 -> 247 us there; five would take spills.
+// the same rows took 186 us, what remains of it is a tile's wait of some 3 us that four waves a SIMD do not hide.  Rows that
+// begin at any address are read almost twice (100,003 x 333 fp16: 262 MB for 133), but that is not what they cost: at a pitch of
+// 384 it is 165 MB and the same 95 us.  The last column block is: 320 columns take 67 us, so its 13 columns cost as much as two
+// full blocks.  In narrow rows a load instruction of a wave touches 16 pieces of 32 bytes, 256 bytes apart: 1,048,576 x 16 bf16
+// 52 us where its 110 MB would take 23.  The bound of 128 registers (four waves instead of three) was worth 273 -> 247 us at
+// 262,144 x 512 bf16; five would take spills.
 template <class T, bool REV>
 __global__ __launch_bounds__(kThreads, 4) void k_scan_fwd(const T* __restrict__ x, int64_t ldx, const T* __restrict__ gate, int64_t ldg, Segs g,
                                                        int64_t D, const float* __restrict__ h0, int CG, Chain ch, int64_t n_tiles,

@@ -152,7 +152,8 @@ int bg_embedding_bwd(int dtype, const void* g, int64_t ldg, const void* ids, int
  * `dtype`, row pitches in elements; h0, h_last: fp32 [n_seg, D], contiguous.  h_last (may be NULL) receives the state
  * after a segment's rows; a segment without rows passes h0 through.  Rows in no segment (before rowptr[0], from
  * rowptr[n_seg] on) are zero in h.  rowptr: int32 [n_seg + 1], non-decreasing; entries outside [0, n_rows] are taken as
- * the nearer end.  rowptr NULL: n_seg segments of n_rows / n_seg rows each.  The state is fp32; h is rounded once.
+ * the nearer end.  rowptr NULL: n_seg segments of n_rows / n_seg rows each.  The state is fp32; h is rounded once; an a or
+ * 1 - a below the smallest normal fp32 number (|gate| > 87.3) counts as 0.
  * heads (may be NULL): fp32 [bg_gated_scan_heads(n_rows, D)], the state before every eighth row, which the
  * backward pass takes.  ws: bg_gated_scan_workspace(n_rows, D) bytes, 16-byte aligned (BG_ERR_SCRATCH when ws_bytes is
  * less); it needs no preparation, and no two calls at once may have the same.  Any alignment and pitch of x, gate and h

@@ -4,10 +4,13 @@ Tolerances.  u = 2^-24 is half a step of fp32, ``half(t)`` half a step of the el
 to the type once.
  * lookup: one product and one rounding of the scale to fp32 (2 u) and the rounding to the type.
  * lookup gradient: m terms added in fp32 in some order: m u sum|g|, then the scale (2 u) and the rounding.
- * a = sigmoid(g) and c = sigmoid(-g) come from exp2 and a reciprocal (1 ulp = 2 u each) with a compensated argument:
-   e within 4 u, 1 / (1 + e) within 5 u, e / (1 + e) within 10 u.  One step of the recurrence adds at most 12 u of
-   a |h| + c |x|, and what a step has wrong decays with the a's behind it: ``err_t = a_t err_{t-1} + 12 u (a |h| + c |x|)``.
-   Joining row groups, tiles and slices of tiles (at most 32 + 32 + tiles / 32 joins, factors at most 1) adds 2 u max|h| each.
+ * a = sigmoid(g) and c = sigmoid(-g): with e = exp(-|g|) the smaller one is e / (1 + e), from exp2 and a reciprocal (1 ulp = 2 u
+   each) with a compensated argument: e within 4 u, of which e / (1 + e) takes half to all, then a sum, a reciprocal and a
+   product: within 8 u (6 u where both are 1/2).  The larger one is 1 minus it: within 7 u.  (Below the smallest normal number,
+   behind |g| = 87.3, the smaller one is 0.)  One step of the recurrence adds at most 12 u of a |h| + c |x| (8 u and two
+   roundings), and what a step has wrong decays with the a's behind it: ``err_t = a_t err_{t-1} + 12 u (a |h| + c |x|)``.
+   Joining row groups, waves, 8 tiles to a group, 8 groups to a block and block to block (at most 24 + tiles / 64 joins of
+   tiles of 128 rows and more, factors at most 1; the bound takes 64 + rows / (32 * 128)) adds 2 u max|h| each.
  * the backward recurrence alike, with the sums of |terms| in the place of |h|; dx and dgate multiply a few factors each
    known to the errors above.
 """
@@ -341,6 +344,7 @@ def test_scan_without_optional_operands(cuda, h0, use_dh, use_dlast):
     check_scan(cuda, c, RAGGED, use_dh=use_dh, use_dlast=use_dlast)
 
 
+# Values only, and the comparison for B == 1 never runs: test_scan_of_a_batch_and_its_gradients has both.
 @pytest.mark.gpu
 @pytest.mark.parametrize("reverse", [False, True])
 def test_scan_of_equal_segments_and_batches(cuda, reverse):
@@ -385,6 +389,7 @@ def test_scan_of_nothing(cuda):
     assert not h.any() and hl.shape == (0, 8)
 
 
+# (What takes two rounds is the marking of a tile's borders, a lane for each segment; its first segment is found by bisection.)
 @pytest.mark.gpu
 @pytest.mark.parametrize("reverse", [False, True])
 def test_scan_with_many_segments(cuda, reverse):
@@ -654,6 +659,7 @@ def test_step_into_another_half_of_the_same_buffer(cuda):
         ops.gated_scan_step(buf[:6, :32], x[:6], x[:6], state_out=buf[1:, :32])
 
 
+# (4,096 is where one workgroup no longer sorts alone, 8,192 no border; the later ones: test_lookup_gradient_at_the_borders_of_the_sort)
 @pytest.mark.gpu
 @pytest.mark.parametrize("V,D,n,kind", [(7, 3, 5000, "uniform"), (20, 1, 999, "hot"), (5, 2, 70000, "missing"), (20, 132, 4097, "missing"),
                                         (21, 132, 4097, "missing"), (5000, 16, 4096, "uniform"), (5000, 16, 4097, "hot"),
