@@ -1064,3 +1064,185 @@ def test_scan_of_a_batch_and_its_gradients(cuda, B, T, D, reverse, dtype):
     got = (h.reshape(B * T, D), last, dz[..., :D].reshape(B * T, D), dz[..., D:].reshape(B * T, D), d0)
     for name, a, b in zip(("h", "h_last", "dx", "dgate", "dh0"), got, want):
         assert torch.equal(a, b), name
+
+
+# ------------------------------------------------------------------------------------------------ calls the limits and the header allow
+@pytest.mark.gpu
+@pytest.mark.parametrize("reverse", [False, True])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_scan_at_the_largest_pitch(cuda, dtype, reverse):
+    """Rows 2^21 elements apart, in tiles of 512 rows: offsets in a tile up to 4 * 511 * 2^21 bytes, just under 2^32."""
+    from building_gan_amd import ops
+    N, D, P = 530, 16, 1 << 21
+    gen = torch.Generator().manual_seed(3)
+    near = [torch.randn(N, D, generator=gen).to(dtype).to(cuda) for _ in range(3)]
+    buf = torch.empty(N, P, dtype=dtype, device=cuda)
+    far = [buf[:, 16 * k:16 * k + D] for k in range(3)]
+    for a, b in zip(far, near):
+        a.copy_(b)
+    ptr = torch.tensor([0, 100, 519, 530], dtype=torch.int32, device=cuda)
+    outs = []
+    for x, gate, dh in (far, near):
+        h, last, heads = ops.gated_scan_raw(x, gate, ptr, None, reverse, keep_heads=True)
+        outs.append((h, last) + ops.gated_scan_grad_raw(x, gate, ptr, None, reverse, heads, dh, None))
+    assert all(torch.equal(a, b) for a, b in zip(*outs))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_widest_rows(cuda, dtype):
+    """2^15 columns of a table, by few rows and sorted, and 2^20 columns of a scan."""
+    from building_gan_amd import ops
+    gen = torch.Generator().manual_seed(1)
+    for V in (20, 23):
+        w = torch.randint(-4, 5, (V, 1 << 15), generator=gen).to(dtype).to(cuda)
+        ids = torch.randint(-1, V + 1, (37,), generator=gen)
+        g = torch.randint(-4, 5, (37, 1 << 15), generator=gen).to(dtype).to(cuda)
+        there = (ids >= 0) & (ids < V)
+        want = torch.zeros(37, 1 << 15, dtype=dtype)
+        want[there] = w.cpu()[ids[there]]
+        assert torch.equal(ops.embedding(w, ids.to(cuda)).cpu(), want)
+        want = torch.zeros(V, 1 << 15).index_add_(0, ids[there], g.cpu()[there].float()).to(dtype)
+        assert torch.equal(ops.embedding_grad_raw(g, ids.to(cuda), V).cpu(), want)
+    D = 1 << 20
+    x, gate = (torch.randn(5, D, generator=gen).to(dtype).to(cuda) for _ in range(2))
+    h, last = ops.gated_scan(x, gate, torch.tensor([0, 3, 5], dtype=torch.int32, device=cuda))
+    for cols in (slice(0, 64), slice(D - 64, D)):
+        c, cl = ops.gated_scan(x[:, cols], gate[:, cols], torch.tensor([0, 3, 5], dtype=torch.int32, device=cuda))
+        assert torch.equal(h[:, cols], c) and torch.equal(last[:, cols], cl)
+    s, new = ops.gated_scan_step(x, gate, torch.ones(5, D, device=cuda))
+    c, cn = ops.gated_scan_step(x[:, -64:], gate[:, -64:], torch.ones(5, 64, device=cuda))
+    assert torch.equal(s[:, -64:], c) and torch.equal(new[:, -64:], cn)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("D", [3, 33, 64, 130])
+def test_pitched_outputs_of_the_entry_points(cuda, D, dtype):
+    """Outputs with a row pitch, which only the C entry points offer: the same bits, and nothing between the rows is written."""
+    from building_gan_amd import _lib, ops
+    lib, s = _lib.load(), _lib.stream()
+    code, N, P = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}[dtype], 700, D + 5
+    ptr = [0, 0, 1, 300, 690]
+    c = scan_case(N, D, ptr, dtype, D)
+    x, gate, h0, dh, dl = c["x"].to(cuda).contiguous(), c["gate"].to(cuda).contiguous(), c["h0"].to(cuda), c["dh"].to(cuda), c["dlast"].to(cuda)
+    rp = torch.tensor(ptr, dtype=torch.int32, device=cuda)
+    size = lib.bg_gated_scan_workspace(N, D)
+    ws = torch.empty(size, dtype=torch.uint8, device=cuda)
+
+    def out(n):                                              # rows D wide, one element off the buffer's start, all sevens
+        buf = torch.full((n * P + 8,), 7.0, dtype=dtype, device=cuda)
+        return buf, buf[1:1 + n * P].view(n, P)[:, :D]
+
+    def rest_is_seven(buf, view):
+        view.fill_(7.0)
+        return bool((buf == 7.0).all())
+
+    for rev in (0, 1):
+        h, last, heads = ops.gated_scan_raw(x, gate, rp, h0, bool(rev), keep_heads=True)
+        dx, dg, d0 = ops.gated_scan_grad_raw(x, gate, rp, h0, bool(rev), heads, dh, dl)
+        (b1, v1), (b2, v2), (b3, v3) = out(N), out(N), out(N)
+        assert lib.bg_gated_scan_fwd(code, x.data_ptr(), D, gate.data_ptr(), D, rp.data_ptr(), 4, N, D, h0.data_ptr(), rev, v1.data_ptr(), P,
+                                     None, None, ws.data_ptr(), size, s) == 0                        # without h_last and heads
+        assert lib.bg_gated_scan_bwd(code, x.data_ptr(), D, gate.data_ptr(), D, dh.data_ptr(), D, dl.data_ptr(), rp.data_ptr(), 4, N, D,
+                                     h0.data_ptr(), rev, heads.data_ptr(), v2.data_ptr(), P, v3.data_ptr(), P, None, ws.data_ptr(), size, s) == 0
+        assert torch.equal(v1, h) and torch.equal(v2, dx) and torch.equal(v3, dg)
+        assert rest_is_seven(b1, v1) and rest_is_seven(b2, v2) and rest_is_seven(b3, v3)
+    state = torch.randn(N, D, device=cuda)
+    want, new = ops.gated_scan_step(x, gate, state)
+    b, v = out(N)
+    assert lib.bg_gated_scan_step(code, x.data_ptr(), D, gate.data_ptr(), D, state.data_ptr(), D, N, D, v.data_ptr(), P, state.data_ptr(), D, s) == 0
+    assert torch.equal(v, want) and torch.equal(state, new) and rest_is_seven(b, v)
+    ids = torch.randint(-1, N, (N,), device=cuda)
+    b, v = out(N)
+    assert lib.bg_embedding_fwd(code, x.data_ptr(), D, N, ids.data_ptr(), 1, N, D, 2.0, v.data_ptr(), P, s) == 0
+    assert torch.equal(v, ops.embedding(x, ids, 2.0)) and rest_is_seven(b, v)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("reverse", [False, True])
+def test_row_pointers_past_the_rows_end_there(cuda, reverse):
+    """Entries outside [0, rows] count as the nearer end."""
+    c = scan_case(460, 20, [0, 100, 460, 460], torch.float32, 5)
+    a = check_scan(cuda, c, [0, 100, 460, 460], reverse)
+    b = check_scan_values(cuda, c, [-7, 100, 461, 2 ** 31 - 1], reverse)
+    assert all(torch.equal(p, q) for p, q in zip(a, b))
+
+
+def check_scan_values(cuda, c, ptr, reverse):
+    from building_gan_amd import ops
+    x, gate, h0 = (c[k].to(cuda).requires_grad_(True) for k in ("x", "gate", "h0"))
+    h, hl = ops.gated_scan(x, gate, torch.tensor(ptr, dtype=torch.int32, device=cuda), h0, reverse)
+    return (h, hl) + torch.autograd.grad((h, hl), (x, gate, h0), (c["dh"].to(cuda), c["dlast"].to(cuda)))
+
+
+@pytest.mark.gpu
+def test_small_tables_captured_and_replayed(cuda):
+    """The sums of tables of up to 20 rows (above 16 they ask for more LDS than a kernel has by itself), no tokens, one-workgroup
+    and many-workgroup sorts: captured, and replayed on changing inputs."""
+    from building_gan_amd import ops
+    cases = [(7, 24, 900), (17, 130, 5000), (20, 3, 4000), (20, 64, 0), (300, 64, 0), (300, 33, 4000), (90000, 8, 9000)]
+    gen = torch.Generator(device=cuda).manual_seed(4)
+    ids = [torch.zeros(n, dtype=torch.int32, device=cuda) for _, _, n in cases]
+    g = [torch.zeros(n, D, device=cuda) for _, D, n in cases]
+
+    def fill():
+        for (V, _, n), i, gg in zip(cases, ids, g):
+            if n:
+                i.copy_(torch.randint(-1, V + 1, (n,), generator=gen, device=cuda))
+                gg.copy_(torch.randn(gg.shape, generator=gen, device=cuda))
+
+    def passes():
+        return [ops.embedding_grad_raw(gg, i, V, 0.5) for (V, _, _), i, gg in zip(cases, ids, g)]
+
+    fill()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        passes()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = passes()
+    for k in range(4):
+        fill()
+        for t in outs:
+            t.fill_(float("nan"))
+        graph.replay()
+        if k % 2:
+            torch.cuda.synchronize()
+        for a, b in zip([t.clone() for t in outs], passes()):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_saved_tensors_kept_elsewhere_and_a_graph_used_twice(cuda):
+    """Operands saved on the host and brought back, one backward pass run twice over a kept graph, a checkpointed call: the same
+    gradients; an operand changed in between is an error."""
+    from torch.utils.checkpoint import checkpoint
+    from building_gan_amd import ops
+    ptr = torch.tensor([0, 33, 200], dtype=torch.int32, device=cuda)
+    z = torch.randn(200, 40, device=cuda, requires_grad=True)
+    h0 = torch.randn(2, 20, device=cuda, requires_grad=True)
+    w = torch.randn(30, 40, device=cuda, requires_grad=True)
+    ids = torch.randint(0, 30, (200,), device=cuda)
+
+    def f(z, h0, w):
+        y = ops.embedding(w, ids) + z
+        h, last = ops.gated_scan(y[:, :20], y[:, 20:], ptr, h0)
+        return (h * h).sum() + last.sum()
+
+    loss = f(z, h0, w)
+    want = torch.autograd.grad(loss, (z, h0, w), retain_graph=True)
+    again = torch.autograd.grad(loss, (z, h0, w))
+    with torch.autograd.graph.save_on_cpu():
+        loss = f(z, h0, w)
+    host = torch.autograd.grad(loss, (z, h0, w))
+    ck = torch.autograd.grad(checkpoint(f, z, h0, w, use_reentrant=False), (z, h0, w))
+    for got in (again, host, ck):
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    x, gate = torch.randn(50, 8, device=cuda), torch.randn(50, 8, device=cuda, requires_grad=True)
+    h, _ = ops.gated_scan(x, gate)
+    x.zero_()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        h.sum().backward()
