@@ -836,7 +836,7 @@ def test_two_captured_graphs_replayed_at_once(cuda):
 @pytest.fixture
 def no_launch(monkeypatch):
     """The wrappers on CPU tensors with every launch left out (results are whatever the memory held): what they do before and
-    after one.  Yields the calls made, as (entry point, arguments)."""
+    after one.  Returns the list of the calls made, as (entry point, arguments)."""
     from building_gan_amd import _lib, ops
     real, calls = _lib.load(), []
 
